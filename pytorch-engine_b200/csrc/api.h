@@ -329,6 +329,19 @@ int pe_rmsnorm_pair_mix_dyt_add(int dtype, const void* a, const void* b, const f
     void* out, int n_rows, int dim, cudaStream_t stream);
 int pe_concat_split(int dtype, const float* a, const float* b, void* hi, void* lo, int n_rows, int dim, cudaStream_t stream);
 
+// quantize_fp8.cu
+int pe_quantize_rows_fp8(int dtype, const void* x, long long x_ld, const int* row_map, const int* n_live, void* values,
+    long long v_ld, float* scales, long long s_ld, int M, int K, int x_rows, int* status, cudaStream_t stream);
+int pe_quantize_weight_fp8(int dtype, const void* w, long long w_ld, void* values, long long v_ld, float* scales, int N, int K,
+    cudaStream_t stream);
+int pe_rmsnorm_residual_fp8(float* residual, const void* delta, const float* weight, void* values, long long v_ld, float* scales,
+    long long s_ld, int n_rows, int dim, float eps, cudaStream_t stream);
+
+// gemm_fp8.cu
+int pe_gemm_fp8(const void* x, long long x_ld, const float* x_scales, long long xs_ld, const void* w, long long w_ld,
+    const float* w_scales, void* y, long long ldy, int M, int N, int K, int out_f32, int kind, float limit, float alpha,
+    const float* bias, const float* row_weight, const int* offsets, int n_groups, int* status, cudaStream_t stream);
+
 // wait_probe.cu
 int pe_wait_probe(unsigned long long* out, int polls, cudaStream_t stream);
 long long pe_wait_limit_polls();

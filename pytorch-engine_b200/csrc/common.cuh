@@ -23,6 +23,7 @@ enum StatusCode : int {
   kStatusPositionOutOfRange = 3,// position beyond the tables or the page table
   kStatusWaitTimedOut = 4,      // a bounded wait (mbarrier / TMA / MMA commit) ran out
   kStatusSlotOutOfRange = 5,
+  kStatusRowOutOfRange = 6,     // a row map names a row outside its tensor
 };
 
 __device__ __forceinline__ void report(int* status, int code, int a = 0, int b = 0, int c = 0) {

@@ -1,0 +1,285 @@
+// Rows and matrices to 8-bit floating point (e4m3: 4 exponent bits, 3 mantissa bits, largest value 448) with one scale for
+// each block: 128 neighbouring features of a row, or 128 x 128 elements of a weight matrix.
+//
+//   a = max |x| over the block ;  s = the smallest 2^e (e >= -126) with a <= 448 * 2^e ;  q = e4m3(x / s)
+//
+// The scale is a power of two: x / s is then exact, so a block's values do not depend on how a quotient is rounded, and a
+// power of two costs e4m3 nothing but its smallest values (its relative precision is the same in every binade).  A NaN stays a
+// NaN and does not count for the block's maximum; an infinity becomes a NaN (e4m3 has none), and with it the block's scale is 2^120.
+//
+// Scales of rows are stored by block, [blocks, rows]: the products (gemm_fp8.cu) read one block's scales of many rows at a time.
+#include "api.h"
+#include "common.cuh"
+#include <cuda_fp8.h>
+
+namespace pe {
+namespace quant8 {
+
+constexpr int BLOCK = 128;      // features of a block
+
+// The scale's bits for the largest magnitude `a` of a block: 448 = 1.75 * 2^8.
+__device__ __forceinline__ uint32_t scale_bits(float a) {
+  const uint32_t b = __float_as_uint(a);
+  const int e = (int)(b >> 23) - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return (uint32_t)max(e, 1) << 23;
+}
+// 1 / s, a power of two itself
+__device__ __forceinline__ float inverse_of(uint32_t scale) { return __uint_as_float((254u << 23) - scale); }
+
+__device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+  return lo | (hi << 16);
+}
+__device__ __forceinline__ float no_infinity(float x) { return fabsf(x) == INFINITY ? __uint_as_float(0x7fffffffu) : x; }
+
+// Eight neighbouring features of a row from column `c`, zeros behind the row's end.
+template <typename T>
+__device__ __forceinline__ void load8(const T* row, int c, int K, bool vec, float (&v)[8]) {
+  if (vec && c + 8 <= K) {
+    if (sizeof(T) == 4) {
+      const float4 a = *reinterpret_cast<const float4*>(row + c), b = *reinterpret_cast<const float4*>(row + c + 4);
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+      const uint4 u = *reinterpret_cast<const uint4*>(row + c);
+      const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = __bfloat1622float2(h[i]);
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = c + i < K ? to_f32<T>(row[c + i]) : 0.f;
+  }
+}
+__device__ __forceinline__ float max8(const float (&v)[8]) {
+  float m = fabsf(v[0]);
+#pragma unroll
+  for (int i = 1; i < 8; ++i) m = fmaxf(m, fabsf(v[i]));
+  return m;
+}
+// Rows of values start on 16-byte boundaries, so eight of them at a multiple of eight are one store.
+__device__ __forceinline__ void store8(uint8_t* row, int c, int K, float (&v)[8], uint32_t scale, float a) {
+  if (a == INFINITY) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = no_infinity(v[i]);
+  }
+  const float inv = inverse_of(scale);
+  uint2 q;
+  q.x = pack4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+  q.y = pack4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
+  if (c + 8 <= K) {
+    *reinterpret_cast<uint2*>(row + c) = q;
+  } else {
+    const uint8_t* b = reinterpret_cast<const uint8_t*>(&q);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (c + i < K) row[c + i] = b[i];
+  }
+}
+
+// Sixteen lanes a block of 128 features, sixteen rows a thread block (so that the scales, which lie by block, leave it 64
+// bytes at a time), U blocks of each row with their loads in flight together.  `row_map`: output row r is input row row_map[r];
+// `n_live` (on the device): only so many rows are there.
+template <typename T, int U>
+__global__ void __launch_bounds__(256) quantize_rows_kernel(const T* x, long long x_ld, const int* row_map,
+                                                            const int* n_live, uint8_t* values, long long v_ld, float* scales, long long s_ld, int M, int K,
+                                                            int x_rows, bool vec, int* status) {
+  pdl_wait_block();
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 15;
+  const int r = blockIdx.y * 16 + (threadIdx.x >> 4);
+  const int kb0 = blockIdx.x * U, blocks = (K + BLOCK - 1) / BLOCK;
+  // all 32 lanes take part in the shuffles: rows beyond the last are not read and not written
+  int src = -1;
+  if (n_live) M = min(M, *n_live);
+  if (r < M) {
+    src = row_map ? row_map[r] : r;
+    if (src < 0 || src >= x_rows) {
+      if (lane == 0 && kb0 == 0) report(status, kStatusRowOutOfRange, r, src, x_rows);
+      src = -1;
+    }
+  }
+  const T* row = x + (size_t)max(src, 0) * x_ld;
+  float v[U][8], a[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) load8<T>(row, (kb0 + u) * BLOCK + lane * 8, src < 0 ? 0 : K, vec, v[u]);
+#pragma unroll
+  for (int u = 0; u < U; ++u) a[u] = max8(v[u]);
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) a[u] = fmaxf(a[u], __shfl_xor_sync(0xffffffffu, a[u], o));
+  if (src < 0) return;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (kb0 + u >= blocks) break;
+    const uint32_t s = scale_bits(a[u]);
+    store8(values + (size_t)r * v_ld, (kb0 + u) * BLOCK + lane * 8, K, v[u], s, a[u]);
+    if (lane == 0) scales[(size_t)(kb0 + u) * s_ld + r] = __uint_as_float(s);
+  }
+}
+
+// One thread block for 128 x 128 elements, which it holds in registers between the maximum and the conversion.  Its successor
+// in the stream may not start early: it may be a product that asks for these values before it waits.
+template <typename T>
+__global__ void __launch_bounds__(256) quantize_weight_kernel(const T* w, long long w_ld, uint8_t* values, long long v_ld,
+                                                              float* scales, int N, int K, bool vec) {
+  __shared__ float red[32];
+  pdl_wait_block();
+  const int blocks = (K + BLOCK - 1) / BLOCK;
+  const int rb = blockIdx.x / blocks, kb = blockIdx.x - rb * blocks;
+  const int c = kb * BLOCK + (threadIdx.x & 15) * 8;
+  float v[8][8];
+  float a = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = rb * BLOCK + i * 16 + (threadIdx.x >> 4);
+    load8<T>(w + (size_t)min(r, N - 1) * w_ld, c, r < N ? K : 0, vec, v[i]);
+    a = fmaxf(a, max8(v[i]));
+  }
+  a = block_max(a, red);
+  const uint32_t s = scale_bits(a);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = rb * BLOCK + i * 16 + (threadIdx.x >> 4);
+    if (r < N) store8(values + (size_t)r * v_ld, c, K, v[i], s, a);
+  }
+  if (threadIdx.x == 0) scales[blockIdx.x] = __uint_as_float(s);
+}
+
+// rmsnorm.cu's norm (with its residual add) whose result, rounded to bfloat16, is quantised on the way out: what rmsnorm.cu's
+// kernel and the one above would give, without the bfloat16 rows between them.  A warp's 32 x 4 features are one block.
+__global__ void __launch_bounds__(1024) rmsnorm_residual_fp8_kernel(float* residual, const __nv_bfloat16* delta,
+                                                                    const float* __restrict__ weight, uint8_t* values,
+                                                                    long long v_ld, float* scales, long long s_ld, int dim,
+                                                                    float eps) {
+  extern __shared__ float row_buf[];  // dim floats
+  __shared__ float red[32];
+  const int c0 = threadIdx.x * 4;
+  float4 w0 = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (c0 < dim) w0 = *reinterpret_cast<const float4*>(weight + c0);   // the weight does not come from the kernel before this one
+  pdl_wait_block();
+  pdl_launch_dependents();
+  const int r = blockIdx.x;
+  float* res_row = residual + (size_t)r * dim;
+  const __nv_bfloat16* d_row = delta ? delta + (size_t)r * dim : nullptr;
+  float ss = 0.f;
+  for (int c = c0; c < dim; c += blockDim.x * 4) {
+    float4 h = *reinterpret_cast<const float4*>(res_row + c);
+    if (d_row) {
+      const uint2 u = *reinterpret_cast<const uint2*>(d_row + c);
+      const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.x));
+      const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.y));
+      h.x += a.x; h.y += a.y; h.z += b.x; h.w += b.y;
+      *reinterpret_cast<float4*>(res_row + c) = h;
+    }
+    *reinterpret_cast<float4*>(row_buf + c) = h;
+    ss += h.x * h.x + h.y * h.y + h.z * h.z + h.w * h.w;
+  }
+  const float inv = rsqrtf(block_sum(ss, red) / (float)dim + eps);
+  // whole warps stay in the loop for the shuffles
+  for (int c = c0; c - (int)(threadIdx.x & 31) * 4 < dim; c += blockDim.x * 4) {
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (c < dim) {
+      const float4 h = *reinterpret_cast<const float4*>(row_buf + c);
+      const float4 w = c == c0 ? w0 : *reinterpret_cast<const float4*>(weight + c);
+      const float2 lo = __bfloat1622float2(__floats2bfloat162_rn(h.x * inv * w.x, h.y * inv * w.y));
+      const float2 hi = __bfloat1622float2(__floats2bfloat162_rn(h.z * inv * w.z, h.w * inv * w.w));
+      y = make_float4(lo.x, lo.y, hi.x, hi.y);
+    }
+    const float a = warp_max(fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))));
+    if (c >= dim) continue;
+    const uint32_t s = scale_bits(a);
+    const float by = inverse_of(s);
+    if (a == INFINITY) y = make_float4(no_infinity(y.x), no_infinity(y.y), no_infinity(y.z), no_infinity(y.w));
+    *reinterpret_cast<uint32_t*>(values + (size_t)r * v_ld + c) = pack4(y.x * by, y.y * by, y.z * by, y.w * by);
+    if ((threadIdx.x & 31) == 0) scales[(size_t)(c / BLOCK) * s_ld + r] = __uint_as_float(s);
+  }
+}
+
+template <typename T>
+static int launch_rows(const T* x, long long x_ld, const int* row_map, const int* n_live, uint8_t* values, long long v_ld, float* scales,
+                       long long s_ld, int M, int K, int x_rows, int* status, cudaStream_t stream) {
+  const bool vec = ((uintptr_t)x % 16) == 0 && (x_ld * (long long)sizeof(T)) % 16 == 0;
+  const int blocks = (K + BLOCK - 1) / BLOCK, row_blocks = (M + 15) / 16;
+  // four blocks of a row a thread block where that still leaves every SM several thread blocks
+  const bool many = (long long)row_blocks * blocks >= 4LL * 8 * kSMs;
+  const dim3 grid(many ? (blocks + 3) / 4 : blocks, row_blocks);
+  cudaError_t e = many ? launch(quantize_rows_kernel<T, 4>, grid, dim3(256), 0, stream, x, x_ld, row_map, n_live, values, v_ld, scales, s_ld, M, K, x_rows, vec, status)
+                       : launch(quantize_rows_kernel<T, 1>, grid, dim3(256), 0, stream, x, x_ld, row_map, n_live, values, v_ld, scales, s_ld, M, K, x_rows, vec, status);
+  if (e != cudaSuccess) return (int)e;
+  PE_LAUNCH_CHECK();
+  return PE_OK;
+}
+
+}  // namespace quant8
+}  // namespace pe
+
+// values[r] (M rows, v_ld bytes apart, a multiple of 16, on 16-byte boundaries), scales[b * s_ld + r]; row r is row row_map[r] of x
+// (row_map null: r), which has x_rows rows x_ld elements apart.  n_live (or null): only the first *n_live rows are there.
+extern "C" int pe_quantize_rows_fp8(int dtype, const void* x, long long x_ld, const int* row_map, const int* n_live, void* values, long long v_ld,
+                                    float* scales, long long s_ld, int M, int K, int x_rows, int* status, cudaStream_t stream) {
+  using namespace pe::quant8;
+  if (M < 0 || K < 0) return PE_ERR_BAD_ARGUMENT;
+  if (M == 0 || K == 0) return PE_OK;
+  if (x == nullptr || values == nullptr || scales == nullptr || x_ld < K || v_ld < K || s_ld < M || x_rows < 1 || (!row_map && M > x_rows))
+    return PE_ERR_BAD_ARGUMENT;
+  if (((uintptr_t)values % 16) || (v_ld % 16)) return PE_ERR_BAD_ARGUMENT;
+  if ((M + 15) / 16 > 65535) return PE_ERR_UNSUPPORTED_SIZE;
+  if (dtype == PE_BF16) return launch_rows((const __nv_bfloat16*)x, x_ld, row_map, n_live, (uint8_t*)values, v_ld, scales, s_ld, M, K, x_rows, status, stream);
+  if (dtype == PE_F32) return launch_rows((const float*)x, x_ld, row_map, n_live, (uint8_t*)values, v_ld, scales, s_ld, M, K, x_rows, status, stream);
+  return PE_ERR_UNSUPPORTED_DTYPE;
+}
+
+// values as above (N rows), scales[rb * ceil(K / 128) + kb].
+extern "C" int pe_quantize_weight_fp8(int dtype, const void* w, long long w_ld, void* values, long long v_ld, float* scales, int N,
+                                      int K, cudaStream_t stream) {
+  using namespace pe::quant8;
+  if (N < 0 || K < 0) return PE_ERR_BAD_ARGUMENT;
+  if (N == 0 || K == 0) return PE_OK;
+  if (w == nullptr || values == nullptr || scales == nullptr || w_ld < K || v_ld < K) return PE_ERR_BAD_ARGUMENT;
+  if (((uintptr_t)values % 16) || (v_ld % 16)) return PE_ERR_BAD_ARGUMENT;
+  const long long cells = (long long)((N + BLOCK - 1) / BLOCK) * ((K + BLOCK - 1) / BLOCK);
+  if (cells > 0x7fffffffLL) return PE_ERR_UNSUPPORTED_SIZE;
+  cudaError_t e;
+  if (dtype == PE_BF16) {
+    const bool vec = ((uintptr_t)w % 16) == 0 && (w_ld * 2) % 16 == 0;
+    e = pe::launch(quantize_weight_kernel<__nv_bfloat16>, dim3((unsigned)cells), dim3(256), 0, stream, (const __nv_bfloat16*)w, w_ld, (uint8_t*)values, v_ld, scales, N, K, vec);
+  } else if (dtype == PE_F32) {
+    const bool vec = ((uintptr_t)w % 16) == 0 && (w_ld * 4) % 16 == 0;
+    e = pe::launch(quantize_weight_kernel<float>, dim3((unsigned)cells), dim3(256), 0, stream, (const float*)w, w_ld, (uint8_t*)values, v_ld, scales, N, K, vec);
+  } else {
+    return PE_ERR_UNSUPPORTED_DTYPE;
+  }
+  if (e != cudaSuccess) return (int)e;
+  PE_LAUNCH_CHECK();
+  return PE_OK;
+}
+
+// Rows of residual (float32) and delta (bfloat16 or null) are packed; dim a multiple of 4, at most 51,200 (a row lies in shared memory).
+extern "C" int pe_rmsnorm_residual_fp8(float* residual, const void* delta, const float* weight, void* values, long long v_ld,
+                                       float* scales, long long s_ld, int n_rows, int dim, float eps, cudaStream_t stream) {
+  using namespace pe::quant8;
+  if (n_rows < 0 || dim < 1) return PE_ERR_BAD_ARGUMENT;
+  if (n_rows == 0) return PE_OK;
+  if (residual == nullptr || weight == nullptr || values == nullptr || scales == nullptr || v_ld < dim || s_ld < n_rows) return PE_ERR_BAD_ARGUMENT;
+  const size_t smem = (size_t)dim * sizeof(float);
+  if (dim % 4 || smem > 200 * 1024) return PE_ERR_UNSUPPORTED_SIZE;
+  if (((uintptr_t)values % 16) || (v_ld % 16) || ((uintptr_t)residual % 16) || ((uintptr_t)weight % 16) || ((uintptr_t)delta % 8)) return PE_ERR_BAD_ARGUMENT;
+  // threads as for rmsnorm.cu's kernel, whose sums these are
+  int threads = dim >= 2048 ? 512 : (dim >= 512 ? 256 : 128);
+  if (n_rows <= 64 && dim > 2048) threads = 1024;
+  cudaError_t e;
+  if (smem > 48 * 1024) {
+    e = cudaFuncSetAttribute(rmsnorm_residual_fp8_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return (int)e;
+  }
+  e = pe::launch(rmsnorm_residual_fp8_kernel, dim3(n_rows), dim3(threads), smem, stream, residual, (const __nv_bfloat16*)delta, weight, (uint8_t*)values, v_ld, scales, s_ld, dim, eps);
+  if (e != cudaSuccess) return (int)e;
+  PE_LAUNCH_CHECK();
+  return PE_OK;
+}

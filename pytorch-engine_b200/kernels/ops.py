@@ -1475,3 +1475,150 @@ def layernorm(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor, eps: flo
     check(library().pe_layernorm(dtype_tag(x.dtype), _ptr(x), _ptr(weight), _ptr(out), x.numel() // dim, dim, float(eps), _stream()),
           "layernorm")
     _count(1)
+
+
+# ---- 8-bit floating point in blocks of 128 ---------------------------------------------------------------------------
+FP8 = torch.float8_e4m3fn
+FP8_BLOCK = 128         # features of a row, or features and rows of a matrix, that share a scale
+
+
+def fp8_blocks(n: int) -> int:
+    return -(-n // FP8_BLOCK)
+
+
+def _fp8_ld(t: torch.Tensor, what: str) -> int:
+    """Bytes between the rows of ``t [rows, K]``; one row may start anywhere 16 divides."""
+    rows, width = t.shape
+    _need(t.dtype == FP8 and (t.stride(1) == 1 or width == 1), f"{what}: float8_e4m3fn rows of neighbouring values")
+    if rows <= 1:
+        return (width + 15) // 16 * 16
+    _need(t.stride(0) % 16 == 0, f"{what}: rows must lie a multiple of 16 bytes apart")
+    return t.stride(0)
+
+
+def _fp8_scales_ld(scales: torch.Tensor, blocks: int, rows: int, what: str) -> int:
+    _need(scales.dtype == torch.float32 and scales.dim() == 2 and scales.shape[0] == blocks and scales.shape[1] == rows
+          and (scales.stride(1) == 1 or rows == 1), f"{what}: scales [blocks of {FP8_BLOCK} features, rows] float32")
+    return max(scales.stride(0), rows) if blocks > 1 else rows
+
+
+def _on_current(what: str, *tensors) -> None:
+    here = _current_device()
+    for t in tensors:
+        _need(t is None or t.get_device() == here, f"{what}: tensors must lie on the current CUDA device")
+
+
+def quantize_rows_fp8(x: torch.Tensor, values: torch.Tensor, scales: torch.Tensor, row_map: Optional[torch.Tensor] = None,
+                      live: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> None:
+    """``x [rows, K]`` (bfloat16 or float32) to e4m3 ``values [M, K]`` and ``scales [fp8_blocks(K), M]``, one for 128 features of a
+    row (csrc/quantize_fp8.cu).  ``row_map`` (int32 ``[M]``): row r of the result is row ``row_map[r]`` of ``x``; a row outside ``x``
+    is left as it is and reported in ``status``.  ``live`` (int32, one number on the device): only so many rows are there."""
+    _need(x.dim() == 2 and values.dim() == 2 and (x.stride(1) == 1 or x.shape[1] == 1), "quantize_rows_fp8: matrices of neighbouring features")
+    m, k = values.shape
+    _need(x.shape[1] == k and (row_map is not None or x.shape[0] == m), "quantize_rows_fp8: shapes do not match")
+    _need(row_map is None or (row_map.dtype == torch.int32 and row_map.is_contiguous() and row_map.numel() == m and status is not None),
+          "quantize_rows_fp8: row_map int32, one per row, with a status word")
+    _need(live is None or (live.dtype == torch.int32 and live.numel() >= 1), "quantize_rows_fp8: live is one int32")
+    v_ld, s_ld = _fp8_ld(values, "quantize_rows_fp8"), _fp8_scales_ld(scales, fp8_blocks(k), m, "quantize_rows_fp8")
+    _on_current("quantize_rows_fp8", x, values, scales, row_map, live)
+    if m == 0 or k == 0:
+        return
+    check(library().pe_quantize_rows_fp8(dtype_tag(x.dtype), _ptr(x), x.stride(0) if x.shape[0] > 1 else k, _ptr(row_map), _ptr(live),
+                                         _ptr(values), v_ld, _ptr(scales), s_ld, m, k, x.shape[0], _ptr(status), _stream()),
+          "quantize_rows_fp8")
+    _count(1)
+
+
+def quantize_weight_fp8(w: torch.Tensor, values: torch.Tensor, scales: torch.Tensor) -> None:
+    """A matrix ``w [N, K]`` (bfloat16 or float32) to e4m3 ``values [N, K]`` and ``scales [fp8_blocks(N), fp8_blocks(K)]``, one for
+    128 x 128 elements (csrc/quantize_fp8.cu)."""
+    _need(w.dim() == 2 and w.shape == values.shape and (w.stride(1) == 1 or w.shape[1] == 1), "quantize_weight_fp8: matrices of one shape")
+    n, k = w.shape
+    v_ld = _fp8_ld(values, "quantize_weight_fp8")
+    _need(scales.dtype == torch.float32 and scales.is_contiguous() and tuple(scales.shape) == (fp8_blocks(n), fp8_blocks(k)),
+          f"quantize_weight_fp8: scales [blocks of {FP8_BLOCK} rows, blocks of {FP8_BLOCK} features] float32")
+    _on_current("quantize_weight_fp8", w, values, scales)
+    if n == 0 or k == 0:
+        return
+    check(library().pe_quantize_weight_fp8(dtype_tag(w.dtype), _ptr(w), w.stride(0) if n > 1 else k, _ptr(values), v_ld, _ptr(scales),
+                                           n, k, _stream()), "quantize_weight_fp8")
+    _count(1)
+
+
+def rmsnorm_residual_fp8_supported(dim: int) -> bool:
+    """Whether csrc/quantize_fp8.cu has the norm and the conversion in one kernel."""
+    return dim % 4 == 0 and dim <= 51200
+
+
+def rmsnorm_residual_fp8(residual: torch.Tensor, delta: Optional[torch.Tensor], weight: torch.Tensor, values: torch.Tensor,
+                         scales: torch.Tensor, eps: float) -> None:
+    """``rmsnorm_residual`` with bfloat16 rows, then ``quantize_rows_fp8`` of what it gives, in one kernel: the stream gets its
+    ``delta`` (bfloat16) added, the normed rows exist as e4m3 only."""
+    n, dim = residual.shape
+    _need(residual.dtype == torch.float32 and weight.dtype == torch.float32 and residual.is_contiguous() and weight.is_contiguous()
+          and weight.numel() == dim, "rmsnorm_residual_fp8: stream and weight float32")
+    _need(delta is None or (delta.dtype == torch.bfloat16 and delta.is_contiguous() and delta.shape == residual.shape),
+          "rmsnorm_residual_fp8: delta must be bfloat16 of the stream's shape")
+    _need(tuple(values.shape) == (n, dim), "rmsnorm_residual_fp8: values must have the stream's shape")
+    v_ld, s_ld = _fp8_ld(values, "rmsnorm_residual_fp8"), _fp8_scales_ld(scales, fp8_blocks(dim), n, "rmsnorm_residual_fp8")
+    _on_current("rmsnorm_residual_fp8", residual, delta, weight, values, scales)
+    check(library().pe_rmsnorm_residual_fp8(_ptr(residual), _ptr(delta), _ptr(weight), _ptr(values), v_ld, _ptr(scales), s_ld, n, dim,
+                                            float(eps), _stream()), "rmsnorm_residual_fp8")
+    _count(1)
+
+
+def _gemm_fp8(what: str, x, x_scales, w, w_scales, out, status, glu, offsets, row_weight) -> None:
+    m, k = x.shape
+    n = out.shape[1]
+    groups = 0
+    if offsets is not None:
+        groups = w.shape[0]
+        _need(w.dim() == 3 and groups >= 1 and offsets.dtype == torch.int32 and offsets.is_contiguous() and offsets.numel() == groups + 1,
+              f"{what}: offsets int32, one more than the groups of w")
+        _need(w.stride(0) == w.shape[1] * w.stride(1) or groups == 1, f"{what}: the groups' matrices must follow each other")
+        _need(w_scales.shape[0] == groups, f"{what}: scales for each group")
+        rows = w.shape[1]
+    else:
+        _need(w.dim() == 2, f"{what}: w is a matrix")
+        rows = w.shape[0]
+    _need(w.shape[-1] == k and rows == (n if glu is None else 2 * n) and out.dim() == 2 and out.shape[0] == m and (out.stride(1) == 1 or n == 1),
+          f"{what}: shapes do not match")
+    _need(out.dtype == torch.bfloat16 or (out.dtype == torch.float32 and glu is None), f"{what}: out bfloat16 (or float32 without an activation)")
+    x_ld = _fp8_ld(x, what)
+    w2 = w if offsets is None else w.view(groups * rows, k) if w.is_contiguous() else w.as_strided((groups * rows, k), (w.stride(1), w.stride(2)))
+    w_ld = _fp8_ld(w2, what)
+    _need(w_scales.dtype == torch.float32 and w_scales.is_contiguous() and tuple(w_scales.shape[-2:]) == (fp8_blocks(rows), fp8_blocks(k)),
+          f"{what}: scales of w [blocks of {FP8_BLOCK} rows, blocks of {FP8_BLOCK} features] float32")
+    xs_ld = _fp8_scales_ld(x_scales, fp8_blocks(k), m, what)
+    _need(row_weight is None or (glu is not None and row_weight.dtype == torch.float32 and row_weight.is_contiguous() and row_weight.numel() >= m),
+          f"{what}: row_weight float32, one per row, before an activation")
+    _on_current(what, x, x_scales, w, w_scales, out, offsets, row_weight, status)
+    if m == 0 or n == 0:
+        return
+    kind, limit, alpha, bias = (0, 0.0, 1.0, None) if glu is None else _glu_args(glu or None, n)
+    check(library().pe_gemm_fp8(_ptr(x), x_ld, _ptr(x_scales), xs_ld, _ptr(w), w_ld, _ptr(w_scales), _ptr(out),
+                                out.stride(0) if m > 1 else n, m, n, k, 1 if out.dtype == torch.float32 else 0, kind, limit, alpha, bias,
+                                _ptr(row_weight), _ptr(offsets), groups, _ptr(status), _stream()), what)
+    _count(1)
+
+
+def gemm_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor,
+             status: torch.Tensor, glu=None) -> None:
+    """``out[m, n] = sum_b x_scales[b, m] * w_scales[n // 128, b] * sum_{k in block b} x[m, k] w[n, k]`` of e4m3 ``x [M, K]`` and
+    ``w [N, K]`` (csrc/gemm_fp8.cu), summed in float32; ``out`` bfloat16 or float32.  Rows of ``x`` and ``w`` lie a multiple of 16
+    bytes apart and start on such boundaries.
+
+    ``glu``: ``w`` holds gate rows, then as many up rows (``out [M, N / 2]``, bfloat16), and ``out = act(gate, up)``; ``()`` is SiLU,
+    else (kind of ``GLU_KINDS``, limit, alpha, float32 bias ``[N]`` or None).
+
+    ``w`` is a weight: the kernel starts to read it while the one launched before it is still running, so that one must
+    not be what writes it (``quantize_weight_fp8`` may be: it lets nothing start early)."""
+    _gemm_fp8("gemm_fp8", x, x_scales, w, w_scales, out, status, glu, None, None)
+
+
+def moe_rows_gemm_fp8(x: torch.Tensor, x_scales: torch.Tensor, offsets: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor,
+                      out: torch.Tensor, status: torch.Tensor, glu=None, row_weight: Optional[torch.Tensor] = None) -> None:
+    """``gemm_fp8`` for rows grouped by expert: rows ``offsets[g] .. offsets[g + 1]`` (int32, on the device) go through ``w[g]`` of ``w
+    [groups, N, K]``, ``w_scales [groups, blocks, blocks]``.  Rows from ``offsets[groups]`` on are left as they are.  ``row_weight``
+    (float32, one per row) multiplies both sums of an output before its activation."""
+    _gemm_fp8("moe_rows_gemm_fp8", x, x_scales, w, w_scales, out, status, glu, offsets, row_weight)

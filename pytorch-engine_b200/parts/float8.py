@@ -1,0 +1,131 @@
+"""Weights and rows in 8-bit floating point, as the products of csrc/gemm_fp8.cu read them.
+
+A matrix is kept as e4m3 values and a float32 scale for each 128 x 128 elements, rows on their way into a product as e4m3
+values and a scale for each 128 features.  What this package quantises itself gets scales that are powers of two
+(csrc/quantize_fp8.cu); a checkpoint's may be any.
+"""
+from __future__ import annotations
+
+from typing import Optional, Sequence
+
+import torch
+
+from ..kernels import ops
+from ..kernels.ops import FP8, FP8_BLOCK, fp8_blocks
+
+
+def _padded_empty(shape, device) -> torch.Tensor:
+    """Uninitialised e4m3 ``[..., K]`` whose rows start on 16-byte boundaries."""
+    *lead, k = shape
+    return torch.empty((*lead, (k + 15) // 16 * 16), dtype=FP8, device=device)[..., :k]
+
+
+class Float8Rows:
+    """``values [M, K]`` (e4m3) and ``scales [fp8_blocks(K), M]`` (float32)."""
+
+    __slots__ = ("values", "scales")
+
+    def __init__(self, values: torch.Tensor, scales: torch.Tensor) -> None:
+        self.values, self.scales = values, scales
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.values.shape
+
+    @property
+    def device(self) -> torch.device:
+        return self.values.device
+
+    @classmethod
+    def empty(cls, rows: int, width: int, device) -> "Float8Rows":
+        return cls(_padded_empty((rows, width), device), torch.empty((fp8_blocks(width), rows), dtype=torch.float32, device=device))
+
+    @classmethod
+    def quantize(cls, x: torch.Tensor, row_map: Optional[torch.Tensor] = None, live: Optional[torch.Tensor] = None,
+                 status: Optional[torch.Tensor] = None) -> "Float8Rows":
+        """``x [rows, K]`` in new storage (``row_map``, ``live``: see ``ops.quantize_rows_fp8``)."""
+        out = cls.empty(x.shape[0] if row_map is None else row_map.numel(), x.shape[1], x.device)
+        ops.quantize_rows_fp8(x, out.values, out.scales, row_map, live, status)
+        return out
+
+    def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        s = self.scales.repeat_interleave(FP8_BLOCK, 0)[:self.values.shape[1]].t()
+        return (self.values.to(torch.float32) * s).to(dtype)
+
+
+class Float8Weight:
+    """``values [N, K]`` (e4m3) and ``scales [fp8_blocks(N), fp8_blocks(K)]`` (float32); or several such matrices stacked in
+    front, ``[G, N, K]`` and ``[G, ...]``.  Rows start on 16-byte boundaries (``aligned`` makes it so)."""
+
+    __slots__ = ("values", "scales")
+    dtype = FP8
+
+    def __init__(self, values: torch.Tensor, scales: torch.Tensor) -> None:
+        if values.dtype != FP8 or scales.dtype != torch.float32:
+            raise ValueError(f"an 8-bit weight is float8_e4m3fn with float32 scales, got {values.dtype} and {scales.dtype}")
+        want = (*values.shape[:-2], fp8_blocks(values.shape[-2]), fp8_blocks(values.shape[-1]))
+        if tuple(scales.shape) != want:
+            raise ValueError(f"an 8-bit weight {list(values.shape)} has scales {list(want)}, got {list(scales.shape)}")
+        self.values, self.scales = values, scales
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.values.shape
+
+    @property
+    def device(self) -> torch.device:
+        return self.values.device
+
+    def nbytes(self) -> int:
+        return self.values.numel() + 4 * self.scales.numel()
+
+    def __getitem__(self, i: int) -> "Float8Weight":
+        """One of several stacked matrices."""
+        return Float8Weight(self.values[i], self.scales[i])
+
+    @classmethod
+    def quantize(cls, w: torch.Tensor) -> "Float8Weight":
+        """A matrix ``[N, K]`` on a CUDA device, quantised into new storage."""
+        values = _padded_empty(w.shape, w.device)
+        scales = torch.empty((fp8_blocks(w.shape[0]), fp8_blocks(w.shape[1])), dtype=torch.float32, device=w.device)
+        ops.quantize_weight_fp8(w, values, scales)
+        return cls(values, scales)
+
+    @classmethod
+    def stack(cls, weights: Sequence["Float8Weight"]) -> "Float8Weight":
+        """Matrices of one shape as one weight ``[G, N, K]``."""
+        first = weights[0]
+        values = _padded_empty((len(weights), *first.shape), first.device)
+        for i, w in enumerate(weights):
+            values[i].copy_(w.values)
+        return cls(values, torch.stack([w.scales for w in weights]).contiguous())
+
+    @staticmethod
+    def stacks_rows(weights: Sequence["Float8Weight"]) -> bool:
+        """Whether ``cat_rows`` keeps every element's block: all but the last must fill their blocks of rows."""
+        return all(w.shape[0] % FP8_BLOCK == 0 for w in weights[:-1])
+
+    @classmethod
+    def cat_rows(cls, weights: Sequence["Float8Weight"]) -> "Float8Weight":
+        """Matrices under each other (see ``stacks_rows``)."""
+        if not cls.stacks_rows(weights):
+            raise ValueError("8-bit weights whose rows end inside a block cannot be put under each other")
+        values = _padded_empty((sum(w.shape[0] for w in weights), weights[0].shape[1]), weights[0].device)
+        at = 0
+        for w in weights:
+            values[at:at + w.shape[0]].copy_(w.values)
+            at += w.shape[0]
+        return cls(values, torch.cat([w.scales for w in weights]).contiguous())
+
+    def to(self, device) -> "Float8Weight":
+        """On ``device``, with rows on 16-byte boundaries."""
+        if self.values.device == torch.device(device) and self.values.stride(-2) % 16 == 0 and self.values.data_ptr() % 16 == 0:
+            return Float8Weight(self.values, self.scales.contiguous())
+        values = _padded_empty(self.shape, device)
+        values.copy_(self.values)
+        return Float8Weight(values, self.scales.to(device).contiguous())
+
+    def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        n, k = self.shape[-2:]
+        s = self.scales.repeat_interleave(FP8_BLOCK, -2)[..., :n, :].repeat_interleave(FP8_BLOCK, -1)[..., :k]
+        return (self.values.to(torch.float32) * s).to(dtype)

@@ -15,6 +15,7 @@ from typing import Dict, Optional, Tuple
 import torch
 
 from ..kernels import KernelError, ops
+from .float8 import Float8Rows, Float8Weight
 
 STATUS_MESSAGES = {
     1: "a token id is outside the embedding table (token row {0}, id {1}, vocabulary {2})",
@@ -22,6 +23,7 @@ STATUS_MESSAGES = {
     3: "a position is beyond the position tables or the page table (token {0}, position {1}, limit {2})",
     4: "a bounded wait inside a kernel ran out (where {0}, detail {1}, {2})",
     5: "a slot number is outside the cache ({0}, {1}, {2})",
+    6: "a row map names a row outside its tensor (row {0}, index {1}, rows {2})",
 }
 
 
@@ -234,9 +236,16 @@ class Runtime:
 
     def linear(self, x: torch.Tensor, weight: torch.Tensor, out: Optional[torch.Tensor] = None,
                out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
-        """``x [M, K] @ weight [N, K]^T -> [M, N]``."""
+        """``x [M, K] @ weight [N, K]^T -> [M, N]``.  With a ``Float8Weight`` the rows are quantised in blocks of 128 on the way
+        (``x`` may be ``Float8Rows`` already); ``out_dtype`` is then bfloat16 unless given."""
         if not self.is_cuda:
             raise KernelError("this package computes on a CUDA device only; there is no CPU path")
+        if type(weight) is Float8Weight:
+            rows = x if type(x) is Float8Rows else Float8Rows.quantize(x)
+            if out is None:
+                out = torch.empty((rows.shape[0], weight.shape[0]), dtype=out_dtype or torch.bfloat16, device=rows.device)
+            ops.gemm_fp8(rows.values, rows.scales, weight.values, weight.scales, out, self.status)
+            return out
         if self.gemm_backend is not None:
             y = self.gemm_backend(x, weight, out, out_dtype)
             if y is not None:
@@ -284,3 +293,32 @@ class Runtime:
         finally:
             if prev[0]:
                 _set_reduced_reductions(*prev)
+
+    def float8_feed_forward(self, x, gate_up: Float8Weight, down: Float8Weight, out: torch.Tensor, glu=None) -> torch.Tensor:
+        """``out = down(act(gate, up))`` with 8-bit weights, ``gate_up`` gate rows and as many up rows; ``x`` rows in bfloat16 or
+        ``Float8Rows``.  The activation is rounded to bfloat16 and quantised in blocks of 128.  ``glu``: as in ``ops.gemm_fp8``
+        (None: SiLU)."""
+        if not self.is_cuda:
+            raise KernelError("this package computes on a CUDA device only; there is no CPU path")
+        rows = x if type(x) is Float8Rows else Float8Rows.quantize(x)
+        act = torch.empty((rows.shape[0], down.shape[1]), dtype=torch.bfloat16, device=rows.device)
+        ops.gemm_fp8(rows.values, rows.scales, gate_up.values, gate_up.scales, act, self.status, glu=glu or ())
+        rows = Float8Rows.quantize(act)
+        ops.gemm_fp8(rows.values, rows.scales, down.values, down.scales, out, self.status)
+        return out
+
+    def float8_experts(self, x, offsets: torch.Tensor, gate_up: Float8Weight, down: Float8Weight, out: torch.Tensor, glu=None,
+                       row_weight: Optional[torch.Tensor] = None, row_token: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """``float8_feed_forward`` with weights ``[experts, ...]`` for rows grouped by expert: rows ``offsets[e] .. offsets[e + 1]`` of
+        ``out [rows, hidden]`` come from expert e.  ``x``: the rows in that order, or with ``row_token`` (int32) rows to take them from.
+        ``row_weight``: as in ``ops.moe_rows_gemm_fp8``.  Rows that no expert has are left as they are."""
+        if not self.is_cuda:
+            raise KernelError("this package computes on a CUDA device only; there is no CPU path")
+        live = offsets[-1:]
+        rows = Float8Rows.quantize(x, row_token, live, self.status)
+        act = torch.empty((rows.shape[0], down.shape[2]), dtype=torch.bfloat16, device=rows.device)
+        ops.moe_rows_gemm_fp8(rows.values, rows.scales, offsets, gate_up.values, gate_up.scales, act, self.status, glu=glu or (),
+                              row_weight=row_weight)
+        rows = Float8Rows.quantize(act, None, live)
+        ops.moe_rows_gemm_fp8(rows.values, rows.scales, offsets, down.values, down.scales, out, self.status)
+        return out

@@ -1,0 +1,403 @@
+"""8-bit weights: the kernels of csrc/quantize_fp8.cu and csrc/gemm_fp8.cu against their definitions in 64 bits.
+
+Tolerances.  A conversion's result is defined to the bit (scales are powers of two, quotients exact, e4m3 to nearest with
+ties to even), so it is compared for equality.  A product's operands are e4m3 (products of two are exact in float32); its float32
+sums of K terms and K / 128 blocks are off by at most (K + 2 K / 128 + 8) * 2^-24 of the sum of the terms' magnitudes, whatever
+their order, and a bfloat16 result by half a step, 2^-8 of its value, more.
+"""
+import itertools
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF16, F32, F64 = torch.bfloat16, torch.float32, torch.float64
+E4M3 = torch.float8_e4m3fn
+
+
+@pytest.fixture(scope="module")
+def ops(pe):
+    pe.kernels.library()
+    return pe.kernels.ops
+
+
+@pytest.fixture(scope="module")
+def f8(pe):
+    return pe.parts.float8
+
+
+@pytest.fixture()
+def status():
+    st = torch.zeros(4, dtype=torch.int32, device=DEV)
+    yield st
+    assert st.tolist()[0] == 0
+
+
+def blocks(n):
+    return -(-n // 128)
+
+
+def plain_scales(a):
+    """The smallest 2^e, e >= -126, with a <= 448 * 2^e, for 64-bit magnitudes: by trying every exponent."""
+    e = torch.full_like(a, 121.0)
+    for k in range(120, -127, -1):
+        e = torch.where(a <= 448.0 * 2.0 ** k, torch.full_like(e, float(k)), e)
+    return torch.exp2(e)
+
+
+E4M3_VALUES = torch.arange(256, dtype=torch.uint8).view(E4M3).to(F64)
+
+
+def plain_e4m3(x):
+    """Nearest e4m3 value of 64-bit numbers, ties to the even code, by looking through all of them (CPU, small tensors)."""
+    pos = E4M3_VALUES[:127]                          # 0 .. 448 in the order of their codes
+    a = x.abs().cpu().clamp(max=448.0)
+    hi = torch.searchsorted(pos, a.contiguous()).clamp(max=126)
+    lo = (hi - 1).clamp(min=0)
+    up, down = pos[hi] - a, a - pos[lo]
+    take_lo = (down < up) | ((down == up) & (lo % 2 == 0))
+    v = torch.where(take_lo, pos[lo], pos[hi])
+    return torch.copysign(v, x.cpu()).to(x.device)
+
+
+def plain_quantize(x, tall):
+    """64-bit values and scales of ``x``; blocks of ``tall`` rows and 128 columns."""
+    x = x.to(F64)
+    n, k = x.shape
+    scales = torch.empty(-(-n // tall), blocks(k), dtype=F64, device=x.device)
+    q = torch.empty_like(x)
+    for i, j in itertools.product(range(scales.shape[0]), range(scales.shape[1])):
+        part = x[i * tall:(i + 1) * tall, j * 128:(j + 1) * 128]
+        scales[i, j] = plain_scales(part.abs().max())
+        q[i * tall:(i + 1) * tall, j * 128:(j + 1) * 128] = plain_e4m3(part / scales[i, j])
+    return q, scales
+
+
+def rows_of(n, k, dtype=BF16, seed=0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    x = torch.randn(n, k, generator=g, device=DEV) * torch.exp(2.0 * torch.randn(n, 1, generator=g, device=DEV))
+    x[:, k // 2] *= 30.0
+    return x.to(dtype)
+
+
+def weight_of(f8, n, k, seed=0, groups=0):
+    """An 8-bit weight with scales that are no powers of two."""
+    g = torch.Generator(device=DEV).manual_seed(seed + 1000)
+    shape = (groups, n, k) if groups else (n, k)
+    ld = -(-k // 16) * 16
+    values = torch.randn(*shape[:-1], ld, generator=g, device=DEV).mul_(60.0).clamp_(-448, 448).to(E4M3)[..., :k]
+    scales = torch.rand(*shape[:-2], blocks(n), blocks(k), generator=g, device=DEV) * 0.01 + 1e-4
+    return f8.Float8Weight(values, scales)
+
+
+def wide(w):
+    """A weight in 64 bits."""
+    n, k = w.shape[-2:]
+    s = w.scales.to(F64).repeat_interleave(128, -2)[..., :n, :].repeat_interleave(128, -1)[..., :k]
+    return w.values.to(F64) * s
+
+
+def wide_rows(r):
+    return r.values.to(F64) * r.scales.to(F64).t().repeat_interleave(128, 1)[:, :r.values.shape[1]]
+
+
+def sum_error(x64, w64):
+    """The bound on a product's float32 sums: see above."""
+    k = x64.shape[1]
+    return (k + 2 * blocks(k) + 8) * 2.0 ** -24 * (x64.abs() @ w64.abs().t())
+
+
+def assert_within(got, want, bound):
+    off = (got.to(F64) - want).abs()
+    worst = (off - bound).max()
+    assert bool((off <= bound).all()), f"off by {float(off.max())}, {float(worst)} more than allowed"
+
+
+# ---- conversion ------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("n,k", [(1, 1), (1, 128), (3, 127), (17, 129), (16, 8), (5, 1043), (33, 512), (2, 4097)])
+def test_rows(ops, f8, dtype, n, k):
+    x = rows_of(n, k, dtype)
+    r = f8.Float8Rows.quantize(x)
+    q, s = plain_quantize(x, 1)
+    assert torch.equal(r.scales.to(F64), s.t())
+    assert torch.equal(r.values.to(F64), q)
+    assert torch.equal(r.dequantize(F64), (q * s.repeat_interleave(128, 1)[:, :k]))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("n,k", [(1, 1), (128, 128), (127, 129), (130, 40), (300, 1043)])
+def test_weight(ops, f8, dtype, n, k):
+    w = rows_of(n, k, dtype, 1)
+    got = f8.Float8Weight.quantize(w)
+    q, s = plain_quantize(w, 128)
+    assert torch.equal(got.scales.to(F64), s)
+    assert torch.equal(got.values.to(F64), q)
+
+
+def test_many_rows_and_strides(ops, f8):
+    """More rows than a tile, rows of a wider matrix that start off 16-byte boundaries, scales in a wider buffer."""
+    base = rows_of(700, 1300, BF16, 3)
+    for x in (base[:, 4:1028], base[:, 3:900], base[::2, :]):
+        m, k = x.shape
+        values = torch.empty(m, 1312, dtype=E4M3, device=DEV)[:, :k]
+        scales = torch.full((blocks(k), m + 5), -1.0, device=DEV)
+        ops.quantize_rows_fp8(x, values, scales[:, :m])
+        whole = f8.Float8Rows.quantize(x.contiguous())
+        assert torch.equal(values.to(F32), whole.values.to(F32)) and torch.equal(scales[:, :m], whole.scales)
+        assert bool((scales[:, m:] == -1.0).all())
+
+
+def test_every_bfloat16(ops, f8):
+    """All finite bfloat16 values, each alone in a block of its own and in a block beside 448 times a power of two."""
+    bits = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(BF16)
+    v = bits[torch.isfinite(bits.to(F32))].to(DEV)
+    x = torch.zeros(v.numel(), 256, dtype=BF16, device=DEV)
+    x[:, 5] = v
+    x[:, 130] = v
+    x[:, 200] = 448.0 * 2.0 ** -20
+    r = f8.Float8Rows.quantize(x)
+    a = x.to(F64).abs()
+    s = plain_scales(torch.stack([a[:, :128].amax(1), a[:, 128:].amax(1)], 1))
+    assert torch.equal(r.scales.to(F64).t(), s)
+    assert torch.equal(r.values[:, 5].to(F64), plain_e4m3(v.to(F64) / s[:, 0]))
+    assert torch.equal(r.values[:, 130].to(F64), plain_e4m3(v.to(F64) / s[:, 1]))
+
+
+def test_not_finite(ops, f8):
+    """A NaN stays one and does not count for its block; an infinity becomes a NaN; other blocks do not notice."""
+    x = rows_of(3, 384, BF16, 5)
+    clean = f8.Float8Rows.quantize(x)
+    x[0, 3] = float("nan")
+    x[1, 200] = float("-inf")
+    r = f8.Float8Rows.quantize(x)
+    nan = torch.isnan(r.values.to(F32))
+    assert bool(nan[0, 3]) and bool(nan[1, 200]) and int(nan.sum()) == 2
+    same = torch.ones(3, 384, dtype=torch.bool, device=DEV)
+    same[0, 3] = False
+    same[1, 128:256] = False
+    assert torch.equal(r.values.to(F32)[same], clean.values.to(F32)[same])
+    assert float(r.scales[1, 1]) == 2.0 ** 120
+    w = x.clone()
+    got = f8.Float8Weight.quantize(w)
+    assert bool(torch.isnan(got.values.to(F32))[1, 200])
+
+
+def test_row_map(ops, f8, status):
+    x = rows_of(9, 300, BF16, 6)
+    pick = torch.tensor([8, 0, 0, 3, 7, 99], dtype=torch.int32, device=DEV)
+    live = torch.tensor([5], dtype=torch.int32, device=DEV)      # the last one is not there: nobody looks at its index
+    r = f8.Float8Rows.empty(6, 300, DEV)
+    r.values.copy_(torch.full((6, 300), 7.0, device=DEV).to(E4M3))
+    r.scales.fill_(7.0)
+    ops.quantize_rows_fp8(x, r.values, r.scales, pick, live, status)
+    whole = f8.Float8Rows.quantize(x)
+    at = pick[:5].long()
+    assert torch.equal(r.values[:5].to(F32), whole.values[at].to(F32)) and torch.equal(r.scales[:, :5], whole.scales[:, at])
+    assert bool((r.values[5].to(F32) == 7.0).all()) and bool((r.scales[:, 5] == 7.0).all())
+
+
+def test_row_map_outside(ops, f8):
+    x = rows_of(4, 130, BF16, 7)
+    st = torch.zeros(4, dtype=torch.int32, device=DEV)
+    r = f8.Float8Rows.empty(2, 130, DEV)
+    r.scales.fill_(7.0)
+    ops.quantize_rows_fp8(x, r.values, r.scales, torch.tensor([1, 4], dtype=torch.int32, device=DEV), None, st)
+    assert st.tolist() == [6, 1, 4, 4]
+    assert bool((r.scales[:, 1] == 7.0).all())
+
+
+@pytest.mark.parametrize("n,dim", [(1, 4), (3, 132), (2, 512), (5, 1000), (70, 2056), (3, 4096), (65, 4096)])
+@pytest.mark.parametrize("delta", [True, False])
+def test_norm(ops, f8, n, dim, delta):
+    """The same bits as the norm's own kernel followed by the conversion's."""
+    g = torch.Generator(device=DEV).manual_seed(n)
+    stream = torch.randn(n, dim, generator=g, device=DEV) * 3
+    d = torch.randn(n, dim, generator=g, device=DEV).to(BF16) if delta else None
+    w = torch.randn(dim, generator=g, device=DEV)
+    two, out = stream.clone(), torch.empty(n, dim, dtype=BF16, device=DEV)
+    ops.rmsnorm_residual(two, d, w, out, 1e-6)
+    want = f8.Float8Rows.quantize(out)
+    r = f8.Float8Rows.empty(n, dim, DEV)
+    ops.rmsnorm_residual_fp8(stream, d, w, r.values, r.scales, 1e-6)
+    assert torch.equal(stream, two)
+    assert torch.equal(r.values.to(F32), want.values.to(F32)) and torch.equal(r.scales, want.scales)
+
+
+# ---- products --------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("out_dtype", [F32, BF16])
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 128, 128), (3, 129, 130), (16, 300, 1040), (17, 64, 2000), (33, 1111, 384),
+                                   (65, 257, 640), (128, 128, 4096), (129, 130, 1043), (300, 384, 512), (8, 4096, 12288), (2, 6144, 4096)])
+def test_product(ops, f8, status, m, n, k, out_dtype):
+    rows, w = f8.Float8Rows.quantize(rows_of(m, k, BF16, m)), weight_of(f8, n, k, n)
+    out = torch.empty(m, n, dtype=out_dtype, device=DEV)
+    ops.gemm_fp8(rows.values, rows.scales, w.values, w.scales, out, status)
+    x64, w64 = wide_rows(rows), wide(w)
+    want = x64 @ w64.t()
+    assert_within(out, want, sum_error(x64, w64) + (2.0 ** -8 * want.abs() if out_dtype == BF16 else 0.0))
+    again = torch.empty_like(out)
+    ops.gemm_fp8(rows.values, rows.scales, w.values, w.scales, again, status)
+    assert torch.equal(out, again)
+
+
+def plain_glu(kind, g, u, limit, alpha):
+    """Activations of a gate and an up sum, in 64 bits."""
+    if kind == "silu":
+        return g * torch.sigmoid(g) * u
+    if kind == "relu":
+        return g.clamp(min=0) * u
+    g, u = g.clamp(max=limit), u.clamp(-limit, limit)
+    return g * torch.sigmoid(alpha * g) * (u + 1)
+
+
+def glu_bound(kind, g, u, eg, eu, limit, alpha, want):
+    """How far act(g, u) may be off for sums off by eg and eu: |d act / dg| <= 1.1 |u'|, |d act / du| <= |act(g)| <= |g| (silu's
+    slope is at most 1.1, u' is u, or |u + 1| <= limit + 1); the exponential and the quotient are good to 2^-20, the result is
+    rounded to bfloat16."""
+    slope = 1.1 if kind != "clamped_swish" else 1.1
+    up = u.abs() if kind != "clamped_swish" else u.clamp(-limit, limit).abs() + 1
+    return slope * (up + eu) * eg + (g.abs() + eg) * eu + (2.0 ** -8 + 2.0 ** -20) * want.abs() + 1e-30
+
+
+@pytest.mark.parametrize("kind,limit,alpha,bias", [("silu", 0.0, 1.0, False), ("relu", 0.0, 1.0, False), ("clamped_swish", 7.0, 1.7, True)])
+@pytest.mark.parametrize("m,inter,k", [(1, 1, 16), (2, 64, 256), (7, 72, 1040), (20, 200, 512), (64, 96, 640), (130, 320, 384), (5, 12288, 4096)])
+def test_gate(ops, f8, status, m, inter, k, kind, limit, alpha, bias):
+    rows, w = f8.Float8Rows.quantize(rows_of(m, k, BF16, m) * 0.01), weight_of(f8, 2 * inter, k, inter)
+    b = torch.randn(2 * inter, device=DEV) if bias else None
+    out = torch.empty(m, inter, dtype=BF16, device=DEV)
+    ops.gemm_fp8(rows.values, rows.scales, w.values, w.scales, out, status, glu=() if kind == "silu" else (kind, limit, alpha, b))
+    x64, w64 = wide_rows(rows), wide(w)
+    sums, err = x64 @ w64.t(), sum_error(x64, w64)
+    if bias:
+        sums = sums + b.to(F64)
+        err = err + 2.0 ** -23 * sums.abs()
+    g, u = sums[:, :inter], sums[:, inter:]
+    want = plain_glu(kind, g, u, limit, alpha)
+    assert_within(out, want, glu_bound(kind, g, u, err[:, :inter], err[:, inter:], limit, alpha, want))
+
+
+# the rows of each expert: none, one, a tile's and beyond, all in one
+@pytest.mark.parametrize("counts", [[0, 1, 0, 3], [5], [16, 17, 0, 33, 1], [0, 0, 200, 0], [0] * 40 + [2, 3] + [0] * 30, [130, 1, 140]])
+@pytest.mark.parametrize("n,k", [(128, 128), (200, 400), (96, 1043)])
+def test_experts_product(ops, f8, status, counts, n, k):
+    live, groups = sum(counts), len(counts)
+    m = live + 3                                       # rows that no expert has
+    offsets = torch.tensor([sum(counts[:i]) for i in range(groups + 1)], dtype=torch.int32, device=DEV)
+    rows, w = f8.Float8Rows.quantize(rows_of(m, k, BF16, m)), weight_of(f8, n, k, n, groups)
+    out = torch.full((m, n), 5.0, device=DEV)
+    ops.moe_rows_gemm_fp8(rows.values, rows.scales, offsets, w.values, w.scales, out, status)
+    x64, w64 = wide_rows(rows), wide(w)
+    for e, c in enumerate(counts):
+        at = slice(int(offsets[e]), int(offsets[e]) + c)
+        assert_within(out[at], x64[at] @ w64[e].t(), sum_error(x64[at], w64[e])) if c else None
+    assert bool((out[live:] == 5.0).all())
+
+
+@pytest.mark.parametrize("weighted", [False, True])
+def test_experts_gate(ops, f8, status, weighted):
+    counts, inter, k = [3, 0, 18, 1], 104, 272
+    m, groups = sum(counts), len(counts)
+    offsets = torch.tensor([0, 3, 3, 21, 22], dtype=torch.int32, device=DEV)
+    rows, w = f8.Float8Rows.quantize(rows_of(m, k, BF16, 9) * 0.01), weight_of(f8, 2 * inter, k, 9, groups)
+    rw = torch.rand(m, device=DEV) if weighted else None
+    out = torch.empty(m, inter, dtype=BF16, device=DEV)
+    ops.moe_rows_gemm_fp8(rows.values, rows.scales, offsets, w.values, w.scales, out, status, glu=(), row_weight=rw)
+    x64, w64 = wide_rows(rows), wide(w)
+    for e in range(groups):
+        at = slice(int(offsets[e]), int(offsets[e + 1]))
+        sums, err = x64[at] @ w64[e].t(), sum_error(x64[at], w64[e])
+        if weighted:
+            f = rw[at, None].to(F64)
+            sums, err = sums * f, err * f + 2.0 ** -23 * (sums * f).abs()
+        g, u = sums[:, :inter], sums[:, inter:]
+        want = plain_glu("silu", g, u, 0, 1)
+        if want.numel():
+            assert_within(out[at], want, glu_bound("silu", g, u, err[:, :inter], err[:, inter:], 0, 1, want))
+
+
+def test_offsets_outside_the_rows(ops, f8, status):
+    """Offsets beyond the rows count as their number: nothing is written behind the output."""
+    k, n = 128, 64
+    rows, w = f8.Float8Rows.quantize(rows_of(6, k)), weight_of(f8, n, k, 0, 2)
+    big = torch.full((40, n), 5.0, device=DEV)
+    ops.moe_rows_gemm_fp8(rows.values, rows.scales, torch.tensor([-4, 2, 1000], dtype=torch.int32, device=DEV), w.values, w.scales,
+                          big[:6], status)
+    assert bool((big[6:] == 5.0).all())
+    x64, w64 = wide_rows(rows), wide(w)
+    assert_within(big[2:6], x64[2:] @ w64[1].t(), sum_error(x64[2:], w64[1]))
+
+
+def test_product_strides(ops, f8, status):
+    """Operands inside wider buffers, an output inside another, scales with room behind them."""
+    m, n, k = 37, 190, 300
+    wide_x = torch.empty(m, 640, dtype=E4M3, device=DEV)
+    scales = torch.empty(blocks(k), 64, device=DEV)
+    x = rows_of(m, k, BF16, 2)
+    ops.quantize_rows_fp8(x, wide_x[:, 32:32 + k], scales[:, :m])
+    w = weight_of(f8, n, k, 3)
+    wide_w = torch.empty(n, 512, dtype=E4M3, device=DEV)
+    wide_w[:, 48:48 + k] = w.values
+    out = torch.full((m, 256), 5.0, dtype=BF16, device=DEV)
+    ops.gemm_fp8(wide_x[:, 32:32 + k], scales[:, :m], wide_w[:, 48:48 + k], w.scales, out[:, 7:7 + n], status)
+    plain = torch.empty(m, n, dtype=BF16, device=DEV)
+    r = f8.Float8Rows.quantize(x)
+    ops.gemm_fp8(r.values, r.scales, w.values, w.scales, plain, status)
+    assert torch.equal(out[:, 7:7 + n], plain)
+    assert bool((out[:, :7] == 5.0).all()) and bool((out[:, 7 + n:] == 5.0).all())
+
+
+def test_empty(ops, f8, status):
+    w = weight_of(f8, 64, 128)
+    r = f8.Float8Rows.empty(0, 128, DEV)
+    out = torch.empty(0, 64, dtype=BF16, device=DEV)
+    ops.gemm_fp8(r.values, r.scales, w.values, w.scales, out, status)
+    ops.quantize_rows_fp8(torch.empty(0, 128, dtype=BF16, device=DEV), r.values, r.scales)
+    ops.rmsnorm_residual_fp8(torch.empty(0, 128, device=DEV), None, torch.ones(128, device=DEV), r.values, r.scales, 1e-6)
+
+
+def test_a_nan_stays_in_its_row(ops, f8, status):
+    x = rows_of(20, 300, BF16, 4)
+    w = weight_of(f8, 130, 300)
+    clean, dirty = (torch.empty(20, 130, dtype=BF16, device=DEV) for _ in range(2))
+    r = f8.Float8Rows.quantize(x)
+    ops.gemm_fp8(r.values, r.scales, w.values, w.scales, clean, status)
+    x[7, 299] = float("inf")
+    r = f8.Float8Rows.quantize(x)
+    ops.gemm_fp8(r.values, r.scales, w.values, w.scales, dirty, status)
+    assert bool(torch.isnan(dirty[7]).all())
+    keep = torch.arange(20, device=DEV) != 7
+    assert torch.equal(clean[keep], dirty[keep])
+
+
+def test_own_stream_and_graph(ops, f8, status):
+    """A run of them on another stream than the default, captured, and replayed on other inputs in the same buffers."""
+    m, k, n = 9, 512, 640
+    w = weight_of(f8, n, k)
+    x = rows_of(m, k, BF16, 1)
+    out = torch.empty(m, n, dtype=BF16, device=DEV)
+    r = f8.Float8Rows.empty(m, k, DEV)
+
+    def chain():
+        ops.quantize_rows_fp8(x, r.values, r.scales)
+        ops.gemm_fp8(r.values, r.scales, w.values, w.scales, out, status)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        chain()
+    side.synchronize()
+    first = out.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        chain()
+    out.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, first)
+    x.copy_(rows_of(m, k, BF16, 2))
+    graph.replay()
+    torch.cuda.synchronize()
+    replayed = out.clone()
+    chain()
+    assert torch.equal(out, replayed) and not torch.equal(out, first)

@@ -6,17 +6,18 @@
 // the outer sum is taken in float32 registers, as the columns of one block after the other are read back.  So the scales cost one
 // multiply-add an output and block and no operand is ever widened.
 //
-// With few rows the product is a stream of the weights through the SMs, and the operands' roles are chosen for that: 128
-// weight rows are the MMA's M dimension, NP = 16 to 128 rows of x its N dimension.  Tensor memory then holds 256 / NP blocks' sums
-// (16 for NP = 16), and the MMAs never wait for the epilogue while a block's weights are on their way.  K is split over the
-// thread blocks of a cluster, which add their sums up through distributed shared memory in the order of their ranks (no
-// atomics: the result does not depend on scheduling).
+// With few rows the product is a stream of the weights through the SMs, and the operands' roles are chosen for that: up to 128
+// weight rows are the MMA's M dimension, NP = 16 to 128 rows of x its N dimension.  K is split over the thread blocks of a cluster;
+// each sends its sums to the block that finishes them through distributed shared memory, where they are added in the order of the
+// ranks (no atomics: the result does not depend on scheduling).
 //
-// Roles: warp 0 copies (TMA), warp 1 allocates tensor memory and issues the MMAs, the other warps are the epilogue: a thread
-// owns a weight row (its tensor memory lane) and NP, for NP = 128 half of them, sums.  The first stages' weights are asked for before
-// the kernel waits for its predecessor in the stream.
+// Roles: warp 0 copies the weights and warp 2 the rows (TMA; a thread starts a copy only every 150 ns or so), warp 1 allocates
+// tensor memory and issues the MMAs, the other warps are the epilogue: a thread owns a weight row (its tensor memory lane) and NP,
+// for NP = 128 half of them, sums.  A stage is KBS k blocks: a commit costs about 0.11 us that the MMAs behind it wait for.
+// The first stages' weights are asked for before the kernel waits for its predecessor in the stream, and its own successor may
+// start at once: with half an SM's shared memory a block, the next product's weights are on their way while this one still works.
 //
-// GLU: a tile is 64 gate rows and the 64 up rows that belong to them, and y = act(gate, up), rounded to bfloat16.
+// GLU: a tile is up to 64 gate rows and the up rows that belong to them, and y = act(gate, up), rounded to bfloat16.
 // Groups (routed experts): the rows of x are ordered by group, offsets[g] .. offsets[g + 1] are those of group g, which has a
 // matrix of its own; a tile of rows belongs to one group.
 //
@@ -30,220 +31,303 @@ namespace fp8 {
 
 struct Params {
   int M, N, K, k_blocks;               // N: output columns
+  bool whole;                          // K is whole blocks
   const float* xs; long long xs_ld;    // [k_blocks][xs_ld]
+  const __nv_bfloat16* x; long long x_ld;   // RAW
   const float* ws; long long ws_group; // per group [ceil(rows / 128)][k_blocks]
   int w_rows;                          // weight rows of a group: N, or 2 N with GLU
   void* y; long long ldy; int out_f32;
-  int tok_tiles, split;
+  int tile_rows, tok_tiles, split;     // tile_rows: weight rows of a tile (GLU: gate rows, and as many ups)
   const int* offsets; int n_groups;    // null, 0: one group of M rows
   GluEpilogue glu; const float* row_weight;
   int* status;
 };
 
-constexpr int kTile = 128;             // weight rows of a tile
-constexpr int kTmemCols = 256;
+constexpr int kTile = 128;             // weight rows of a full tile
+constexpr int kRoles = 3;              // warps before the epilogue's
 
 template <int NP> struct Shape {
-  static constexpr int kStages = NP == 16 ? 5 : NP == 32 ? 5 : NP == 64 ? 4 : 3;
-  static constexpr int kStage = kTile * BK + NP * BK;
-  static constexpr int kSlots = kTmemCols / NP;
+  static constexpr int kKbs = 2;           // k blocks of a stage
+  static constexpr int kStages = NP == 16 ? 3 : 2;
+  static constexpr int kPerSm = NP == 128 ? 1 : 2;         // thread blocks an SM holds
+  static constexpr int kStage = kKbs * (kTile * BK + NP * BK);
   static constexpr int kEpiWarps = NP == 128 ? 8 : 4;
   static constexpr int kCols = NP / (kEpiWarps / 4);       // sums of a thread
-  static constexpr int kThreads = 64 + 32 * kEpiWarps;
+  static constexpr int kThreads = 32 * (kRoles + kEpiWarps);
   static constexpr int kChunk = NP == 128 ? 16 : 32;       // k blocks whose scales lie in shared memory
+  static constexpr int kTmem = kStages * kKbs * NP <= 128 ? 128 : kStages * kKbs * NP <= 256 ? 256 : 512;
   static constexpr size_t kSmem = 1024 + (size_t)kStages * kStage;
 };
 
+__device__ __forceinline__ void load_5d(void* dst, const CUtensorMap* map, int x, int row, int block, int group, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];\n"
+      ::"r"(tma::smem_addr(dst)), "l"(map), "r"(x), "r"(row), "r"(0), "r"(block), "r"(group), "r"(tma::smem_addr(bar)) : "memory");
+}
 __device__ __forceinline__ void epilogue_sync(int threads) { asm volatile("bar.sync 1, %0;\n" ::"r"(threads) : "memory"); }
 
-// Which group, and which of its tiles of NP rows, token tile `j` is: all lanes of a warp take part.
-// Offsets outside 0 .. M count as these.
-__device__ __forceinline__ bool find_group(const int* offsets, int n_groups, int M, int np, int j, int& group, int& row0, int& rows) {
-  const int lane = threadIdx.x & 31;
-  int before = 0;
-  for (int base = 0; base < n_groups; base += 32) {
-    const int g = base + lane;
-    int lo = 0, n = 0;
-    if (g < n_groups) {
-      lo = min(max(offsets[g], 0), M);
-      n = max(min(max(offsets[g + 1], 0), M) - lo, 0);
-    }
-    const int tiles = (n + np - 1) / np;
-    int sum = tiles;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += up;
-    }
-    const int first = before + sum - tiles;
-    const unsigned hit = __ballot_sync(0xffffffffu, j >= first && j < first + tiles);
-    if (hit) {
-      const int from = __ffs(hit) - 1;
-      group = base + from;
-      const int t = j - __shfl_sync(0xffffffffu, first, from);
-      row0 = __shfl_sync(0xffffffffu, lo, from) + t * np;
-      rows = min(np, __shfl_sync(0xffffffffu, n, from) - t * np);
-      return true;
-    }
-    before += __shfl_sync(0xffffffffu, sum, 31);
-  }
-  return false;
-}
+// The bfloat16 rows of a stage on their way into it (RAW): sixteen lanes a row and block, eight features a lane.
+struct RawRows {
+  uint4 v[4];
+};
 
-template <int NP, bool GLU>
-__global__ void __launch_bounds__(Shape<NP>::kThreads, 2)
+template <int NP, bool GLU, bool RAW>
+__global__ void __launch_bounds__(Shape<NP>::kThreads, Shape<NP>::kPerSm)
 gemm_fp8_kernel(Params p, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap) {
   using S = Shape<NP>;
-  constexpr int STAGES = S::kStages, SLOTS = S::kSlots, EPI = S::kEpiWarps, COLS = S::kCols, CH = S::kChunk;
+  constexpr int STAGES = S::kStages, KBS = S::kKbs, EPI = S::kEpiWarps, COLS = S::kCols, CH = S::kChunk, ET = 32 * EPI;
   extern __shared__ char smem_raw[];
-  __shared__ uint64_t full_bar[STAGES], empty_bar[STAGES], acc_full[SLOTS], acc_empty[SLOTS];
+  __shared__ uint64_t full_bar[STAGES], done_bar[STAGES], read_bar[STAGES];
   __shared__ __align__(16) float sx_s[CH][NP];
-  __shared__ float sw_s[CH][4];
+  __shared__ float sw_s[4][CH];
   __shared__ uint32_t tmem_holder;
   __shared__ volatile int failed;
+  __shared__ int started[2];
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = p.split > 1 ? (int)cluster_rank() : 0;
   const int tile = (int)blockIdx.x / p.split;
   const int row_tile = tile / p.tok_tiles, tok_tile = tile - row_tile * p.tok_tiles;
-  const int n0 = row_tile * (GLU ? kTile / 2 : kTile);
+  const int R = p.tile_rows, n0 = row_tile * R, n_out = min(R, p.N - n0), tile_bytes = (GLU ? 2 : 1) * R * BK;
   const int kb_lo = (int)((long long)p.k_blocks * rank / p.split), kb_hi = (int)((long long)p.k_blocks * (rank + 1) / p.split);
-  const int n_kb = kb_hi - kb_lo;
+  const int n_kb = kb_hi - kb_lo, n_st = (n_kb + KBS - 1) / KBS;
 
   int group = 0, row0 = tok_tile * NP, rows = min(NP, p.M - row0);
-  auto load_w = [&](int i) {           // the weights of this block's k block i
+  auto load_w = [&](int i) {           // the weights of this block's stage i (blocks beyond n_kb are loaded and not used)
     const int stage = i % STAGES;
     char* sw = smem + stage * S::kStage;
-    tma::mbar_expect_tx(&full_bar[stage], S::kStage);
-    const int x = (kb_lo + i) * BK, y = group * p.w_rows + n0;
-    tma::load_2d(sw, &wmap, x, y, &full_bar[stage]);
-    if (GLU) tma::load_2d(sw + kTile / 2 * BK, &wmap, x, y + p.N, &full_bar[stage]);
+    tma::mbar_expect_tx(&full_bar[stage], KBS * tile_bytes);
+    const int kb = kb_lo + i * KBS;
+    if (p.whole) {
+      load_5d(sw, &wmap, 0, n0, kb, group, &full_bar[stage]);
+    } else {
+      for (int j = 0; j < KBS; ++j) load_5d(sw + j * tile_bytes, &wmap, (kb + j) * BK, n0, 0, group, &full_bar[stage]);
+    }
+  };
+  const int e_tid = (int)threadIdx.x - 32 * kRoles;
+  // The rows of scales that the tile's weight rows fall into: up to two, and with GLU two more for the ups.
+  const int up0 = p.N + n0;
+  auto load_sw = [&](int kb0) {        // of the chunk of blocks from kb0 on
+    static_assert(4 * CH <= ET, "a scale a thread");
+    const int which = e_tid / CH, b = e_tid % CH;
+    if (which < (GLU ? 4 : 2) && kb0 + b < n_kb) {
+      const int sr = min((which < 2 ? n0 : up0) / 128 + (which & 1), (p.w_rows - 1) / 128);
+      sw_s[which][b] = p.ws[(size_t)group * p.ws_group + (size_t)sr * p.k_blocks + kb_lo + kb0 + b];
+    }
+  };
+  auto load_sx = [&](int kb0) {
+    float v[CH * NP / ET];
+#pragma unroll
+    for (int q = 0; q < CH * NP / ET; ++q) {
+      const int e = q * ET + e_tid, b = e / NP, t = e % NP;
+      v[q] = kb0 + b < n_kb && t < rows ? p.xs[(size_t)(kb_lo + kb0 + b) * p.xs_ld + row0 + t] : 0.f;
+    }
+#pragma unroll
+    for (int q = 0; q < CH * NP / ET; ++q) (&sx_s[0][0])[q * ET + e_tid] = v[q];
   };
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      tma::mbar_init(&full_bar[s], 1);
-      tma::mbar_init(&empty_bar[s], 1);
-    }
-    for (int s = 0; s < SLOTS; ++s) {
-      tma::mbar_init(&acc_full[s], 1);
-      tma::mbar_init(&acc_empty[s], EPI);
+      tma::mbar_init(&full_bar[s], RAW ? 1 + EPI : 2);    // the weights' producer, and the rows' or the warps that convert them
+      tma::mbar_init(&done_bar[s], 1);    // the commit behind a stage's MMAs
+      tma::mbar_init(&read_bar[s], EPI);  // the epilogue's warps
     }
     failed = 0;
     tma::fence_barrier_init();
     // without groups the weights' place is known now: they do not come from the kernel before this one
     if (p.n_groups == 0)
-      for (int i = 0; i < min(STAGES, n_kb); ++i) load_w(i);
+      for (int i = 0; i < min(STAGES, n_st); ++i) load_w(i);
   }
-  if (warp == 1) tmem_alloc<1>(&tmem_holder, kTmemCols);
+  if (warp == 1) tmem_alloc<1>(&tmem_holder, S::kTmem);
+  if (warp >= kRoles && p.n_groups == 0) load_sw(0);
   fence_before_sync();
   pdl_wait_block();
+  pdl_launch_dependents();
   fence_after_sync();
   const uint32_t tmem_base = tmem_holder;
   bool live = true;
   if (p.n_groups > 0) live = find_group(p.offsets, p.n_groups, p.M, NP, tok_tile, group, row0, rows);   // the same answer in every warp
 
-  int loaded = 0;                      // warp 0: k blocks whose copies were started
+  int loaded = 0;                      // warps 0 and 2: stages whose copies were started
   if (!live) {
     // more tiles were launched than the groups' rows fill
-  } else if (warp == 0) {
+  } else if (warp == 0 || (warp == 2 && !RAW)) {
     if (lane == 0) {
-      for (; loaded < n_kb && !failed; ++loaded) {
+      for (; loaded < n_st && !failed; ++loaded) {
         const int stage = loaded % STAGES;
-        if (loaded >= STAGES && !tma::mbar_wait(&empty_bar[stage], ((loaded / STAGES) & 1) ^ 1)) {
+        if (loaded >= STAGES && !tma::mbar_wait(&done_bar[stage], ((loaded / STAGES) & 1) ^ 1)) {
           report(p.status, kStatusWaitTimedOut, 70, tile, loaded);
           failed = 1;
           break;
         }
-        if (p.n_groups > 0 || loaded >= STAGES) load_w(loaded);
-        tma::load_2d(smem + stage * S::kStage + kTile * BK, &xmap, (kb_lo + loaded) * BK, row0, &full_bar[stage]);
+        if (warp == 0) {
+          if (p.n_groups > 0 || loaded >= STAGES) load_w(loaded);
+        } else {
+          tma::mbar_expect_tx(&full_bar[stage], KBS * NP * BK);
+          load_blocks(smem + stage * S::kStage + KBS * kTile * BK, &xmap, kb_lo + loaded * KBS, row0, KBS, NP, p.whole, &full_bar[stage]);
+        }
       }
     }
     __syncwarp();
   } else if (warp == 1) {
     if (lane == 0) {
       constexpr uint32_t idesc = instr_desc(kTile, NP);
-      for (int i = 0; i < n_kb && !failed; ++i) {
-        const int stage = i % STAGES, slot = i % SLOTS;
-        if ((i >= SLOTS && !tma::mbar_wait(&acc_empty[slot], ((i / SLOTS) & 1) ^ 1)) ||
-            !tma::mbar_wait(&full_bar[stage], (i / STAGES) & 1)) {
-          report(p.status, kStatusWaitTimedOut, 71, tile, i);
-          failed = 1;
-          break;
-        }
-        fence_after_sync();
-        const uint32_t sw = tma::smem_addr(smem + stage * S::kStage), sx = sw + kTile * BK;
+      const uint32_t base = tma::smem_addr(smem);
+      // Unrolled over the stages: an MMA's descriptors are registers that it reads when it starts, and a loop that writes the same
+      // ones again waits for that (a stage of two blocks of 16 rows took 1,290 cycles, of which the MMAs are some 500).
+      for (int i0 = 0; i0 < n_st && !failed; i0 += STAGES) {
 #pragma unroll
-        for (int k = 0; k < BK / 32; ++k)
-          umma(tmem_base + slot * NP, smem_desc(sw + k * 32), smem_desc(sx + k * 32), idesc, k > 0 ? 1u : 0u);
-        umma_commit(&empty_bar[stage]);
-        umma_commit(&acc_full[slot]);
+        for (int stage = 0; stage < STAGES; ++stage) {
+          const int i = i0 + stage, n = n_kb - i * KBS;
+          if (n <= 0) break;
+          if ((i >= STAGES && !tma::mbar_wait(&read_bar[stage], ((i / STAGES) & 1) ^ 1)) ||
+              !tma::mbar_wait(&full_bar[stage], (i / STAGES) & 1)) {
+            report(p.status, kStatusWaitTimedOut, 71, tile, i);
+            failed = 1;
+            break;
+          }
+          fence_after_sync();
+          const uint32_t sw = base + stage * S::kStage, sx = sw + KBS * kTile * BK;
+#pragma unroll
+          for (int j = 0; j < KBS; ++j) {
+            if (j >= n) break;
+#pragma unroll
+            for (int k = 0; k < BK / 32; ++k)
+              umma(tmem_base + (stage * KBS + j) * NP, smem_desc(sw + j * tile_bytes + k * 32), smem_desc(sx + j * NP * BK + k * 32), idesc,
+                   k > 0 ? 1u : 0u);
+          }
+          umma_commit(&done_bar[stage]);
+        }
       }
     }
     __syncwarp();
-    pdl_launch_dependents();
   }
+  // RAW: pass q of this warp is row t of x and block j of the stage; rows that are not there are left out.
+  const int raw_lane = 8 * (lane & 15);
+  auto raw_at = [&](int q, int& j, int& t) {
+    const int item = q * 8 + (warp - kRoles) * 2 + (lane >> 4);
+    j = item & (KBS - 1);
+    t = item / KBS;
+  };
+  auto raw_load = [&](int i, RawRows& r) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      int j, t;
+      raw_at(q, j, t);
+      const int at = (kb_lo + i * KBS + j) * BK + raw_lane;
+      r.v[q] = make_uint4(0, 0, 0, 0);
+      if (t < rows && i * KBS + j < n_kb && at < p.K) {
+        const __nv_bfloat16* x = p.x + (size_t)(row0 + t) * p.x_ld + at;
+        if (at + 8 <= p.K) {
+          r.v[q] = *reinterpret_cast<const uint4*>(x);
+        } else {
+          __nv_bfloat16 e[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) e[k] = at + k < p.K ? x[k] : __float2bfloat16_rn(0.f);
+          r.v[q] = *reinterpret_cast<const uint4*>(e);
+        }
+      }
+    }
+  };
+  auto raw_store = [&](int i, const RawRows& r) {
+    const int stage = i % STAGES;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      int j, t;
+      raw_at(q, j, t);
+      if (__all_sync(0xffffffffu, t >= rows)) break;
+      float v[8], top = 0.f;
+      const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&r.v[q]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 e = __bfloat1622float2(h[k]);
+        v[2 * k] = e.x;
+        v[2 * k + 1] = e.y;
+        top = fmaxf(top, fmaxf(fabsf(e.x), fabsf(e.y)));
+      }
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const uint32_t scale = scale_bits(top);
+      const float by = inverse_of(scale);
+      if (top == INFINITY) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = no_infinity(v[k]);
+      }
+      char* to = smem + stage * S::kStage + KBS * kTile * BK + (j * NP + t) * BK;
+      *reinterpret_cast<uint2*>(to + ((((raw_lane >> 4) ^ (t & 7)) << 4) | (raw_lane & 8))) =
+          make_uint2(pack4(v[0] * by, v[1] * by, v[2] * by, v[3] * by), pack4(v[4] * by, v[5] * by, v[6] * by, v[7] * by));
+      if ((lane & 15) == 0) sx_s[(i * KBS + j) % CH][t] = __uint_as_float(scale);
+    }
+    tma::fence_proxy_async();          // the MMAs read what was written here
+    __syncwarp();
+    if (lane == 0) tma::mbar_arrive(&full_bar[stage]);
+  };
   float acc[COLS];
-  const int quarter = warp & 3, row = quarter * 32 + lane;         // of the tile's weight rows
-  const int col0 = EPI == 8 && warp >= 6 ? COLS : 0;               // first of this thread's rows of x
-  if (live && warp >= 2) {
+  const int quarter = warp & 3, row = quarter * 32 + lane;         // of the tile's weight rows: with GLU R gates, then R ups
+  const int col0 = EPI == 8 && warp >= kRoles + 4 ? COLS : 0;      // first of this thread's rows of x
+  // where the operands' stages were, when every copy has arrived and every MMA has read them: [rank][its rows of x][weight row]
+  float* sums = reinterpret_cast<float*>(smem);
+  if (live && warp >= kRoles) {
 #pragma unroll
     for (int t = 0; t < COLS; ++t) acc[t] = 0.f;
-    // the rows of scales that the tile's weight rows fall into: one, or with GLU the gates' and up to two of the ups'
-    const int up0 = p.N + n0;
-    const int srow = GLU ? (row < 64 ? 0 : 1 + ((up0 + row - 64) / 128 - up0 / 128)) : 0;
-    const float* ws = p.ws + (size_t)group * p.ws_group;
-    const int last_srow = (p.w_rows - 1) / 128;
-    const int e_tid = threadIdx.x - 64;
+    const bool up = GLU && row >= R;
+    const int srow = up ? 2 + ((up0 + row - R) / 128 - up0 / 128) : (n0 + row) / 128 - n0 / 128;
+    const bool used = row < (GLU ? 2 : 1) * R;
+    RawRows raw[RAW ? STAGES : 1];
+    if (RAW) {
+#pragma unroll
+      for (int i = 0; i < STAGES; ++i) raw_load(i, raw[i]);
+#pragma unroll
+      for (int i = 0; i < STAGES; ++i)
+        if (i < n_st) raw_store(i, raw[i]);
+    }
     // this loop has barriers in it: after a wait that ran out it goes on without waiting
-    for (int i = 0; i < n_kb; ++i) {
-      const int slot = i % SLOTS, c = i % CH;
-      if (c == 0) {                    // the next chunk of scales
-        epilogue_sync(EPI * 32);
-        const int n = min(CH, n_kb - i);
-        for (int e = e_tid; e < n * NP; e += EPI * 32) {
-          const int b = e / NP, t = e - b * NP;
-          sx_s[b][t] = t < rows ? p.xs[(size_t)(kb_lo + i + b) * p.xs_ld + row0 + t] : 0.f;
-        }
-        for (int e = e_tid; e < n * 3; e += EPI * 32) {
-          const int b = e / 3, which = e - b * 3;
-          const int sr = which == 0 ? n0 / 128 : min(up0 / 128 + which - 1, last_srow);
-          if (GLU || which == 0) sw_s[b][which] = ws[(size_t)sr * p.k_blocks + kb_lo + i + b];
-        }
-        epilogue_sync(EPI * 32);
+    for (int i = 0; i < n_st; ++i) {
+      const int stage = i % STAGES, kb0 = i * KBS;
+      if (kb0 % CH == 0) {             // the next chunk of scales
+        if (i > 0) epilogue_sync(ET);  // everybody is done with the last one
+        if (i > 0 || p.n_groups > 0) load_sw(kb0);
+        if (!RAW) load_sx(kb0);
+        epilogue_sync(ET);
       }
-      if (!failed && !tma::mbar_wait(&acc_full[slot], (i / SLOTS) & 1)) {
+      if (RAW && i + STAGES < n_st) raw_load(i + STAGES, raw[0]);
+      if (!failed && !tma::mbar_wait(&done_bar[stage], (i / STAGES) & 1)) {
         if (lane == 0) report(p.status, kStatusWaitTimedOut, 72, tile, i);
         failed = 1;
       }
+      if (RAW && !failed) tma::mbar_wait(&full_bar[stage], (i / STAGES) & 1);    // long complete: the other warps' scales are seen
       __syncwarp();
       fence_after_sync();
-      const float sw = sw_s[c][srow];
-      const uint32_t t_row = tmem_base + slot * NP + col0 + ((uint32_t)(quarter * 32) << 16);
 #pragma unroll
-      for (int t = 0; t < COLS; t += 16) {
-        uint32_t v[16];
-        tmem_ld16(t_row + t, v);
-        tmem_ld_wait();
+      for (int j = 0; j < KBS; ++j) {
+        if (kb0 + j >= n_kb) break;
+        const int c = (kb0 + j) % CH;
+        const float sw = used ? sw_s[srow][c] : 0.f;
+        const uint32_t t_row = tmem_base + (stage * KBS + j) * NP + col0 + ((uint32_t)(quarter * 32) << 16);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float4 sx = *reinterpret_cast<const float4*>(&sx_s[c][col0 + t + 4 * q]);
-          acc[t + 4 * q] = fmaf(__uint_as_float(v[4 * q]), sx.x * sw, acc[t + 4 * q]);
-          acc[t + 4 * q + 1] = fmaf(__uint_as_float(v[4 * q + 1]), sx.y * sw, acc[t + 4 * q + 1]);
-          acc[t + 4 * q + 2] = fmaf(__uint_as_float(v[4 * q + 2]), sx.z * sw, acc[t + 4 * q + 2]);
-          acc[t + 4 * q + 3] = fmaf(__uint_as_float(v[4 * q + 3]), sx.w * sw, acc[t + 4 * q + 3]);
+        for (int t = 0; t < COLS; t += 16) {
+          uint32_t v[16];
+          tmem_ld16(t_row + t, v);
+          tmem_ld_wait();
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float4 sx = *reinterpret_cast<const float4*>(&sx_s[c][col0 + t + 4 * q]);
+            acc[t + 4 * q] = fmaf(__uint_as_float(v[4 * q]), sx.x * sw, acc[t + 4 * q]);
+            acc[t + 4 * q + 1] = fmaf(__uint_as_float(v[4 * q + 1]), sx.y * sw, acc[t + 4 * q + 1]);
+            acc[t + 4 * q + 2] = fmaf(__uint_as_float(v[4 * q + 2]), sx.z * sw, acc[t + 4 * q + 2]);
+            acc[t + 4 * q + 3] = fmaf(__uint_as_float(v[4 * q + 3]), sx.w * sw, acc[t + 4 * q + 3]);
+          }
         }
       }
       fence_before_sync();
       __syncwarp();
-      if (lane == 0) tma::mbar_arrive(&acc_empty[slot]);
+      if (lane == 0) tma::mbar_arrive(&read_bar[stage]);
+      if (RAW && i + STAGES < n_st) raw_store(i + STAGES, raw[0]);
     }
-    // the operands' stages are free now: every copy has arrived and every MMA has read them
-    if (p.split > 1 || GLU) {
-      float* red = reinterpret_cast<float*>(smem);
+    if (p.split == 1 && GLU) {
 #pragma unroll
-      for (int t = 0; t < COLS; ++t) red[(col0 + t) * kTile + row] = acc[t];
-      if (p.split == 1) epilogue_sync(EPI * 32);
-    } else if (!failed && n0 + row < p.N) {
+      for (int t = 0; t < COLS; ++t) sums[(col0 + t) * kTile + row] = acc[t];
+      epilogue_sync(ET);
+    } else if (p.split == 1 && !failed && row < n_out) {
 #pragma unroll
       for (int t = 0; t < COLS; ++t) {
         if (col0 + t >= rows) break;
@@ -253,83 +337,152 @@ gemm_fp8_kernel(Params p, const __grid_constant__ CUtensorMap wmap, const __grid
       }
     }
   }
-  if (p.split > 1) cluster_sync();     // all ranks' sums lie in their shared memory
-  if (live && warp >= 2 && !failed && (p.split > 1 || GLU)) {
-    const uint32_t red = tma::smem_addr(smem);
-    uint32_t from[8];
+  __syncwarp();
+  const int per_rank = (NP + p.split - 1) / p.split;
+  if (p.split > 1) {
+    // row t of x is finished by rank t % split, as its row t / split
+    cluster_sync();                    // every rank's stages are free: its MMAs have read them
+    if (live && warp >= kRoles) {
+      const uint32_t mine = tma::smem_addr(sums) + (uint32_t)(rank * per_rank * kTile + row) * 4;
+      int to = col0 % p.split, at = col0 / p.split;
 #pragma unroll
-    for (int q = 0; q < 8; ++q) from[q] = q < p.split ? (p.split > 1 ? map_to_rank(red, q) : red) : 0;
-    auto total = [&](int t, int r) {
-      float v[8], s = 0.f;
-      const uint32_t off = (uint32_t)(t * kTile + r) * 4;
-#pragma unroll
-      for (int q = 0; q < 8; ++q) v[q] = q < p.split ? ld_cluster(from[q] + off) : 0.f;
-#pragma unroll
-      for (int q = 0; q < 8; ++q) s += v[q];
-      return s;
+      for (int t = 0; t < COLS; ++t) {
+        if (col0 + t < rows) st_cluster(map_to_rank(mine + (uint32_t)at * (kTile * 4), to), acc[t]);
+        if (++to == p.split) { to = 0; ++at; }
+      }
+    }
+    cluster_sync();
+  }
+  if (live && warp >= kRoles && !failed && (p.split > 1 || GLU)) {
+    // four neighbouring outputs a thread and turn
+    const int stride = per_rank * kTile, quads = (n_out + 3) / 4, mine = rows > rank ? (rows - rank + p.split - 1) / p.split : 0;
+    auto total = [&](int at) {                         // over the ranks, whose sums lie `stride` apart
+      float4 v = *reinterpret_cast<const float4*>(sums + at);
+      for (int q = 1; q < p.split; ++q) {
+        const float4 o = *reinterpret_cast<const float4*>(sums + q * stride + at);
+        v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+      }
+      return v;
     };
-    constexpr int PER = GLU ? 64 : 128;                // outputs of a row of x
-    const int e_tid = threadIdx.x - 64, r = e_tid % PER, sub = e_tid / PER, step = EPI * 32 / PER;
-    for (int t = rank + p.split * sub; t < rows; t += p.split * step) {
-      float v = total(t, r);
-      const size_t at = (size_t)(row0 + t) * p.ldy + n0 + r;
+    const int es = p.out_f32 ? 4 : 2;
+    const bool vec = n_out % 4 == 0 && ((uintptr_t)p.y % 16) == 0 && (p.ldy * es) % 16 == 0;
+#pragma unroll 2
+    for (int e = e_tid; e < mine * quads; e += ET) {
+      const int i = e / quads, r = (e - i * quads) * 4, t = rank + p.split * i;
+      const float4 g4 = total(i * kTile + r);
+      float v[4] = {g4.x, g4.y, g4.z, g4.w};
       if (GLU) {
-        float u = total(t, r + 64);
-        if (n0 + r >= p.N) continue;
-        if (p.row_weight) {
-          const float w = p.row_weight[row0 + t];
-          v *= w;
-          u *= w;
+        const float4 u4 = total(i * kTile + R + r);
+        float u[4] = {u4.x, u4.y, u4.z, u4.w};
+        const float w = p.row_weight ? p.row_weight[row0 + t] : 1.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          v[k] *= w;
+          u[k] *= w;
+          if (p.glu.bias && r + k < n_out) {
+            v[k] += p.glu.bias[n0 + r + k];
+            u[k] += p.glu.bias[p.N + n0 + r + k];
+          }
+          v[k] = glu_fast(p.glu, v[k], u[k]);
         }
-        if (p.glu.bias) {
-          v += p.glu.bias[n0 + r];
-          u += p.glu.bias[p.N + n0 + r];
+      }
+      const size_t at = (size_t)(row0 + t) * p.ldy + n0 + r;
+      if (p.out_f32) {
+        float* y = reinterpret_cast<float*>(p.y) + at;
+        if (vec) *reinterpret_cast<float4*>(y) = make_float4(v[0], v[1], v[2], v[3]);
+        else
+          for (int k = 0; k < 4 && r + k < n_out; ++k) y[k] = v[k];
+      } else {
+        __nv_bfloat16* y = reinterpret_cast<__nv_bfloat16*>(p.y) + at;
+        const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
+        if (vec) {
+          *reinterpret_cast<uint2*>(y) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+        } else {
+          const __nv_bfloat16 o[4] = {a.x, a.y, b.x, b.y};
+          for (int k = 0; k < 4 && r + k < n_out; ++k) y[k] = o[k];
         }
-        reinterpret_cast<__nv_bfloat16*>(p.y)[at] = __float2bfloat16_rn(glu_fast(p.glu, v, u));
-      } else if (n0 + r < p.N) {
-        if (p.out_f32) reinterpret_cast<float*>(p.y)[at] = v;
-        else reinterpret_cast<__nv_bfloat16*>(p.y)[at] = __float2bfloat16_rn(v);
       }
     }
   }
-  if (warp == 0 && lane == 0 && failed) {              // copies still on their way to this block's shared memory
-    for (int i = max(0, loaded - STAGES); i < loaded; ++i) tma::mbar_wait(&full_bar[i % STAGES], (i / STAGES) & 1);
-  }
+  if (lane == 0 && (warp == 0 || warp == 2)) started[warp >> 1] = max(loaded, warp == 0 && p.n_groups == 0 ? min(STAGES, n_st) : 0);
   fence_before_sync();
   __syncthreads();
-  if (p.split > 1) cluster_sync();     // nobody reads this block's sums any more
+  if (failed && threadIdx.x == 0) {    // copies still on their way to this block's shared memory
+    // (with RAW the epilogue has converted every stage all the same: only weights can be missing)
+    const int last = RAW ? n_st : max(started[0], started[1]);
+    for (int i = max(0, last - STAGES); i < last; ++i) {
+      if (i >= started[0] || (!RAW && i >= started[1])) tma::mbar_arrive(&full_bar[i % STAGES]);     // for the operand that was not asked for
+      tma::mbar_wait(&full_bar[i % STAGES], (i / STAGES) & 1);
+    }
+  }
   if (warp == 1) {
     fence_after_sync();
-    tmem_dealloc<1>(tmem_base, kTmemCols);
+    tmem_dealloc<1>(tmem_base, S::kTmem);
   }
 }
 
-template <int NP, bool GLU>
+// The weights as [group][block][half][row][128] (half: gates and ups; see fp8::make_map): a copy brings KBS blocks of a tile.
+static int make_weight_map(CUtensorMap* map, const void* w, const Params& p, uint64_t ld, bool glu, int groups, uint32_t kbs) {
+  tma::EncodeTiledFn fn = tma::encode_fn();
+  if (fn == nullptr) return -5;
+  const uint64_t halves = glu ? 2 : 1;
+  cuuint64_t dims[5] = {p.whole ? (uint64_t)BK : p.K, (uint64_t)p.N, halves, p.whole ? (uint64_t)p.k_blocks : 1, (uint64_t)groups};
+  cuuint64_t strides[4] = {ld, (uint64_t)p.N * ld, (uint64_t)(p.whole ? BK : ld), halves * p.N * ld};
+  cuuint32_t box[5] = {BK, (cuuint32_t)p.tile_rows, (cuuint32_t)halves, p.whole ? kbs : 1, 1};
+  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, const_cast<void*>(w), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : -2;
+}
+
+// How a product is cut: weight rows of a tile, token tiles, thread blocks that share K.
+struct Cut {
+  int rows, tok_tiles, split;
+  long long blocks;
+  int waves_blocks;                    // k blocks one after the other on an SM, over all waves
+};
+static Cut cut_of(int M, int N, int k_blocks, int n_groups, int np, bool glu) {
+  const int places = (np == 128 ? 1 : 2) * kSMs, full = glu ? kTile / 2 : kTile;
+  Cut c;
+  // with groups: every group's last tile may be partly empty, and no more tiles than rows
+  c.tok_tiles = n_groups > 0 ? M / np + (n_groups < M ? n_groups : M) : (M + np - 1) / np;
+  auto tiles_of = [&](int rows) { return (long long)((N + rows - 1) / rows) * c.tok_tiles; };
+  c.rows = full;
+  c.split = 1;
+  // Clusters of 2, 4 or 8: those of 3 or 6 do not pack into the chip (6,144 x 4,096, 8 rows: 7.5 us with 4, 9.0 with 3, 12.8 with 6).
+  while (c.split < 8 && tiles_of(full) * c.split * 2 <= places && c.split * 2 * 2 <= k_blocks) c.split *= 2;
+  // Where the tiles fill the places once and not to the end, smaller ones spread the weights evenly (12,288 gates of 4,096, 8 rows:
+  // 19.1 us with 48 rows a tile, 20.8 with 64).
+  if (c.split == 1)
+    while (c.rows > full / 2 && tiles_of(c.rows - 8) <= places) c.rows -= 8;
+  c.blocks = tiles_of(c.rows) * c.split;
+  c.waves_blocks = (int)((c.blocks + kSMs - 1) / kSMs) * ((k_blocks + c.split - 1) / c.split);
+  return c;
+}
+
+template <int NP, bool GLU, bool RAW = false>
 static int launch_np(Params p, const void* x, long long x_ld, long long x_rows, const void* w, long long w_ld, cudaStream_t stream) {
   using S = Shape<NP>;
   const int groups = p.n_groups > 0 ? p.n_groups : 1;
-  const int per = GLU ? kTile / 2 : kTile;
-  const long long row_tiles = (p.N + per - 1) / per;
-  // with groups: every group's last tile may be partly empty, and no more tiles than rows
-  p.tok_tiles = p.n_groups > 0 ? p.M / NP + (p.n_groups < p.M ? p.n_groups : p.M) : (p.M + NP - 1) / NP;
-  const long long tiles = row_tiles * p.tok_tiles;
-  // K is split until a thread block for every SM's two places exists
-  int split = 1;
-  while (split < 8 && tiles * (split + 1) <= 2 * kSMs && (split + 1) * 4 <= p.k_blocks) ++split;
-  p.split = split;
-  if (tiles * split > 0x7fffffffLL) return PE_ERR_UNSUPPORTED_SIZE;
+  const Cut c = cut_of(p.M, p.N, p.k_blocks, p.n_groups, NP, GLU);
+  p.tile_rows = c.rows;
+  p.tok_tiles = c.tok_tiles;
+  const int split = p.split = c.split;
+  if (c.blocks > 0x7fffffffLL) return PE_ERR_UNSUPPORTED_SIZE;
   CUtensorMap wmap, xmap;
-  int e = make_map(&wmap, w, p.K, (uint64_t)groups * p.w_rows, w_ld, GLU ? kTile / 2 : kTile);
-  if (e == 0) e = make_map(&xmap, x, p.K, x_rows, x_ld, NP);
+  int e = make_weight_map(&wmap, w, p, w_ld, GLU, groups, S::kKbs);
+  if (e == 0 && !RAW) e = make_map(&xmap, x, p.K, x_rows, x_ld, NP, p.whole, S::kKbs);
   if (e != 0) return e;
+  if (RAW) xmap = wmap;                // not used
   static bool attr_set = false;
   if (!attr_set) {
-    cudaError_t ce = cudaFuncSetAttribute(gemm_fp8_kernel<NP, GLU>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem);
+    cudaError_t ce = cudaFuncSetAttribute(gemm_fp8_kernel<NP, GLU, RAW>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem);
     if (ce != cudaSuccess) return (int)ce;
     attr_set = true;
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(tiles * split));
+  cfg.gridDim = dim3((unsigned)c.blocks);
   cfg.blockDim = dim3(S::kThreads);
   cfg.dynamicSmemBytes = S::kSmem;
   cfg.stream = stream;
@@ -349,7 +502,7 @@ static int launch_np(Params p, const void* x, long long x_ld, long long x_rows, 
   }
   cfg.attrs = attr;
   cfg.numAttrs = n_attr;
-  cudaError_t ce = cudaLaunchKernelEx(&cfg, gemm_fp8_kernel<NP, GLU>, p, wmap, xmap);
+  cudaError_t ce = cudaLaunchKernelEx(&cfg, gemm_fp8_kernel<NP, GLU, RAW>, p, wmap, xmap);
   if (ce != cudaSuccess) return (int)ce;
   PE_LAUNCH_CHECK();
   return PE_OK;
@@ -357,6 +510,59 @@ static int launch_np(Params p, const void* x, long long x_ld, long long x_rows, 
 
 }  // namespace fp8
 }  // namespace pe
+
+// Whether bfloat16 rows are quantised inside the product: up to 16 rows (of an average group).
+static bool takes_raw(int M, int n_groups) { return (n_groups > 0 ? (M + n_groups - 1) / n_groups : M) <= 16; }
+
+// raw: x is bfloat16, x_ld in elements, x_scales unused.
+static int product(bool raw, const void* x, long long x_ld, const float* x_scales, long long xs_ld, const void* w, long long w_ld,
+                   const float* w_scales, void* y, long long ldy, int M, int N, int K, int out_f32, int kind, float limit, float alpha,
+                   const float* bias, const float* row_weight, const int* offsets, int n_groups, int* status, cudaStream_t stream) {
+  using namespace pe::fp8;
+  if (M < 0 || N < 0 || K < 1 || kind < 0 || kind > 3 || n_groups < 0) return PE_ERR_BAD_ARGUMENT;
+  if (M == 0 || N == 0) return PE_OK;
+  if (x == nullptr || (!raw && x_scales == nullptr) || w == nullptr || w_scales == nullptr || y == nullptr) return PE_ERR_BAD_ARGUMENT;
+  if (x_ld < K || w_ld < K || (!raw && xs_ld < M) || ldy < N || (kind > 0 && out_f32) || (kind == 0 && (bias || row_weight)))
+    return PE_ERR_BAD_ARGUMENT;
+  if ((n_groups > 0) != (offsets != nullptr)) return PE_ERR_BAD_ARGUMENT;
+  if (((uintptr_t)x % 16) || ((uintptr_t)w % 16) || (x_ld * (raw ? 2 : 1)) % 16 || (w_ld % 16)) return PE_ERR_BAD_ARGUMENT;
+  if (N > (1 << 28) || (long long)(n_groups > 0 ? n_groups : 1) * N > (1 << 29)) return PE_ERR_UNSUPPORTED_SIZE;
+  const int rows = n_groups > 0 ? (M + n_groups - 1) / n_groups : M;     // of an average group
+  const int k_blocks = (K + BK - 1) / BK;
+  // Many rows: tiles of 128 x 256 (gemm_fp8_many.cu) where they take no longer.  A block of K takes an SM 0.60 us there and 0.55 us in
+  // this file's tiles of 128 x 128, which can share K out (4,096 x 6,144, both files' times in us: 128 rows 24.4 and 15.6, 384 rows 24.8
+  // and 21.7, 512 rows 26.2 and 42.9; 12,288 x 4,096: 512 rows 60.1 and 56.0, 700 rows 62.9 and 107.9).
+  if (n_groups == 0 && !row_weight && M > 64 && (kind == 0 || N % 128 == 0)) {
+    const long long tiles = ((M + 127) / 128) * (long long)(kind > 0 ? N / 128 : (N + 255) / 256);
+    const Cut c = cut_of(M, N, k_blocks, 0, 128, kind > 0);
+    if (11 * ((tiles + pe::kSMs - 1) / pe::kSMs) * k_blocks <= 10LL * c.waves_blocks)
+      return pe_gemm_fp8_many(x, x_ld, x_scales, xs_ld, w, w_ld, w_scales, y, ldy, nullptr, 0, M, N, K, out_f32, kind, limit, alpha, bias,
+                              status, stream);
+  }
+  Params p;
+  p.M = M; p.N = N; p.K = K; p.k_blocks = k_blocks; p.whole = K % BK == 0;
+  p.xs = x_scales; p.xs_ld = xs_ld; p.ws = w_scales;
+  p.x = (const __nv_bfloat16*)x; p.x_ld = x_ld;
+  p.w_rows = kind > 0 ? 2 * N : N;
+  p.ws_group = (long long)((p.w_rows + 127) / 128) * p.k_blocks;
+  p.y = y; p.ldy = ldy; p.out_f32 = out_f32;
+  p.offsets = offsets; p.n_groups = n_groups;
+  p.glu = pe::GluEpilogue{kind, limit, alpha, bias};
+  p.row_weight = row_weight;
+  p.status = status;
+  if (raw) {
+    if (rows > 16) return PE_ERR_UNSUPPORTED_SIZE;
+    return kind > 0 ? launch_np<16, true, true>(p, x, x_ld, M, w, w_ld, stream) : launch_np<16, false, true>(p, x, x_ld, M, w, w_ld, stream);
+  }
+#define PE_FP8_LAUNCH(NP) \
+  return kind > 0 ? launch_np<NP, true>(p, x, x_ld, M, w, w_ld, stream) : launch_np<NP, false>(p, x, x_ld, M, w, w_ld, stream)
+  // the least tile of rows that holds them all, for groups what an average group has
+  if (rows <= 16) PE_FP8_LAUNCH(16);
+  if (rows <= 32) PE_FP8_LAUNCH(32);
+  if (rows <= 64) PE_FP8_LAUNCH(64);
+  PE_FP8_LAUNCH(128);
+#undef PE_FP8_LAUNCH
+}
 
 // x: M rows of K bytes, x_ld apart; x_scales[b * xs_ld + m]; w: n_groups (0: 1) matrices of N (kind > 0: 2 N, gates then ups) rows,
 // w_ld apart; w_scales packed, [group][ceil(rows / 128)][ceil(K / 128)]; kind 0: y = the product, bfloat16 or float32; 1 to 3:
@@ -367,31 +573,30 @@ extern "C" int pe_gemm_fp8(const void* x, long long x_ld, const float* x_scales,
                            const float* w_scales, void* y, long long ldy, int M, int N, int K, int out_f32, int kind, float limit,
                            float alpha, const float* bias, const float* row_weight, const int* offsets, int n_groups, int* status,
                            cudaStream_t stream) {
-  using namespace pe::fp8;
-  if (M < 0 || N < 0 || K < 1 || kind < 0 || kind > 3 || n_groups < 0) return PE_ERR_BAD_ARGUMENT;
+  return product(false, x, x_ld, x_scales, xs_ld, w, w_ld, w_scales, y, ldy, M, N, K, out_f32, kind, limit, alpha, bias, row_weight,
+                 offsets, n_groups, status, stream);
+}
+
+// pe_gemm_fp8 of rows in bfloat16 or float32, which are quantised first (pe_quantize_rows_fp8's dtype, x, x_ld, row_map, x_rows; with
+// groups only the rows below offsets[n_groups]): into `scratch` (16-byte aligned), M rows of ceil(K / 16) * 16 bytes and behind them
+// ceil(K / 128) * M floats; or, with scratch null, inside the product: bfloat16 rows on 16-byte boundaries, up to 16 (of an average
+// group), no row map.
+extern "C" int pe_linear_fp8(int dtype, const void* x, long long x_ld, const int* row_map, int x_rows, void* scratch, const void* w,
+                             long long w_ld, const float* w_scales, void* y, long long ldy, int M, int N, int K, int out_f32, int kind,
+                             float limit, float alpha, const float* bias, const float* row_weight, const int* offsets, int n_groups,
+                             int* status, cudaStream_t stream) {
+  if (M < 0 || N < 0 || K < 1 || n_groups < 0) return PE_ERR_BAD_ARGUMENT;
   if (M == 0 || N == 0) return PE_OK;
-  if (x == nullptr || x_scales == nullptr || w == nullptr || w_scales == nullptr || y == nullptr) return PE_ERR_BAD_ARGUMENT;
-  if (x_ld < K || w_ld < K || xs_ld < M || ldy < N || (kind > 0 && out_f32) || (kind == 0 && (bias || row_weight))) return PE_ERR_BAD_ARGUMENT;
-  if ((n_groups > 0) != (offsets != nullptr)) return PE_ERR_BAD_ARGUMENT;
-  if (((uintptr_t)x % 16) || ((uintptr_t)w % 16) || (x_ld % 16) || (w_ld % 16)) return PE_ERR_BAD_ARGUMENT;
-  if (N > (1 << 28) || (long long)(n_groups > 0 ? n_groups : 1) * N > (1 << 29)) return PE_ERR_UNSUPPORTED_SIZE;
-  Params p;
-  p.M = M; p.N = N; p.K = K; p.k_blocks = (K + BK - 1) / BK;
-  p.xs = x_scales; p.xs_ld = xs_ld; p.ws = w_scales;
-  p.w_rows = kind > 0 ? 2 * N : N;
-  p.ws_group = (long long)((p.w_rows + 127) / 128) * p.k_blocks;
-  p.y = y; p.ldy = ldy; p.out_f32 = out_f32;
-  p.offsets = offsets; p.n_groups = n_groups;
-  p.glu = pe::GluEpilogue{kind, limit, alpha, bias};
-  p.row_weight = row_weight;
-  p.status = status;
-  // rows of a tile: the least that hold them all, for groups what an average group has
-  const int rows = n_groups > 0 ? (M + n_groups - 1) / n_groups : M;
-#define PE_FP8_LAUNCH(NP) \
-  return kind > 0 ? launch_np<NP, true>(p, x, x_ld, M, w, w_ld, stream) : launch_np<NP, false>(p, x, x_ld, M, w, w_ld, stream)
-  if (rows <= 16) PE_FP8_LAUNCH(16);
-  if (rows <= 32) PE_FP8_LAUNCH(32);
-  if (rows <= 64) PE_FP8_LAUNCH(64);
-  PE_FP8_LAUNCH(128);
-#undef PE_FP8_LAUNCH
+  if (scratch == nullptr) {
+    if (dtype != PE_BF16 || row_map != nullptr || !takes_raw(M, n_groups)) return PE_ERR_BAD_ARGUMENT;
+    return product(true, x, x_ld, nullptr, 0, w, w_ld, w_scales, y, ldy, M, N, K, out_f32, kind, limit, alpha, bias, row_weight, offsets,
+                   n_groups, status, stream);
+  }
+  const long long ld = ((long long)K + 15) / 16 * 16;
+  float* scales = reinterpret_cast<float*>(reinterpret_cast<char*>(scratch) + ld * M);
+  const int e = pe_quantize_rows_fp8(dtype, x, x_ld, row_map, n_groups > 0 ? offsets + n_groups : nullptr, scratch, ld, scales, M, M, K,
+                                     x_rows, status, stream);
+  if (e != PE_OK) return e;
+  return pe_gemm_fp8(scratch, ld, scales, M, w, w_ld, w_scales, y, ldy, M, N, K, out_f32, kind, limit, alpha, bias, row_weight, offsets,
+                     n_groups, status, stream);
 }

@@ -1,0 +1,395 @@
+// gemm_fp8.cu's products for many rows: y = x . W^T of e4m3 operands with a scale for each block of 128, in tiles of 128 rows of x
+// and 256 weight rows.
+//
+//   y[m, n] = sum_b sx[b, m] * sw[n / 128, b] * sum_{k in block b} x[m, k] * w[n, k]
+//
+// A k block of 128 is four MMAs (tcgen05.mma kind::f8f6f4) into one of two halves of tensor memory (256 columns), and its sums are
+// added up in registers while the next block's MMAs fill the other half.  The rows of x are the MMA's M dimension, so that an
+// epilogue thread owns one row: 128 of its columns lie in one block of weight rows, and a block of 128 x 128 outputs takes one
+// multiply-add an output with one number a thread, sx * sw.
+//
+// What bounds it is the way round a half of tensor memory: MMAs, commit, eight warps that read it, their arrival, the next MMAs.
+// Two SMs on one tile (cta_group::2) load a third less but have that way lead through the other SM: 1,750 cycles a block and
+// half, one SM 1,050.
+//
+// GLU: the tile's weight rows are 128 gates and the 128 ups that belong to them, a thread owns 64 of each, and act(gate, up),
+// rounded to bfloat16, goes out as it is or quantised again: the tile's 128 outputs of a row are one block, whose largest
+// magnitude two threads find together.
+//
+// Roles: warps 0 and 1 copy x and the weights (TMA; a thread starts a copy only every 150 ns or so), warp 2 allocates tensor memory
+// and issues the MMAs, warps 3 to 10 are the epilogue.
+//
+// Every wait is bounded; one that runs out records kStatusWaitTimedOut, every role leaves its loop, copies still in flight are
+// waited for (bounded again) and tensor memory is freed.
+#include "api.h"
+#include "fp8.cuh"
+
+namespace pe {
+namespace fp8many {
+using namespace fp8;
+
+constexpr int BM = 128;          // rows of x of a tile
+constexpr int BN = 256;          // weight rows of a tile
+constexpr int STAGES = 4;        // of one k block
+constexpr int kBytesA = BM * BK, kBytesB = BN * BK, kStage = kBytesA + kBytesB;
+constexpr int kTmemCols = 512;
+constexpr int kRoles = 3, kThreads = 32 * (kRoles + 8);
+constexpr size_t kSmem = 1024 + (size_t)STAGES * kStage;
+
+__device__ long long g_trace[16][128];
+#define TR(r,i) do { if (blockIdx.x==0 && (i)<128) g_trace[r][i]=clock64(); } while(0)
+enum Mode { kBf16 = 0, kF32 = 1, kGlu = 2, kGluFp8 = 3 };
+
+struct Params {
+  int M, N, K, k_blocks;                // N: output columns
+  bool whole;
+  const float* xs; long long xs_ld;
+  const float* ws;                      // [ceil(w rows / 128)][k_blocks]
+  void* y; long long ldy;
+  float* ys; long long ys_ld;           // kGluFp8: scales of the outputs, [block][row]
+  int m_tiles, n_tiles;
+  GluEpilogue glu;
+  int* status;
+};
+
+__device__ __forceinline__ void load_4d(void* dst, const CUtensorMap* map, int x, int row, int block, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n"
+      ::"r"(tma::smem_addr(dst)), "l"(map), "r"(x), "r"(row), "r"(0), "r"(block), "r"(tma::smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+template <int MODE>
+__global__ void __launch_bounds__(kThreads, 1)
+gemm_fp8_many_kernel(Params p, const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap) {
+  constexpr bool GLU = MODE == kGlu || MODE == kGluFp8;
+  extern __shared__ char smem_raw[];
+  __shared__ uint64_t full_bar[STAGES], empty_bar[STAGES], acc_full[2], acc_empty[2];
+  __shared__ float top_s[2][BM];
+  __shared__ uint32_t tmem_holder;
+  __shared__ volatile int failed;
+  __shared__ int started[2];
+  char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n_tiles_total = p.m_tiles * p.n_tiles;
+  constexpr int kPerTile = GLU ? BN / 2 : BN;     // outputs of a row in a tile
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      tma::mbar_init(&full_bar[s], 2);    // the two producers
+      tma::mbar_init(&empty_bar[s], 1);   // the commit behind a block's MMAs
+    }
+    for (int b = 0; b < 2; ++b) {
+      tma::mbar_init(&acc_full[b], 1);
+      tma::mbar_init(&acc_empty[b], 8);   // the epilogue's warps
+    }
+    failed = 0;
+    tma::fence_barrier_init();
+  }
+  if (warp == 2) tmem_alloc<1>(&tmem_holder, kTmemCols);
+  fence_before_sync();
+  pdl_wait_block();
+  pdl_launch_dependents();
+  fence_after_sync();
+  const uint32_t tmem_base = tmem_holder;
+
+  int loaded = 0;                         // warps 0 and 1: blocks whose copies were started
+  if (warp < 2) {
+    if (lane == 0) {
+      for (int tile = blockIdx.x; tile < n_tiles_total && !failed; tile += gridDim.x) {
+        const int m0 = (tile % p.m_tiles) * BM, n0 = (tile / p.m_tiles) * kPerTile;
+        for (int kb = 0; kb < p.k_blocks; ++kb, ++loaded) {
+          const int stage = loaded % STAGES;
+          if (!tma::mbar_wait(&empty_bar[stage], ((loaded / STAGES) & 1) ^ 1)) {
+            report(p.status, kStatusWaitTimedOut, 90, tile, kb);
+            failed = 1;
+            break;
+          }
+          char* to = smem + stage * kStage;
+          const int x = p.whole ? 0 : kb * BK, z = p.whole ? kb : 0;
+          if (warp == 0) {
+            tma::mbar_expect_tx(&full_bar[stage], kBytesA);
+            load_3d(to, &amap, x, m0, z, &full_bar[stage]);
+          } else {
+            tma::mbar_expect_tx(&full_bar[stage], kBytesB);
+            load_4d(to + kBytesA, &bmap, x, n0, z, &full_bar[stage]);
+          }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 2) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = instr_desc(BM, BN);
+      const int my_tiles = (n_tiles_total - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
+      const int total = my_tiles * p.k_blocks;      // k blocks: block `it` goes to half it & 1 of tensor memory
+      const uint32_t base = tma::smem_addr(smem);
+      for (int it0 = 0; it0 < total && !failed; it0 += STAGES) {
+#pragma unroll
+        for (int stage = 0; stage < STAGES; ++stage) {
+          const int it = it0 + stage, half = stage & 1;
+          if (it >= total) break;
+          if (!tma::mbar_wait(&full_bar[stage], (it / STAGES) & 1)) failed = 1;
+          TR(0,it);
+          if (!tma::mbar_wait(&full_bar[stage], (it / STAGES) & 1) || !tma::mbar_wait(&acc_empty[half], ((it >> 1) & 1) ^ 1)) {
+            report(p.status, kStatusWaitTimedOut, 91, (int)blockIdx.x, it);
+            failed = 1;
+            break;
+          }
+          TR(1,it);
+          fence_after_sync();
+          const uint32_t sa = base + stage * kStage, sb = sa + kBytesA;
+#pragma unroll
+          for (int k = 0; k < BK / 32; ++k)
+            umma(tmem_base + half * BN, smem_desc(sa + k * 32), smem_desc(sb + k * 32), idesc, k > 0 ? 1u : 0u);
+          umma_commit(&acc_full[half]);
+          umma_commit(&empty_bar[stage]);
+          TR(2,it);
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---- epilogue: a warp owns a quarter of the rows (the tensor memory lanes that it may read) and half of the columns: 128
+    // neighbouring ones, or with GLU 64 gates and their 64 ups ----
+    const int quarter = warp & 3, h = (warp - kRoles) >> 2;
+    const int r_tile = quarter * 32 + lane;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    // first columns of the thread's two runs of 64
+    const int c0 = GLU ? h * 64 : h * 128, c1 = GLU ? 128 + h * 64 : h * 128 + 64;
+    int it = 0;
+    // the fused conversion has barriers in it: after a wait that ran out the warps go on without waiting
+    for (int tile = blockIdx.x; tile < n_tiles_total; tile += gridDim.x) {
+      const int m0 = (tile % p.m_tiles) * BM, n0 = (tile / p.m_tiles) * kPerTile;
+      const int row = m0 + r_tile;
+      const bool live = row < p.M;
+      const float* sx_p = p.xs + (live ? row : 0);
+      const int last = ((GLU ? 2 * p.N : p.N) - 1) / 128;
+      const float* sw0_p = p.ws + (size_t)min(GLU ? n0 / 128 : (n0 + c0) / 128, last) * p.k_blocks;
+      const float* sw1_p = p.ws + (size_t)min(GLU ? (p.N + n0) / 128 : (n0 + c0) / 128, last) * p.k_blocks;
+      unsigned long long sums[64];        // 128 sums, two neighbouring ones each
+#pragma unroll
+      for (int j = 0; j < 64; ++j) sums[j] = 0ull;
+      float sx = live ? sx_p[0] : 0.f, sw0 = sw0_p[0], sw1 = GLU ? sw1_p[0] : 0.f;
+      for (int kb = 0; kb < p.k_blocks; ++kb, ++it) {
+        const int half = it & 1;
+        const unsigned long long ss0 = pair_of(sx * sw0, sx * sw0), ss1 = GLU ? pair_of(sx * sw1, sx * sw1) : ss0;
+        if (kb + 1 < p.k_blocks) {        // the next block's scales are on their way during this one
+          sx = live ? sx_p[(size_t)(kb + 1) * p.xs_ld] : 0.f;
+          sw0 = sw0_p[kb + 1];
+          if (GLU) sw1 = sw1_p[kb + 1];
+        }
+        if (!failed && !tma::mbar_wait(&acc_full[half], (it >> 1) & 1)) {
+          if (lane == 0) report(p.status, kStatusWaitTimedOut, 92, tile, kb);
+          failed = 1;
+        }
+        __syncwarp();
+        if(lane==0 && warp==3) TR(3,it);
+        fence_after_sync();
+        const uint32_t t_row = tmem_base + half * BN + lanes;
+        uint32_t v[2][16];
+        tmem_ld16(t_row + c0, v[0]);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          tmem_ld_wait();
+          if (q < 7) tmem_ld16(t_row + (q + 1 < 4 ? c0 + (q + 1) * 16 : c1 + (q - 3) * 16), v[(q + 1) & 1]);
+          if (q == 7) {                   // all of the half is read: hand it back
+            if(lane==0) TR(warp+1,it);
+            fence_before_sync();
+            __syncwarp();
+            if (lane == 0) tma::mbar_arrive(&acc_empty[half]);
+          }
+          const unsigned long long s = q < 4 ? ss0 : ss1;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) fma2(sums[q * 8 + j], v[q & 1][2 * j], v[q & 1][2 * j + 1], s);
+        }
+      }
+      float acc[128];
+#pragma unroll
+      for (int j = 0; j < 64; ++j) {
+        const float2 f = unpair(sums[j]);
+        acc[2 * j] = f.x;
+        acc[2 * j + 1] = f.y;
+      }
+      if constexpr (!GLU) {
+        if (live && !failed) {
+          const int left = p.N - (n0 + c0);
+          if (MODE == kF32) {
+            float* y = reinterpret_cast<float*>(p.y) + (size_t)row * p.ldy + n0 + c0;
+            const bool vec = ((uintptr_t)p.y % 16) == 0 && p.ldy % 4 == 0;
+#pragma unroll
+            for (int j = 0; j < 128; j += 4) {
+              if (vec && j + 4 <= left) {
+                *reinterpret_cast<float4*>(y + j) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+              } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  if (j + k < left) y[j + k] = acc[j + k];
+              }
+            }
+          } else {
+            __nv_bfloat16* y = reinterpret_cast<__nv_bfloat16*>(p.y) + (size_t)row * p.ldy + n0 + c0;
+            const bool vec = ((uintptr_t)p.y % 16) == 0 && p.ldy % 8 == 0;
+#pragma unroll
+            for (int j = 0; j < 128; j += 8) {
+              if (vec && j + 8 <= left) {
+                *reinterpret_cast<uint4*>(y + j) = make_uint4(pack2(acc[j], acc[j + 1]), pack2(acc[j + 2], acc[j + 3]),
+                                                              pack2(acc[j + 4], acc[j + 5]), pack2(acc[j + 6], acc[j + 7]));
+              } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                  if (j + k < left) y[j + k] = __float2bfloat16_rn(acc[j + k]);
+              }
+            }
+          }
+        }
+      } else {
+        // N is a multiple of 128 here: the tile's outputs are all there
+        uint32_t o[32];                   // 64 outputs as bfloat16
+        if (p.glu.kind == 1 && p.glu.bias == nullptr) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) o[j] = pack2(silu_mul_fast(acc[2 * j], acc[64 + 2 * j]), silu_mul_fast(acc[2 * j + 1], acc[64 + 2 * j + 1]));
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            float g[2] = {acc[2 * j], acc[2 * j + 1]}, u[2] = {acc[64 + 2 * j], acc[64 + 2 * j + 1]};
+            if (p.glu.bias) {
+              const int col = n0 + c0 + 2 * j;
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                g[k] += p.glu.bias[col + k];
+                u[k] += p.glu.bias[p.N + col + k];
+              }
+            }
+            o[j] = glu_fast_pair(p.glu, g[0], g[1], u[0], u[1]);
+          }
+        }
+        if (MODE == kGlu) {
+          if (live) {
+            __nv_bfloat16* y = reinterpret_cast<__nv_bfloat16*>(p.y) + (size_t)row * p.ldy + n0 + c0;
+            if (((uintptr_t)p.y % 16) == 0 && p.ldy % 8 == 0) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) reinterpret_cast<uint4*>(y)[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                y[2 * j] = reinterpret_cast<const __nv_bfloat162*>(o)[j].x;
+                y[2 * j + 1] = reinterpret_cast<const __nv_bfloat162*>(o)[j].y;
+              }
+            }
+          }
+        } else {
+          float top = 0.f;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const float2 f = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(o)[j]);
+            top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+          }
+          top_s[h][r_tile] = top;         // the other half of the row's 128 outputs is another warp's
+          asm volatile("bar.sync 1, 256;\n" ::: "memory");
+          top = fmaxf(top_s[0][r_tile], top_s[1][r_tile]);
+          const uint32_t scale = scale_bits(top);
+          const float by = inverse_of(scale);
+          const bool inf = top == INFINITY;
+          uint32_t q8[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const float2 a = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(o)[2 * j]);
+            const float2 b = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(o)[2 * j + 1]);
+            q8[j] = inf ? pack4(no_infinity(a.x) * by, no_infinity(a.y) * by, no_infinity(b.x) * by, no_infinity(b.y) * by)
+                        : pack4(a.x * by, a.y * by, b.x * by, b.y * by);
+          }
+          if (live) {
+            uint4* y = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(p.y) + (size_t)row * p.ldy + n0 + c0);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] = make_uint4(q8[4 * j], q8[4 * j + 1], q8[4 * j + 2], q8[4 * j + 3]);
+            if (h == 0) p.ys[(size_t)(n0 / 128) * p.ys_ld + row] = __uint_as_float(scale);
+          }
+          asm volatile("bar.sync 1, 256;\n" ::: "memory");     // the next tile writes top_s again
+        }
+      }
+    }
+  }
+  if (warp < 2 && lane == 0) started[warp] = loaded;
+  fence_before_sync();
+  __syncthreads();
+  if (failed && threadIdx.x == 0) {       // copies still on their way to this block's shared memory
+    const int last = max(started[0], started[1]);
+    for (int i = max(0, last - STAGES); i < last; ++i) {
+      if (i >= started[0] || i >= started[1]) tma::mbar_arrive(&full_bar[i % STAGES]);     // for the operand that was not asked for
+      tma::mbar_wait(&full_bar[i % STAGES], (i / STAGES) & 1);
+    }
+  }
+  if (warp == 2) {
+    fence_after_sync();
+    tmem_dealloc<1>(tmem_base, kTmemCols);
+  }
+}
+
+// The weights as [block][half][row][128] (half: gates and ups; see fp8::make_map): a copy brings a block of a tile.
+static int make_weight_map(CUtensorMap* map, const void* w, const Params& p, uint64_t ld, bool glu) {
+  tma::EncodeTiledFn fn = tma::encode_fn();
+  if (fn == nullptr) return -5;
+  const cuuint32_t halves = glu ? 2 : 1;
+  cuuint64_t dims[4] = {p.whole ? (uint64_t)BK : p.K, (uint64_t)p.N, halves, p.whole ? (uint64_t)p.k_blocks : 1};
+  cuuint64_t strides[3] = {ld, (uint64_t)p.N * ld, (uint64_t)(p.whole ? BK : ld)};
+  cuuint32_t box[4] = {BK, BN / halves, halves, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(w), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : -2;
+}
+
+template <int MODE>
+static int launch_mode(const Params& p, const CUtensorMap& amap, const CUtensorMap& bmap, cudaStream_t stream) {
+  static bool attr_set = false;
+  if (!attr_set) {
+    const cudaError_t ce = cudaFuncSetAttribute(gemm_fp8_many_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
+    if (ce != cudaSuccess) return (int)ce;
+    attr_set = true;
+  }
+  const int tiles = p.m_tiles * p.n_tiles;
+  const cudaError_t ce = pe::launch(gemm_fp8_many_kernel<MODE>, dim3(tiles < pe::kSMs ? tiles : pe::kSMs), dim3(kThreads), kSmem, stream, p, amap, bmap);
+  if (ce != cudaSuccess) return (int)ce;
+  PE_LAUNCH_CHECK();
+  return PE_OK;
+}
+
+}  // namespace fp8many
+}  // namespace pe
+
+// The arguments of pe_gemm_fp8 (gemm_fp8.cu) without groups; with an activation N is a multiple of 128.  y_scales (or null): the outputs
+// are quantised again, y is e4m3 (ldy bytes between rows, a multiple of 16) and y_scales[b * ys_ld + m] their blocks' scales.
+extern "C" int pe_gemm_fp8_many(const void* x, long long x_ld, const float* x_scales, long long xs_ld, const void* w, long long w_ld,
+                                const float* w_scales, void* y, long long ldy, float* y_scales, long long ys_ld, int M, int N, int K,
+                                int out_f32, int kind, float limit, float alpha, const float* bias, int* status, cudaStream_t stream) {
+  using namespace pe::fp8many;
+  if (M < 0 || N < 0 || K < 1 || kind < 0 || kind > 3) return PE_ERR_BAD_ARGUMENT;
+  if (M == 0 || N == 0) return PE_OK;
+  if (x == nullptr || x_scales == nullptr || w == nullptr || w_scales == nullptr || y == nullptr) return PE_ERR_BAD_ARGUMENT;
+  if (x_ld < K || w_ld < K || xs_ld < M || ldy < N || (kind > 0 && out_f32) || (kind == 0 && (bias || y_scales))) return PE_ERR_BAD_ARGUMENT;
+  if (((uintptr_t)x % 16) || ((uintptr_t)w % 16) || (x_ld % 16) || (w_ld % 16)) return PE_ERR_BAD_ARGUMENT;
+  if (y_scales && ((ldy % 16) || ((uintptr_t)y % 16) || ys_ld < M)) return PE_ERR_BAD_ARGUMENT;
+  if ((kind > 0 && N % 128) || N > (1 << 28)) return PE_ERR_UNSUPPORTED_SIZE;
+  Params p;
+  p.M = M; p.N = N; p.K = K; p.k_blocks = (K + BK - 1) / BK; p.whole = K % BK == 0;
+  p.xs = x_scales; p.xs_ld = xs_ld; p.ws = w_scales;
+  p.y = y; p.ldy = ldy; p.ys = y_scales; p.ys_ld = ys_ld;
+  p.m_tiles = (M + BM - 1) / BM;
+  p.n_tiles = kind > 0 ? N / (BN / 2) : (N + BN - 1) / BN;
+  p.glu = pe::GluEpilogue{kind, limit, alpha, bias};
+  p.status = status;
+  if ((long long)p.m_tiles * p.n_tiles > 0x7fffffffLL) return PE_ERR_UNSUPPORTED_SIZE;
+  CUtensorMap amap, bmap;
+  int e = make_map(&amap, x, K, M, x_ld, BM, p.whole, 1);
+  if (e == 0) e = make_weight_map(&bmap, w, p, w_ld, kind > 0);
+  if (e != 0) return e;
+  if (kind == 0) return out_f32 ? launch_mode<kF32>(p, amap, bmap, stream) : launch_mode<kBf16>(p, amap, bmap, stream);
+  return y_scales ? launch_mode<kGluFp8>(p, amap, bmap, stream) : launch_mode<kGlu>(p, amap, bmap, stream);
+}
+
+extern "C" int trace_get(long long* out) { return (int)cudaMemcpyFromSymbol(out, pe::fp8many::g_trace, sizeof(long long)*16*128); }

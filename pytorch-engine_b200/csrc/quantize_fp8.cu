@@ -9,29 +9,13 @@
 //
 // Scales of rows are stored by block, [blocks, rows]: the products (gemm_fp8.cu) read one block's scales of many rows at a time.
 #include "api.h"
-#include "common.cuh"
-#include <cuda_fp8.h>
+#include "fp8.cuh"
 
 namespace pe {
 namespace quant8 {
+using namespace fp8;
 
-constexpr int BLOCK = 128;      // features of a block
-
-// The scale's bits for the largest magnitude `a` of a block: 448 = 1.75 * 2^8.
-__device__ __forceinline__ uint32_t scale_bits(float a) {
-  const uint32_t b = __float_as_uint(a);
-  const int e = (int)(b >> 23) - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
-  return (uint32_t)max(e, 1) << 23;
-}
-// 1 / s, a power of two itself
-__device__ __forceinline__ float inverse_of(uint32_t scale) { return __uint_as_float((254u << 23) - scale); }
-
-__device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
-  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
-  return lo | (hi << 16);
-}
-__device__ __forceinline__ float no_infinity(float x) { return fabsf(x) == INFINITY ? __uint_as_float(0x7fffffffu) : x; }
+constexpr int BLOCK = BK;       // features of a block
 
 // Eight neighbouring features of a row from column `c`, zeros behind the row's end.
 template <typename T>

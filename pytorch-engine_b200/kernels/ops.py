@@ -1567,38 +1567,69 @@ def rmsnorm_residual_fp8(residual: torch.Tensor, delta: Optional[torch.Tensor], 
     _count(1)
 
 
-def _gemm_fp8(what: str, x, x_scales, w, w_scales, out, status, glu, offsets, row_weight) -> None:
-    m, k = x.shape
-    n = out.shape[1]
-    groups = 0
+# Up to so many rows, and so many bytes of weights, a product quantises bfloat16 rows itself (csrc/gemm_fp8.cu, RAW): each of its
+# blocks converts all rows of its share of K, which hides behind few weights.  Inside : in front, us on the device: 1 row, 4,096 x
+# 6,144 weights 9.5 : 10.2; 8 rows, 4,096 x 4,096 8.5 : 9.2, 4,096 x 6,144 10.6 : 10.3 (and 5 us less for the host), 12,288 x 4,096
+# 15.2 : 13.9, 4,096 x 24,576 28.6 : 21.3; 16 rows, 4,096 x 6,144 11.9 : 10.5.
+FP8_INSIDE_ROWS, FP8_INSIDE_BYTES = 8, 32 << 20
+
+
+def _fp8_product_error(what: str, m: int, k: int, w, w_scales, out, glu, offsets, row_weight, tensors) -> None:
+    """Says what ``_fp8_product`` refused."""
+    n = out.shape[1] if out.dim() == 2 else -1
+    rows = n if glu is None else 2 * n
+    _need(out.dim() == 2 and out.shape[0] == m and (out.stride(1) == 1 or n == 1), f"{what}: out is a matrix with a row for each of x, of neighbouring features")
+    _need(out.dtype == torch.bfloat16 or (out.dtype == torch.float32 and glu is None), f"{what}: out bfloat16 (or float32 without an activation)")
     if offsets is not None:
-        groups = w.shape[0]
-        _need(w.dim() == 3 and groups >= 1 and offsets.dtype == torch.int32 and offsets.is_contiguous() and offsets.numel() == groups + 1,
-              f"{what}: offsets int32, one more than the groups of w")
-        _need(w.stride(0) == w.shape[1] * w.stride(1) or groups == 1, f"{what}: the groups' matrices must follow each other")
-        _need(w_scales.shape[0] == groups, f"{what}: scales for each group")
-        rows = w.shape[1]
+        _need(w.dim() == 3 and offsets.dtype == torch.int32 and offsets.is_contiguous() and offsets.numel() == w.shape[0] + 1 and w.shape[0] >= 1,
+              f"{what}: w [groups, N, K], offsets int32, one more than the groups")
+        _need(w.shape[0] == 1 or w.stride(0) == w.shape[1] * w.stride(1), f"{what}: the groups' matrices must follow each other")
     else:
         _need(w.dim() == 2, f"{what}: w is a matrix")
-        rows = w.shape[0]
-    _need(w.shape[-1] == k and rows == (n if glu is None else 2 * n) and out.dim() == 2 and out.shape[0] == m and (out.stride(1) == 1 or n == 1),
-          f"{what}: shapes do not match")
-    _need(out.dtype == torch.bfloat16 or (out.dtype == torch.float32 and glu is None), f"{what}: out bfloat16 (or float32 without an activation)")
-    x_ld = _fp8_ld(x, what)
-    w2 = w if offsets is None else w.view(groups * rows, k) if w.is_contiguous() else w.as_strided((groups * rows, k), (w.stride(1), w.stride(2)))
-    w_ld = _fp8_ld(w2, what)
-    _need(w_scales.dtype == torch.float32 and w_scales.is_contiguous() and tuple(w_scales.shape[-2:]) == (fp8_blocks(rows), fp8_blocks(k)),
-          f"{what}: scales of w [blocks of {FP8_BLOCK} rows, blocks of {FP8_BLOCK} features] float32")
-    xs_ld = _fp8_scales_ld(x_scales, fp8_blocks(k), m, what)
+    _need(w.dtype == FP8 and tuple(w.shape[-2:]) == (rows, k), f"{what}: w float8_e4m3fn [{rows}, {k}], got {list(w.shape)}")
+    _need((w.stride(-1) == 1 or k == 1) and w.stride(-2) % 16 == 0, f"{what}: rows of w must be neighbouring values, a multiple of 16 bytes apart")
+    _need(w_scales.dtype == torch.float32 and w_scales.is_contiguous() and tuple(w_scales.shape) == (*w.shape[:-2], fp8_blocks(rows), fp8_blocks(k)),
+          f"{what}: scales of w [blocks of {FP8_BLOCK} rows, blocks of {FP8_BLOCK} features] float32 (for each group)")
     _need(row_weight is None or (glu is not None and row_weight.dtype == torch.float32 and row_weight.is_contiguous() and row_weight.numel() >= m),
           f"{what}: row_weight float32, one per row, before an activation")
-    _on_current(what, x, x_scales, w, w_scales, out, offsets, row_weight, status)
+    _on_current(what, *tensors)
+    raise KernelError(f"{what}: bad arguments")
+
+
+def _fp8_product(what: str, m: int, k: int, w, w_scales, out, glu, offsets, row_weight, *tensors) -> tuple:
+    """Checks a product's weight, output and options; (columns of out, bytes between w's rows, groups, activation arguments).  One
+    expression for all of it: a decode step's product takes the device little longer than this takes the host."""
+    here, n = _current_device(), out.shape[-1]
+    rows, shape, w_stride, groups = n if glu is None else 2 * n, w.shape, w.stride(), 0
+    ok = (len(shape) == (2 if offsets is None else 3) and shape[-1] == k and shape[-2] == rows and w.dtype is FP8 and out.dim() == 2
+          and out.shape[0] == m and (out.stride(1) == 1 or n == 1) and (out.dtype is torch.bfloat16 or (out.dtype is torch.float32 and glu is None))
+          and (w_stride[-1] == 1 or k == 1) and w_scales.dtype is torch.float32 and w_scales.is_contiguous()
+          and tuple(w_scales.shape) == (*shape[:-2], (rows + 127) >> 7, (k + 127) >> 7) and w.get_device() == here and out.get_device() == here
+          and w_scales.get_device() == here)
+    for t in tensors:
+        ok = ok and (t is None or t.get_device() == here)
+    if ok and offsets is not None:
+        groups = shape[0]
+        ok = (groups >= 1 and offsets.dtype is torch.int32 and offsets.is_contiguous() and offsets.numel() == groups + 1 and offsets.get_device() == here
+              and (groups == 1 or w_stride[0] == rows * w_stride[1]))
+    if ok and row_weight is not None:
+        ok = glu is not None and row_weight.dtype is torch.float32 and row_weight.is_contiguous() and row_weight.numel() >= m and row_weight.get_device() == here
+    w_ld = w_stride[-2] if rows > 1 or groups > 1 else (k + 15) // 16 * 16
+    if not ok or w_ld % 16:
+        _fp8_product_error(what, m, k, w, w_scales, out, glu, offsets, row_weight, (*tensors, w, w_scales, out, offsets, row_weight))
+    return n, w_ld, groups, (0, 0.0, 1.0, None) if glu is None else _glu_args(glu or None, n)
+
+
+def _gemm_fp8(what: str, x, x_scales, w, w_scales, out, status, glu, offsets, row_weight) -> None:
+    m, k = x.shape
+    n, w_ld, groups, act = _fp8_product(what, m, k, w, w_scales, out, glu, offsets, row_weight, x, x_scales, status)
+    x_ld, xs_ld = _fp8_ld(x, what), _fp8_scales_ld(x_scales, fp8_blocks(k), m, what)
     if m == 0 or n == 0:
         return
-    kind, limit, alpha, bias = (0, 0.0, 1.0, None) if glu is None else _glu_args(glu or None, n)
-    check(library().pe_gemm_fp8(_ptr(x), x_ld, _ptr(x_scales), xs_ld, _ptr(w), w_ld, _ptr(w_scales), _ptr(out),
-                                out.stride(0) if m > 1 else n, m, n, k, 1 if out.dtype == torch.float32 else 0, kind, limit, alpha, bias,
-                                _ptr(row_weight), _ptr(offsets), groups, _ptr(status), _stream()), what)
+    check(library().pe_gemm_fp8(x.data_ptr(), x_ld, x_scales.data_ptr(), xs_ld, w.data_ptr(), w_ld, w_scales.data_ptr(), out.data_ptr(),
+                                out.stride(0) if m > 1 else n, m, n, k, 1 if out.dtype == torch.float32 else 0, *act,
+                                None if row_weight is None else row_weight.data_ptr(), None if offsets is None else offsets.data_ptr(), groups,
+                                status.data_ptr(), _stream()), what)
     _count(1)
 
 
@@ -1622,3 +1653,35 @@ def moe_rows_gemm_fp8(x: torch.Tensor, x_scales: torch.Tensor, offsets: torch.Te
     [groups, N, K]``, ``w_scales [groups, blocks, blocks]``.  Rows from ``offsets[groups]`` on are left as they are.  ``row_weight``
     (float32, one per row) multiplies both sums of an output before its activation."""
     _gemm_fp8("moe_rows_gemm_fp8", x, x_scales, w, w_scales, out, status, glu, offsets, row_weight)
+
+
+def linear_fp8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor, status: torch.Tensor, glu=None,
+               offsets: Optional[torch.Tensor] = None, row_weight: Optional[torch.Tensor] = None,
+               row_map: Optional[torch.Tensor] = None) -> None:
+    """``quantize_rows_fp8`` of ``x`` (bfloat16 or float32, ``row_map`` as there), then ``gemm_fp8``, or with ``offsets``
+    ``moe_rows_gemm_fp8``.  A handful of bfloat16 rows are quantised inside the product
+    (``FP8_INSIDE_ROWS``)."""
+    src_rows, k = x.shape
+    x_ld, x_step = x.stride()
+    if src_rows <= 1:
+        x_ld = (k + 7) // 8 * 8
+    m = src_rows
+    if row_map is not None:
+        _need(row_map.dtype == torch.int32 and row_map.is_contiguous() and (src_rows > 0 or row_map.numel() == 0), "linear_fp8: row_map int32, of rows that are there")
+        m = row_map.numel()
+    if x_step != 1 and k != 1:
+        raise KernelError("linear_fp8: x must have rows of neighbouring features")
+    n, w_ld, groups, act = _fp8_product("linear_fp8", m, k, w, w_scales, out, glu, offsets, row_weight, x, status, row_map)
+    if m == 0 or n == 0:
+        return
+    px, scratch = x.data_ptr(), None
+    raw = (m <= FP8_INSIDE_ROWS * (groups or 1) and w.numel() <= FP8_INSIDE_BYTES and row_map is None and x.dtype is torch.bfloat16
+           and x_ld % 8 == 0 and px % 16 == 0)
+    if not raw:
+        scratch = torch.empty(m * ((k + 15) // 16 * 16 + 4 * fp8_blocks(k)), dtype=torch.uint8, device=x.device)
+    check(library().pe_linear_fp8(dtype_tag(x.dtype), px, x_ld, None if row_map is None else row_map.data_ptr(), src_rows,
+                                  None if raw else scratch.data_ptr(), w.data_ptr(), w_ld, w_scales.data_ptr(), out.data_ptr(),
+                                  out.stride(0) if m > 1 else n, m, n, k, 1 if out.dtype is torch.float32 else 0, *act,
+                                  None if row_weight is None else row_weight.data_ptr(), None if offsets is None else offsets.data_ptr(), groups,
+                                  status.data_ptr(), _stream()), "linear_fp8")
+    _count(1 if raw else 2)

@@ -17,6 +17,8 @@ from ..kernels.ops import FP8, FP8_BLOCK, fp8_blocks
 def _padded_empty(shape, device) -> torch.Tensor:
     """Uninitialised e4m3 ``[..., K]`` whose rows start on 16-byte boundaries."""
     *lead, k = shape
+    if k % 16 == 0:
+        return torch.empty((*lead, k), dtype=FP8, device=device)
     return torch.empty((*lead, (k + 15) // 16 * 16), dtype=FP8, device=device)[..., :k]
 
 
@@ -61,10 +63,11 @@ class Float8Weight:
     dtype = FP8
 
     def __init__(self, values: torch.Tensor, scales: torch.Tensor) -> None:
-        if values.dtype != FP8 or scales.dtype != torch.float32:
+        shape = values.shape
+        if values.dtype is not FP8 or scales.dtype is not torch.float32:
             raise ValueError(f"an 8-bit weight is float8_e4m3fn with float32 scales, got {values.dtype} and {scales.dtype}")
-        want = (*values.shape[:-2], fp8_blocks(values.shape[-2]), fp8_blocks(values.shape[-1]))
-        if tuple(scales.shape) != want:
+        want = (*shape[:-2], (shape[-2] + 127) >> 7, (shape[-1] + 127) >> 7)
+        if scales.shape != want:
             raise ValueError(f"an 8-bit weight {list(values.shape)} has scales {list(want)}, got {list(scales.shape)}")
         self.values, self.scales = values, scales
 

@@ -241,11 +241,9 @@ class Runtime:
         if not self.is_cuda:
             raise KernelError("this package computes on a CUDA device only; there is no CPU path")
         if type(weight) is Float8Weight:
-            rows = x if type(x) is Float8Rows else Float8Rows.quantize(x)
             if out is None:
-                out = torch.empty((rows.shape[0], weight.shape[0]), dtype=out_dtype or torch.bfloat16, device=rows.device)
-            ops.gemm_fp8(rows.values, rows.scales, weight.values, weight.scales, out, self.status)
-            return out
+                out = torch.empty((x.shape[0], weight.shape[0]), dtype=out_dtype or torch.bfloat16, device=x.device)
+            return self._float8_product(x, weight, out)
         if self.gemm_backend is not None:
             y = self.gemm_backend(x, weight, out, out_dtype)
             if y is not None:
@@ -294,18 +292,24 @@ class Runtime:
             if prev[0]:
                 _set_reduced_reductions(*prev)
 
+    def _float8_product(self, x, weight: Float8Weight, out: torch.Tensor, glu=None, offsets=None, row_weight=None, row_map=None) -> torch.Tensor:
+        if type(x) is not Float8Rows:
+            ops.linear_fp8(x, weight.values, weight.scales, out, self.status, glu, offsets, row_weight, row_map)
+        elif offsets is None:
+            ops.gemm_fp8(x.values, x.scales, weight.values, weight.scales, out, self.status, glu)
+        else:
+            ops.moe_rows_gemm_fp8(x.values, x.scales, offsets, weight.values, weight.scales, out, self.status, glu, row_weight)
+        return out
+
     def float8_feed_forward(self, x, gate_up: Float8Weight, down: Float8Weight, out: torch.Tensor, glu=None) -> torch.Tensor:
         """``out = down(act(gate, up))`` with 8-bit weights, ``gate_up`` gate rows and as many up rows; ``x`` rows in bfloat16 or
         ``Float8Rows``.  The activation is rounded to bfloat16 and quantised in blocks of 128.  ``glu``: as in ``ops.gemm_fp8``
         (None: SiLU)."""
         if not self.is_cuda:
             raise KernelError("this package computes on a CUDA device only; there is no CPU path")
-        rows = x if type(x) is Float8Rows else Float8Rows.quantize(x)
-        act = torch.empty((rows.shape[0], down.shape[1]), dtype=torch.bfloat16, device=rows.device)
-        ops.gemm_fp8(rows.values, rows.scales, gate_up.values, gate_up.scales, act, self.status, glu=glu or ())
-        rows = Float8Rows.quantize(act)
-        ops.gemm_fp8(rows.values, rows.scales, down.values, down.scales, out, self.status)
-        return out
+        act = torch.empty((x.shape[0], down.shape[1]), dtype=torch.bfloat16, device=x.device)
+        self._float8_product(x, gate_up, act, glu or ())
+        return self._float8_product(act, down, out)
 
     def float8_experts(self, x, offsets: torch.Tensor, gate_up: Float8Weight, down: Float8Weight, out: torch.Tensor, glu=None,
                        row_weight: Optional[torch.Tensor] = None, row_token: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -314,11 +318,6 @@ class Runtime:
         ``row_weight``: as in ``ops.moe_rows_gemm_fp8``.  Rows that no expert has are left as they are."""
         if not self.is_cuda:
             raise KernelError("this package computes on a CUDA device only; there is no CPU path")
-        live = offsets[-1:]
-        rows = Float8Rows.quantize(x, row_token, live, self.status)
-        act = torch.empty((rows.shape[0], down.shape[2]), dtype=torch.bfloat16, device=rows.device)
-        ops.moe_rows_gemm_fp8(rows.values, rows.scales, offsets, gate_up.values, gate_up.scales, act, self.status, glu=glu or (),
-                              row_weight=row_weight)
-        rows = Float8Rows.quantize(act, None, live)
-        ops.moe_rows_gemm_fp8(rows.values, rows.scales, offsets, down.values, down.scales, out, self.status)
-        return out
+        act = torch.empty((out.shape[0], down.shape[2]), dtype=torch.bfloat16, device=x.device)
+        self._float8_product(x, gate_up, act, glu or (), offsets, row_weight, row_token)
+        return self._float8_product(act, down, out, None, offsets)

@@ -401,3 +401,63 @@ def test_own_stream_and_graph(ops, f8, status):
     replayed = out.clone()
     chain()
     assert torch.equal(out, replayed) and not torch.equal(out, first)
+
+
+# ---- quantised on the way ----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("m,n,k", [(1, 64, 128), (1, 6144, 4096), (5, 200, 1043), (8, 4096, 12288), (16, 333, 2000), (17, 64, 300), (70, 256, 512),
+                                   (700, 2816, 2048)])
+@pytest.mark.parametrize("gate", [False, True])
+def test_linear(ops, f8, status, m, n, k, dtype, gate):
+    """The same bits as conversion and product one after the other, whichever kernels take it."""
+    if gate:
+        n = n // 2 * 2
+    x, w = rows_of(m, k, dtype, m) * 0.01, weight_of(f8, n, k, n)
+    x = x.to(dtype)
+    cols, glu = (n // 2, ()) if gate else (n, None)
+    one, two = (torch.empty(m, cols, dtype=BF16, device=DEV) for _ in range(2))
+    ops.linear_fp8(x, w.values, w.scales, one, status, glu)
+    r = f8.Float8Rows.quantize(x)
+    ops.gemm_fp8(r.values, r.scales, w.values, w.scales, two, status, glu)
+    assert torch.equal(one, two)
+
+
+def test_linear_of_rows_off_the_boundary(ops, f8, status):
+    base, w = rows_of(9, 600, BF16, 1), weight_of(f8, 130, 500, 1)
+    for x in (base[:, 3:503], base[:, 8:508], base.t()[:500].t()):
+        assert x.stride(1) == 1
+        one, two = (torch.empty(9, 130, dtype=BF16, device=DEV) for _ in range(2))
+        ops.linear_fp8(x, w.values, w.scales, one, status)
+        ops.linear_fp8(x.contiguous(), w.values, w.scales, two, status)
+        assert torch.equal(one, two)
+
+
+@pytest.mark.parametrize("counts", [[0, 1, 0, 3], [16, 17, 0, 33, 1], [1] * 40, [300, 0, 5]])
+@pytest.mark.parametrize("mapped", [False, True])
+def test_experts_linear(ops, f8, status, counts, mapped):
+    """Grouped rows, taken from others by a map or not: as the grouped product of quantised rows."""
+    k, n, m, groups = 400, 144, sum(counts), len(counts)
+    offsets = torch.tensor([sum(counts[:i]) for i in range(groups + 1)], dtype=torch.int32, device=DEV)
+    w = weight_of(f8, n, k, 2, groups)
+    src = rows_of(50, k, BF16, 3)
+    pick = torch.randint(0, 50, (m + 2,), device=DEV, dtype=torch.int32)
+    pick[m:] = 12345                                    # rows that no expert has: nobody looks at their index
+    x = src if mapped else src[pick[:m].long()]
+    out = torch.full((m + 2 if mapped else m, n), 5.0, dtype=BF16, device=DEV)
+    ops.linear_fp8(x, w.values, w.scales, out, status, offsets=offsets, row_map=pick if mapped else None)
+    r = f8.Float8Rows.quantize(src[pick[:m].long()])
+    want = torch.empty(m, n, dtype=BF16, device=DEV)
+    ops.moe_rows_gemm_fp8(r.values, r.scales, offsets, w.values, w.scales, want, status)
+    assert torch.equal(out[:m], want) and bool((out[m:] == 5.0).all())
+
+
+def test_linear_nan_and_infinity(ops, f8, status):
+    for m in (3, 40):
+        x, w = rows_of(m, 300, BF16, 4), weight_of(f8, 130, 300)
+        clean, dirty = (torch.empty(m, 130, dtype=BF16, device=DEV) for _ in range(2))
+        ops.linear_fp8(x, w.values, w.scales, clean, status)
+        x[1, 7], x[2, 299] = float("nan"), float("inf")
+        ops.linear_fp8(x, w.values, w.scales, dirty, status)
+        assert bool(torch.isnan(dirty[1:3]).all())
+        keep = (torch.arange(m, device=DEV) < 1) | (torch.arange(m, device=DEV) > 2)
+        assert torch.equal(clean[keep], dirty[keep])

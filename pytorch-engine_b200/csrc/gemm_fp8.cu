@@ -511,6 +511,17 @@ static int launch_np(Params p, const void* x, long long x_ld, long long x_rows, 
 }  // namespace fp8
 }  // namespace pe
 
+// Whether a product (not of groups) runs in tiles of 128 x 256 (gemm_fp8_many.cu): where they take no longer.  A block of K takes an SM
+// 0.60 us there and 0.55 us in this file's tiles of 128 x 128, which can share K out (4,096 x 6,144, both files' times in us: 128 rows
+// 24.4 and 15.6, 384 rows 24.8 and 21.7, 512 rows 26.2 and 42.9; 12,288 x 4,096: 512 rows 60.1 and 56.0, 700 rows 62.9 and 107.9).
+extern "C" int pe_gemm_fp8_many_takes(int M, int N, int K, int kind) {
+  if (M <= 64 || N < 1 || K < 1 || (kind > 0 && N % 128)) return 0;
+  const int k_blocks = (K + pe::fp8::BK - 1) / pe::fp8::BK;
+  const long long tiles = ((M + 127LL) / 128) * (kind > 0 ? N / 128 : (N + 255) / 256);
+  const pe::fp8::Cut c = pe::fp8::cut_of(M, N, k_blocks, 0, 128, kind > 0);
+  return 11 * ((tiles + pe::kSMs - 1) / pe::kSMs) * k_blocks <= 10LL * c.waves_blocks ? 1 : 0;
+}
+
 // Whether bfloat16 rows are quantised inside the product: up to 16 rows (of an average group).
 static bool takes_raw(int M, int n_groups) { return (n_groups > 0 ? (M + n_groups - 1) / n_groups : M) <= 16; }
 
@@ -529,16 +540,9 @@ static int product(bool raw, const void* x, long long x_ld, const float* x_scale
   if (N > (1 << 28) || (long long)(n_groups > 0 ? n_groups : 1) * N > (1 << 29)) return PE_ERR_UNSUPPORTED_SIZE;
   const int rows = n_groups > 0 ? (M + n_groups - 1) / n_groups : M;     // of an average group
   const int k_blocks = (K + BK - 1) / BK;
-  // Many rows: tiles of 128 x 256 (gemm_fp8_many.cu) where they take no longer.  A block of K takes an SM 0.60 us there and 0.55 us in
-  // this file's tiles of 128 x 128, which can share K out (4,096 x 6,144, both files' times in us: 128 rows 24.4 and 15.6, 384 rows 24.8
-  // and 21.7, 512 rows 26.2 and 42.9; 12,288 x 4,096: 512 rows 60.1 and 56.0, 700 rows 62.9 and 107.9).
-  if (n_groups == 0 && !row_weight && M > 64 && (kind == 0 || N % 128 == 0)) {
-    const long long tiles = ((M + 127) / 128) * (long long)(kind > 0 ? N / 128 : (N + 255) / 256);
-    const Cut c = cut_of(M, N, k_blocks, 0, 128, kind > 0);
-    if (11 * ((tiles + pe::kSMs - 1) / pe::kSMs) * k_blocks <= 10LL * c.waves_blocks)
-      return pe_gemm_fp8_many(x, x_ld, x_scales, xs_ld, w, w_ld, w_scales, y, ldy, nullptr, 0, M, N, K, out_f32, kind, limit, alpha, bias,
-                              status, stream);
-  }
+  if (n_groups == 0 && !row_weight && !raw && pe_gemm_fp8_many_takes(M, N, K, kind))
+    return pe_gemm_fp8_many(x, x_ld, x_scales, xs_ld, w, w_ld, w_scales, y, ldy, nullptr, 0, M, N, K, out_f32, kind, limit, alpha, bias, status,
+                            stream);
   Params p;
   p.M = M; p.N = N; p.K = K; p.k_blocks = k_blocks; p.whole = K % BK == 0;
   p.xs = x_scales; p.xs_ld = xs_ld; p.ws = w_scales;

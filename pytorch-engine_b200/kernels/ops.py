@@ -1516,17 +1516,40 @@ def quantize_rows_fp8(x: torch.Tensor, values: torch.Tensor, scales: torch.Tenso
     _need(x.dim() == 2 and values.dim() == 2 and (x.stride(1) == 1 or x.shape[1] == 1), "quantize_rows_fp8: matrices of neighbouring features")
     m, k = values.shape
     _need(x.shape[1] == k and (row_map is not None or x.shape[0] == m), "quantize_rows_fp8: shapes do not match")
-    _need(row_map is None or (row_map.dtype == torch.int32 and row_map.is_contiguous() and row_map.numel() == m and status is not None),
-          "quantize_rows_fp8: row_map int32, one per row, with a status word")
-    _need(live is None or (live.dtype == torch.int32 and live.numel() >= 1), "quantize_rows_fp8: live is one int32")
     v_ld, s_ld = _fp8_ld(values, "quantize_rows_fp8"), _fp8_scales_ld(scales, fp8_blocks(k), m, "quantize_rows_fp8")
-    _on_current("quantize_rows_fp8", x, values, scales, row_map, live)
+    _on_current("quantize_rows_fp8", values, scales)
+    _quantize_rows(x, m, k, values.data_ptr(), v_ld, scales.data_ptr(), s_ld, row_map, live, status)
+
+
+def _quantize_rows(x, m, k, values: int, v_ld: int, scales: int, s_ld: int, row_map, live, status) -> None:
+    """The launch, into memory that is known to fit; checks what is read."""
+    rows = x.shape[0]
+    _on_current("quantize_rows_fp8", x, row_map, live)
+    if row_map is not None:
+        _need(row_map.dtype == torch.int32 and row_map.is_contiguous() and row_map.numel() == m and status is not None,
+              "quantize_rows_fp8: row_map int32, one per row, with a status word")
+    _need(live is None or (live.dtype == torch.int32 and live.numel() >= 1), "quantize_rows_fp8: live is one int32")
     if m == 0 or k == 0:
         return
-    check(library().pe_quantize_rows_fp8(dtype_tag(x.dtype), _ptr(x), x.stride(0) if x.shape[0] > 1 else k, _ptr(row_map), _ptr(live),
-                                         _ptr(values), v_ld, _ptr(scales), s_ld, m, k, x.shape[0], _ptr(status), _stream()),
-          "quantize_rows_fp8")
+    check(library().pe_quantize_rows_fp8(dtype_tag(x.dtype), x.data_ptr(), x.stride(0) if rows > 1 else k, None if row_map is None else row_map.data_ptr(),
+                                         None if live is None else live.data_ptr(), values, v_ld, scales, s_ld, m, k, rows,
+                                         None if status is None else status.data_ptr(), _stream()), "quantize_rows_fp8")
     _count(1)
+
+
+def new_rows_fp8(x: torch.Tensor, row_map: Optional[torch.Tensor] = None, live: Optional[torch.Tensor] = None,
+                 status: Optional[torch.Tensor] = None) -> tuple:
+    """``quantize_rows_fp8`` into new tensors: (values, scales)."""
+    if x.dim() != 2 or (x.stride(1) != 1 and x.shape[1] != 1):
+        raise KernelError("quantize_rows_fp8: a matrix of neighbouring features")
+    m, k = x.shape
+    if row_map is not None:
+        m = row_map.numel()
+    ld = (k + 15) // 16 * 16
+    values = torch.empty((m, ld), dtype=FP8, device=x.device)
+    scales = torch.empty(((k + 127) >> 7, m), dtype=torch.float32, device=x.device)
+    _quantize_rows(x, m, k, values.data_ptr(), ld, scales.data_ptr(), m, row_map, live, status)
+    return (values if ld == k else values[:, :k]), scales
 
 
 def quantize_weight_fp8(w: torch.Tensor, values: torch.Tensor, scales: torch.Tensor) -> None:
@@ -1685,3 +1708,30 @@ def linear_fp8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: to
                                   None if row_weight is None else row_weight.data_ptr(), None if offsets is None else offsets.data_ptr(), groups,
                                   status.data_ptr(), _stream()), "linear_fp8")
     _count(1 if raw else 2)
+
+
+def gemm_fp8_gated_supported(rows: int, width: int, k: int) -> bool:
+    """Whether ``gemm_fp8_gated`` takes a product of so many rows and ``width`` gates (many rows, a multiple of 128 gates)."""
+    return bool(library().pe_gemm_fp8_many_takes(rows, width, k, 1))
+
+
+def gemm_fp8_gated(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, values: torch.Tensor,
+                   scales: torch.Tensor, status: torch.Tensor, glu=()) -> None:
+    """``gemm_fp8`` with an activation whose outputs, rounded to bfloat16, are quantised on the way out (csrc/gemm_fp8_many.cu): e4m3
+    ``values [M, N]`` and ``scales [fp8_blocks(N), M]``, the bits that ``quantize_rows_fp8`` of ``gemm_fp8``'s output gives."""
+    what = "gemm_fp8_gated"
+    m, k = x.shape
+    n = values.shape[1]
+    _need(values.dim() == 2 and values.shape[0] == m and w.dim() == 2 and tuple(w.shape) == (2 * n, k) and w.dtype == FP8, f"{what}: shapes do not match")
+    _need(gemm_fp8_gated_supported(m, n, k) or m == 0, f"{what}: not for {m} rows and {n} gates")
+    _need(w.stride(1) == 1 and w.stride(0) % 16 == 0, f"{what}: rows of w must be neighbouring values, a multiple of 16 bytes apart")
+    _need(w_scales.dtype == torch.float32 and w_scales.is_contiguous() and tuple(w_scales.shape) == (fp8_blocks(2 * n), fp8_blocks(k)), f"{what}: scales of w")
+    x_ld, xs_ld = _fp8_ld(x, what), _fp8_scales_ld(x_scales, fp8_blocks(k), m, what)
+    y_ld, ys_ld = _fp8_ld(values, what), _fp8_scales_ld(scales, fp8_blocks(n), m, what)
+    _on_current(what, x, x_scales, w, w_scales, values, scales, status)
+    if m == 0:
+        return
+    kind, limit, alpha, bias = _glu_args(glu or None, n)
+    check(library().pe_gemm_fp8_many(x.data_ptr(), x_ld, x_scales.data_ptr(), xs_ld, w.data_ptr(), w.stride(0), w_scales.data_ptr(), values.data_ptr(), y_ld,
+                                     scales.data_ptr(), ys_ld, m, n, k, 0, kind, limit, alpha, bias, status.data_ptr(), _stream()), what)
+    _count(1)

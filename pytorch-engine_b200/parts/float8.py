@@ -46,9 +46,7 @@ class Float8Rows:
     def quantize(cls, x: torch.Tensor, row_map: Optional[torch.Tensor] = None, live: Optional[torch.Tensor] = None,
                  status: Optional[torch.Tensor] = None) -> "Float8Rows":
         """``x [rows, K]`` in new storage (``row_map``, ``live``: see ``ops.quantize_rows_fp8``)."""
-        out = cls.empty(x.shape[0] if row_map is None else row_map.numel(), x.shape[1], x.device)
-        ops.quantize_rows_fp8(x, out.values, out.scales, row_map, live, status)
-        return out
+        return cls(*ops.new_rows_fp8(x, row_map, live, status))
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         s = self.scales.repeat_interleave(FP8_BLOCK, 0)[:self.values.shape[1]].t()

@@ -307,8 +307,15 @@ class Runtime:
         (None: SiLU)."""
         if not self.is_cuda:
             raise KernelError("this package computes on a CUDA device only; there is no CPU path")
-        act = torch.empty((x.shape[0], down.shape[1]), dtype=torch.bfloat16, device=x.device)
-        self._float8_product(x, gate_up, act, glu or ())
+        m, (hidden, inter) = x.shape[0], down.shape
+        if m > 64 and ops.gemm_fp8_gated_supported(m, inter, hidden):
+            # many rows: the activation leaves the product's epilogue quantised
+            rows = x if type(x) is Float8Rows else Float8Rows.quantize(x)
+            act = Float8Rows.empty(m, inter, x.device)
+            ops.gemm_fp8_gated(rows.values, rows.scales, gate_up.values, gate_up.scales, act.values, act.scales, self.status, glu or ())
+        else:
+            act = torch.empty((m, inter), dtype=torch.bfloat16, device=x.device)
+            self._float8_product(x, gate_up, act, glu or ())
         return self._float8_product(act, down, out)
 
     def float8_experts(self, x, offsets: torch.Tensor, gate_up: Float8Weight, down: Float8Weight, out: torch.Tensor, glu=None,

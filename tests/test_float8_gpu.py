@@ -461,3 +461,42 @@ def test_linear_nan_and_infinity(ops, f8, status):
         assert bool(torch.isnan(dirty[1:3]).all())
         keep = (torch.arange(m, device=DEV) < 1) | (torch.arange(m, device=DEV) > 2)
         assert torch.equal(clean[keep], dirty[keep])
+
+
+@pytest.mark.parametrize("m,inter,k", [(513, 12288, 256), (700, 1408, 2048), (2100, 640, 1043)])
+@pytest.mark.parametrize("kind", ["silu", "clamped_swish"])
+def test_gate_quantized(ops, f8, status, m, inter, k, kind):
+    """The same bits as the gated product and the conversion of what it gives; sizes that other tiles take are refused."""
+    rows, w = f8.Float8Rows.quantize(rows_of(m, k, BF16, m) * 0.01), weight_of(f8, 2 * inter, k, inter)
+    glu = () if kind == "silu" else (kind, 7.0, 1.7, torch.randn(2 * inter, device=DEV))
+    out = torch.empty(m, inter, dtype=BF16, device=DEV)
+    ops.gemm_fp8(rows.values, rows.scales, w.values, w.scales, out, status, glu=glu)
+    want = f8.Float8Rows.quantize(out)
+    got = f8.Float8Rows.empty(m, inter, DEV)
+    if not ops.gemm_fp8_gated_supported(m, inter, k):
+        with pytest.raises(RuntimeError, match="gemm_fp8_gated"):
+            ops.gemm_fp8_gated(rows.values, rows.scales, w.values, w.scales, got.values, got.scales, status, glu)
+        return
+    ops.gemm_fp8_gated(rows.values, rows.scales, w.values, w.scales, got.values, got.scales, status, glu)
+    assert torch.equal(got.scales, want.scales) and torch.equal(got.values.to(F32), want.values.to(F32))
+
+
+@pytest.mark.parametrize("m", [1, 9, 64, 65, 600, 1030])
+@pytest.mark.parametrize("hidden,inter", [(512, 1408), (256, 200)])
+def test_feed_forward(pe, ops, f8, m, hidden, inter):
+    """The run of them against the products one by one."""
+    from pytorch_engine_b200.parts.runtime import Runtime
+
+    rt = Runtime(DEV, BF16)
+    x, gate_up, down = rows_of(m, hidden, BF16, m) * 0.01, weight_of(f8, 2 * inter, hidden, 1), weight_of(f8, hidden, inter, 2)
+    out, act, want = (torch.empty(m, n, dtype=BF16, device=DEV) for n in (hidden, inter, hidden))
+    rt.float8_feed_forward(x, gate_up, down, out)
+    rows = f8.Float8Rows.quantize(x)
+    ops.gemm_fp8(rows.values, rows.scales, gate_up.values, gate_up.scales, act, rt.status, glu=())
+    r = f8.Float8Rows.quantize(act)
+    ops.gemm_fp8(r.values, r.scales, down.values, down.scales, want, rt.status)
+    assert torch.equal(out, want)
+    again = torch.empty_like(out)
+    rt.float8_feed_forward(rows, gate_up, down, again)
+    assert torch.equal(out, again)
+    rt.raise_on_status()

@@ -346,12 +346,13 @@ int pe_linear_fp8(int dtype, const void* x, long long x_ld, const int* row_map, 
     long long w_ld, const float* w_scales, void* y, long long ldy, int M, int N, int K, int out_f32, int kind, float limit,
     float alpha, const float* bias, const float* row_weight, const int* offsets, int n_groups, int* status, cudaStream_t stream);
 
-int pe_gemm_fp8_many_takes(int M, int N, int K, int kind);
+int pe_gemm_fp8_many_takes(int M, int N, int K, int kind, int n_groups);
 
 // gemm_fp8_many.cu
 int pe_gemm_fp8_many(const void* x, long long x_ld, const float* x_scales, long long xs_ld, const void* w, long long w_ld,
     const float* w_scales, void* y, long long ldy, float* y_scales, long long ys_ld, int M, int N, int K, int out_f32, int kind,
-    float limit, float alpha, const float* bias, int* status, cudaStream_t stream);
+    float limit, float alpha, const float* bias, const float* row_weight, const int* offsets, int n_groups, int* status,
+    cudaStream_t stream);
 
 // wait_probe.cu
 int pe_wait_probe(unsigned long long* out, int polls, cudaStream_t stream);

@@ -58,6 +58,29 @@ __device__ __forceinline__ void load_blocks(char* dst, const CUtensorMap* map, i
   }
 }
 
+// The weights of `groups` matrices of N rows (glu: 2 N, gates then ups), `ld` bytes apart, as [group][block][half][row][128] (half: gates
+// and ups): a copy brings `kbs` blocks of `box_rows` rows, of both halves with glu.  Rows beyond a half's N arrive as zeros.
+inline int make_weight_map(CUtensorMap* map, const void* w, uint64_t width, uint64_t N, uint64_t ld, bool glu, uint64_t groups,
+                           uint32_t box_rows, bool whole, uint32_t kbs) {
+  tma::EncodeTiledFn fn = tma::encode_fn();
+  if (fn == nullptr) return -5;
+  if (((uintptr_t)w % 16) || (ld % 16) || box_rows > 256) return -2;
+  const uint32_t halves = glu ? 2 : 1;
+  cuuint64_t dims[5] = {whole ? (uint64_t)BK : width, N, halves, whole ? width / BK : 1, groups};
+  cuuint64_t strides[4] = {ld, N * ld, (uint64_t)(whole ? BK : ld), halves * N * ld};
+  cuuint32_t box[5] = {BK, box_rows, halves, whole ? kbs : 1, 1};
+  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, const_cast<void*>(w), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : -2;
+}
+__device__ __forceinline__ void load_5d(void* dst, const CUtensorMap* map, int x, int row, int block, int group, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];\n"
+      ::"r"(tma::smem_addr(dst)), "l"(map), "r"(x), "r"(row), "r"(0), "r"(block), "r"(group), "r"(tma::smem_addr(bar)) : "memory");
+}
+
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
@@ -192,6 +215,18 @@ __device__ __forceinline__ bool find_group(const int* offsets, int n_groups, int
     before += __shfl_sync(0xffffffffu, sum, 31);
   }
   return false;
+}
+
+// How many tiles of `np` rows the groups have; all lanes of a warp take part.
+__device__ __forceinline__ int count_tiles(const int* offsets, int n_groups, int M, int np) {
+  int tiles = 0;
+  for (int g = threadIdx.x & 31; g < n_groups; g += 32) {
+    const int lo = min(max(offsets[g], 0), M);
+    tiles += (max(min(max(offsets[g + 1], 0), M) - lo, 0) + np - 1) / np;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
+  return tiles;
 }
 
 }  // namespace fp8

@@ -59,11 +59,6 @@ template <int NP> struct Shape {
   static constexpr size_t kSmem = 1024 + (size_t)kStages * kStage;
 };
 
-__device__ __forceinline__ void load_5d(void* dst, const CUtensorMap* map, int x, int row, int block, int group, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];\n"
-      ::"r"(tma::smem_addr(dst)), "l"(map), "r"(x), "r"(row), "r"(0), "r"(block), "r"(group), "r"(tma::smem_addr(bar)) : "memory");
-}
 __device__ __forceinline__ void epilogue_sync(int threads) { asm volatile("bar.sync 1, %0;\n" ::"r"(threads) : "memory"); }
 
 // The bfloat16 rows of a stage on their way into it (RAW): sixteen lanes a row and block, eight features a lane.
@@ -421,21 +416,6 @@ gemm_fp8_kernel(Params p, const __grid_constant__ CUtensorMap wmap, const __grid
   }
 }
 
-// The weights as [group][block][half][row][128] (half: gates and ups; see fp8::make_map): a copy brings KBS blocks of a tile.
-static int make_weight_map(CUtensorMap* map, const void* w, const Params& p, uint64_t ld, bool glu, int groups, uint32_t kbs) {
-  tma::EncodeTiledFn fn = tma::encode_fn();
-  if (fn == nullptr) return -5;
-  const uint64_t halves = glu ? 2 : 1;
-  cuuint64_t dims[5] = {p.whole ? (uint64_t)BK : p.K, (uint64_t)p.N, halves, p.whole ? (uint64_t)p.k_blocks : 1, (uint64_t)groups};
-  cuuint64_t strides[4] = {ld, (uint64_t)p.N * ld, (uint64_t)(p.whole ? BK : ld), halves * p.N * ld};
-  cuuint32_t box[5] = {BK, (cuuint32_t)p.tile_rows, (cuuint32_t)halves, p.whole ? kbs : 1, 1};
-  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, const_cast<void*>(w), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? 0 : -2;
-}
-
 // How a product is cut: weight rows of a tile, token tiles, thread blocks that share K.
 struct Cut {
   int rows, tok_tiles, split;
@@ -471,7 +451,7 @@ static int launch_np(Params p, const void* x, long long x_ld, long long x_rows, 
   const int split = p.split = c.split;
   if (c.blocks > 0x7fffffffLL) return PE_ERR_UNSUPPORTED_SIZE;
   CUtensorMap wmap, xmap;
-  int e = make_weight_map(&wmap, w, p, w_ld, GLU, groups, S::kKbs);
+  int e = make_weight_map(&wmap, w, p.K, p.N, w_ld, GLU, groups, p.tile_rows, p.whole, S::kKbs);
   if (e == 0 && !RAW) e = make_map(&xmap, x, p.K, x_rows, x_ld, NP, p.whole, S::kKbs);
   if (e != 0) return e;
   if (RAW) xmap = wmap;                // not used
@@ -511,14 +491,16 @@ static int launch_np(Params p, const void* x, long long x_ld, long long x_rows, 
 }  // namespace fp8
 }  // namespace pe
 
-// Whether a product (not of groups) runs in tiles of 128 x 256 (gemm_fp8_many.cu): where they take no longer.  A block of K takes an SM
-// 0.60 us there and 0.55 us in this file's tiles of 128 x 128, which can share K out (4,096 x 6,144, both files' times in us: 128 rows
-// 24.4 and 15.6, 384 rows 24.8 and 21.7, 512 rows 26.2 and 42.9; 12,288 x 4,096: 512 rows 60.1 and 56.0, 700 rows 62.9 and 107.9).
-extern "C" int pe_gemm_fp8_many_takes(int M, int N, int K, int kind) {
-  if (M <= 64 || N < 1 || K < 1 || (kind > 0 && N % 128)) return 0;
+// Whether a product runs in tiles of 128 x 256 (gemm_fp8_many.cu): where they take no longer.  A block of K takes an SM 0.60 us there
+// and 0.55 us in this file's tiles of 128 x 128, which can share K out (4,096 x 6,144, both files' times in us: 128 rows 24.4 and 15.6,
+// 384 rows 24.8 and 21.7, 512 rows 26.2 and 42.9; 12,288 x 4,096: 512 rows 60.1 and 56.0, 700 rows 62.9 and 107.9).  Of groups half are
+// taken to fill their last tile and half not to have it.
+extern "C" int pe_gemm_fp8_many_takes(int M, int N, int K, int kind, int n_groups) {
+  if (N < 1 || K < 1 || (kind > 0 && N % 128)) return 0;
+  if ((n_groups > 0 ? (M + n_groups - 1) / n_groups : M) <= 64) return 0;
   const int k_blocks = (K + pe::fp8::BK - 1) / pe::fp8::BK;
-  const long long tiles = ((M + 127LL) / 128) * (kind > 0 ? N / 128 : (N + 255) / 256);
-  const pe::fp8::Cut c = pe::fp8::cut_of(M, N, k_blocks, 0, 128, kind > 0);
+  const long long m_tiles = (M + 127LL) / 128 + n_groups / 2, tiles = m_tiles * (kind > 0 ? N / 128 : (N + 255) / 256);
+  const pe::fp8::Cut c = pe::fp8::cut_of((int)(m_tiles * 128), N, k_blocks, 0, 128, kind > 0);
   return 11 * ((tiles + pe::kSMs - 1) / pe::kSMs) * k_blocks <= 10LL * c.waves_blocks ? 1 : 0;
 }
 
@@ -540,9 +522,9 @@ static int product(bool raw, const void* x, long long x_ld, const float* x_scale
   if (N > (1 << 28) || (long long)(n_groups > 0 ? n_groups : 1) * N > (1 << 29)) return PE_ERR_UNSUPPORTED_SIZE;
   const int rows = n_groups > 0 ? (M + n_groups - 1) / n_groups : M;     // of an average group
   const int k_blocks = (K + BK - 1) / BK;
-  if (n_groups == 0 && !row_weight && !raw && pe_gemm_fp8_many_takes(M, N, K, kind))
-    return pe_gemm_fp8_many(x, x_ld, x_scales, xs_ld, w, w_ld, w_scales, y, ldy, nullptr, 0, M, N, K, out_f32, kind, limit, alpha, bias, status,
-                            stream);
+  if (!raw && (n_groups > 0 || !row_weight) && pe_gemm_fp8_many_takes(M, N, K, kind, n_groups))
+    return pe_gemm_fp8_many(x, x_ld, x_scales, xs_ld, w, w_ld, w_scales, y, ldy, nullptr, 0, M, N, K, out_f32, kind, limit, alpha, bias,
+                            row_weight, offsets, n_groups, status, stream);
   Params p;
   p.M = M; p.N = N; p.K = K; p.k_blocks = k_blocks; p.whole = K % BK == 0;
   p.xs = x_scales; p.xs_ld = xs_ld; p.ws = w_scales;

@@ -34,35 +34,47 @@ constexpr int STAGES = 4;        // of one k block
 constexpr int kBytesA = BM * BK, kBytesB = BN * BK, kStage = kBytesA + kBytesB;
 constexpr int kTmemCols = 512;
 constexpr int kRoles = 3, kThreads = 32 * (kRoles + 8);
-constexpr size_t kSmem = 1024 + (size_t)STAGES * kStage;
+constexpr int kOutRow = 80, kOutWarp = 32 * kOutRow;      // what an epilogue warp has for 64 bytes of each of its rows on their way out
+constexpr size_t kSmem = 1024 + (size_t)STAGES * kStage + 8 * kOutWarp;
 
-__device__ long long g_trace[16][128];
-#define TR(r,i) do { if (blockIdx.x==0 && (i)<128) g_trace[r][i]=clock64(); } while(0)
 enum Mode { kBf16 = 0, kF32 = 1, kGlu = 2, kGluFp8 = 3 };
 
 struct Params {
   int M, N, K, k_blocks;                // N: output columns
   bool whole;
   const float* xs; long long xs_ld;
-  const float* ws;                      // [ceil(w rows / 128)][k_blocks]
+  const float* ws; long long ws_group;  // per group [ceil(w rows / 128)][k_blocks]
+  const int* offsets; int n_groups;     // null, 0: one group of M rows
+  const float* row_weight;
   void* y; long long ldy;
   float* ys; long long ys_ld;           // kGluFp8: scales of the outputs, [block][row]
-  int m_tiles, n_tiles;
+  int m_tiles, n_tiles;                 // m_tiles: without groups
   GluEpilogue glu;
   int* status;
 };
 
-__device__ __forceinline__ void load_4d(void* dst, const CUtensorMap* map, int x, int row, int block, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n"
-      ::"r"(tma::smem_addr(dst)), "l"(map), "r"(x), "r"(row), "r"(0), "r"(block), "r"(tma::smem_addr(bar)) : "memory");
+// 64 bytes of each of a warp's 32 rows (a row a lane) to rows `row_bytes` apart, of which `n` are there: through shared memory, so that
+// four lanes store a row (a lane that stored its own row touched 32 lines with each instruction).  Rows of `buf` are 80 bytes, so that
+// the 16-byte accesses of eight lanes to eight rows fall into different banks.
+__device__ __forceinline__ void put64(char* buf, int lane, const uint4 (&v)[4], char* to, long long row_bytes, int n) {
+  uint4* mine = reinterpret_cast<uint4*>(buf + lane * kOutRow);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) mine[j] = v[j];
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = 8 * i + (lane >> 2), part = lane & 3;
+    if (r < n) *reinterpret_cast<uint4*>(to + (size_t)r * row_bytes + part * 16) = *reinterpret_cast<const uint4*>(buf + r * kOutRow + part * 16);
+  }
+  __syncwarp();
 }
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-template <int MODE>
+// GROUPS: rows grouped by expert, and weights on rows; the plain products keep kernels of their own, which have registers left.
+template <int MODE, bool GROUPS>
 __global__ void __launch_bounds__(kThreads, 1)
 gemm_fp8_many_kernel(Params p, const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap) {
   constexpr bool GLU = MODE == kGlu || MODE == kGluFp8;
@@ -74,7 +86,6 @@ gemm_fp8_many_kernel(Params p, const __grid_constant__ CUtensorMap amap, const _
   __shared__ int started[2];
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n_tiles_total = p.m_tiles * p.n_tiles;
   constexpr int kPerTile = GLU ? BN / 2 : BN;     // outputs of a row in a tile
 
   if (threadIdx.x == 0) {
@@ -95,12 +106,25 @@ gemm_fp8_many_kernel(Params p, const __grid_constant__ CUtensorMap amap, const _
   pdl_launch_dependents();
   fence_after_sync();
   const uint32_t tmem_base = tmem_holder;
+  // With groups the tiles of rows are those that the offsets give: none is empty.
+  const int m_tiles = GROUPS ? count_tiles(p.offsets, p.n_groups, p.M, BM) : p.m_tiles;
+  const int n_tiles_total = m_tiles * p.n_tiles;
+  auto find = [&](int tile, int& group, int& row0, int& rows) {         // all lanes of a warp take part
+    const int mt = tile % m_tiles;
+    group = 0;
+    row0 = mt * BM;
+    rows = min(BM, p.M - row0);
+    if (GROUPS) find_group(p.offsets, p.n_groups, p.M, BM, mt, group, row0, rows);
+  };
 
   int loaded = 0;                         // warps 0 and 1: blocks whose copies were started
   if (warp < 2) {
-    if (lane == 0) {
-      for (int tile = blockIdx.x; tile < n_tiles_total && !failed; tile += gridDim.x) {
-        const int m0 = (tile % p.m_tiles) * BM, n0 = (tile / p.m_tiles) * kPerTile;
+    for (int tile = blockIdx.x; tile < n_tiles_total; tile += gridDim.x) {
+      if (__any_sync(0xffffffffu, failed)) break;
+      int group, m0, rows;
+      find(tile, group, m0, rows);
+      const int n0 = (tile / m_tiles) * kPerTile;
+      if (lane == 0) {
         for (int kb = 0; kb < p.k_blocks; ++kb, ++loaded) {
           const int stage = loaded % STAGES;
           if (!tma::mbar_wait(&empty_bar[stage], ((loaded / STAGES) & 1) ^ 1)) {
@@ -115,16 +139,16 @@ gemm_fp8_many_kernel(Params p, const __grid_constant__ CUtensorMap amap, const _
             load_3d(to, &amap, x, m0, z, &full_bar[stage]);
           } else {
             tma::mbar_expect_tx(&full_bar[stage], kBytesB);
-            load_4d(to + kBytesA, &bmap, x, n0, z, &full_bar[stage]);
+            load_5d(to + kBytesA, &bmap, x, n0, z, group, &full_bar[stage]);
           }
         }
       }
+      __syncwarp();
     }
-    __syncwarp();
   } else if (warp == 2) {
     if (lane == 0) {
       constexpr uint32_t idesc = instr_desc(BM, BN);
-      const int my_tiles = (n_tiles_total - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
+      const int my_tiles = max(0, (n_tiles_total - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x);
       const int total = my_tiles * p.k_blocks;      // k blocks: block `it` goes to half it & 1 of tensor memory
       const uint32_t base = tma::smem_addr(smem);
       for (int it0 = 0; it0 < total && !failed; it0 += STAGES) {
@@ -133,13 +157,11 @@ gemm_fp8_many_kernel(Params p, const __grid_constant__ CUtensorMap amap, const _
           const int it = it0 + stage, half = stage & 1;
           if (it >= total) break;
           if (!tma::mbar_wait(&full_bar[stage], (it / STAGES) & 1)) failed = 1;
-          TR(0,it);
           if (!tma::mbar_wait(&full_bar[stage], (it / STAGES) & 1) || !tma::mbar_wait(&acc_empty[half], ((it >> 1) & 1) ^ 1)) {
             report(p.status, kStatusWaitTimedOut, 91, (int)blockIdx.x, it);
             failed = 1;
             break;
           }
-          TR(1,it);
           fence_after_sync();
           const uint32_t sa = base + stage * kStage, sb = sa + kBytesA;
 #pragma unroll
@@ -147,7 +169,6 @@ gemm_fp8_many_kernel(Params p, const __grid_constant__ CUtensorMap amap, const _
             umma(tmem_base + half * BN, smem_desc(sa + k * 32), smem_desc(sb + k * 32), idesc, k > 0 ? 1u : 0u);
           umma_commit(&acc_full[half]);
           umma_commit(&empty_bar[stage]);
-          TR(2,it);
         }
       }
     }
@@ -158,18 +179,22 @@ gemm_fp8_many_kernel(Params p, const __grid_constant__ CUtensorMap amap, const _
     const int quarter = warp & 3, h = (warp - kRoles) >> 2;
     const int r_tile = quarter * 32 + lane;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    char* out_buf = smem + STAGES * kStage + (warp - kRoles) * kOutWarp;
     // first columns of the thread's two runs of 64
     const int c0 = GLU ? h * 64 : h * 128, c1 = GLU ? 128 + h * 64 : h * 128 + 64;
     int it = 0;
     // the fused conversion has barriers in it: after a wait that ran out the warps go on without waiting
     for (int tile = blockIdx.x; tile < n_tiles_total; tile += gridDim.x) {
-      const int m0 = (tile % p.m_tiles) * BM, n0 = (tile / p.m_tiles) * kPerTile;
+      int group, m0, rows;
+      find(tile, group, m0, rows);
+      const int n0 = (tile / m_tiles) * kPerTile;
       const int row = m0 + r_tile;
-      const bool live = row < p.M;
+      const bool live = r_tile < rows;
       const float* sx_p = p.xs + (live ? row : 0);
       const int last = ((GLU ? 2 * p.N : p.N) - 1) / 128;
-      const float* sw0_p = p.ws + (size_t)min(GLU ? n0 / 128 : (n0 + c0) / 128, last) * p.k_blocks;
-      const float* sw1_p = p.ws + (size_t)min(GLU ? (p.N + n0) / 128 : (n0 + c0) / 128, last) * p.k_blocks;
+      const float* ws = p.ws + (size_t)group * p.ws_group;
+      const float* sw0_p = ws + (size_t)min(GLU ? n0 / 128 : (n0 + c0) / 128, last) * p.k_blocks;
+      const float* sw1_p = ws + (size_t)min(GLU ? (p.N + n0) / 128 : (n0 + c0) / 128, last) * p.k_blocks;
       unsigned long long sums[64];        // 128 sums, two neighbouring ones each
 #pragma unroll
       for (int j = 0; j < 64; ++j) sums[j] = 0ull;
@@ -187,7 +212,6 @@ gemm_fp8_many_kernel(Params p, const __grid_constant__ CUtensorMap amap, const _
           failed = 1;
         }
         __syncwarp();
-        if(lane==0 && warp==3) TR(3,it);
         fence_after_sync();
         const uint32_t t_row = tmem_base + half * BN + lanes;
         uint32_t v[2][16];
@@ -197,7 +221,6 @@ gemm_fp8_many_kernel(Params p, const __grid_constant__ CUtensorMap amap, const _
           tmem_ld_wait();
           if (q < 7) tmem_ld16(t_row + (q + 1 < 4 ? c0 + (q + 1) * 16 : c1 + (q - 3) * 16), v[(q + 1) & 1]);
           if (q == 7) {                   // all of the half is read: hand it back
-            if(lane==0) TR(warp+1,it);
             fence_before_sync();
             __syncwarp();
             if (lane == 0) tma::mbar_arrive(&acc_empty[half]);
@@ -214,40 +237,46 @@ gemm_fp8_many_kernel(Params p, const __grid_constant__ CUtensorMap amap, const _
         acc[2 * j] = f.x;
         acc[2 * j + 1] = f.y;
       }
+      // this warp's first row of y, and how many of its rows are there
+      const int es = MODE == kF32 ? 4 : MODE == kGluFp8 ? 1 : 2, n_rows = failed ? 0 : rows - quarter * 32;
+      const long long row_bytes = p.ldy * es;
+      char* first = reinterpret_cast<char*>(p.y) + (size_t)(m0 + quarter * 32) * row_bytes + (size_t)(n0 + c0) * es;
+      const bool vec = ((uintptr_t)p.y % 16) == 0 && row_bytes % 16 == 0;
       if constexpr (!GLU) {
-        if (live && !failed) {
-          const int left = p.N - (n0 + c0);
-          if (MODE == kF32) {
-            float* y = reinterpret_cast<float*>(p.y) + (size_t)row * p.ldy + n0 + c0;
-            const bool vec = ((uintptr_t)p.y % 16) == 0 && p.ldy % 4 == 0;
+        const int left = p.N - (n0 + c0);
+        constexpr int PER = 64 / (MODE == kF32 ? 4 : 2);        // outputs of a row that go together
 #pragma unroll
-            for (int j = 0; j < 128; j += 4) {
-              if (vec && j + 4 <= left) {
-                *reinterpret_cast<float4*>(y + j) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
-              } else {
+        for (int j = 0; j < 128; j += PER) {
+          if (vec && j + PER <= left) {
+            uint4 v[4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                  if (j + k < left) y[j + k] = acc[j + k];
-              }
+            for (int k = 0; k < 4; ++k) {
+              if (MODE == kF32)
+                v[k] = make_uint4(__float_as_uint(acc[j + 4 * k]), __float_as_uint(acc[j + 4 * k + 1]), __float_as_uint(acc[j + 4 * k + 2]),
+                                  __float_as_uint(acc[j + 4 * k + 3]));
+              else
+                v[k] = make_uint4(pack2(acc[(j + 8 * k) & 127], acc[(j + 8 * k + 1) & 127]), pack2(acc[(j + 8 * k + 2) & 127], acc[(j + 8 * k + 3) & 127]),
+                                  pack2(acc[(j + 8 * k + 4) & 127], acc[(j + 8 * k + 5) & 127]), pack2(acc[(j + 8 * k + 6) & 127], acc[(j + 8 * k + 7) & 127]));
             }
-          } else {
-            __nv_bfloat16* y = reinterpret_cast<__nv_bfloat16*>(p.y) + (size_t)row * p.ldy + n0 + c0;
-            const bool vec = ((uintptr_t)p.y % 16) == 0 && p.ldy % 8 == 0;
+            put64(out_buf, lane, v, first + j * es, row_bytes, n_rows);
+          } else if (lane < n_rows) {
+            char* y = first + (size_t)lane * row_bytes;
 #pragma unroll
-            for (int j = 0; j < 128; j += 8) {
-              if (vec && j + 8 <= left) {
-                *reinterpret_cast<uint4*>(y + j) = make_uint4(pack2(acc[j], acc[j + 1]), pack2(acc[j + 2], acc[j + 3]),
-                                                              pack2(acc[j + 4], acc[j + 5]), pack2(acc[j + 6], acc[j + 7]));
-              } else {
-#pragma unroll
-                for (int k = 0; k < 8; ++k)
-                  if (j + k < left) y[j + k] = __float2bfloat16_rn(acc[j + k]);
+            for (int k = 0; k < PER; ++k) {
+              if (j + k < left) {
+                if (MODE == kF32) reinterpret_cast<float*>(y)[j + k] = acc[j + k];
+                else reinterpret_cast<__nv_bfloat16*>(y)[j + k] = __float2bfloat16_rn(acc[j + k]);
               }
             }
           }
         }
       } else {
         // N is a multiple of 128 here: the tile's outputs are all there
+        if (GROUPS && p.row_weight && live) {
+          const float w = p.row_weight[row];
+#pragma unroll
+          for (int j = 0; j < 128; ++j) acc[j] *= w;
+        }
         uint32_t o[32];                   // 64 outputs as bfloat16
         if (p.glu.kind == 1 && p.glu.bias == nullptr) {
 #pragma unroll
@@ -268,16 +297,19 @@ gemm_fp8_many_kernel(Params p, const __grid_constant__ CUtensorMap amap, const _
           }
         }
         if (MODE == kGlu) {
-          if (live) {
-            __nv_bfloat16* y = reinterpret_cast<__nv_bfloat16*>(p.y) + (size_t)row * p.ldy + n0 + c0;
-            if (((uintptr_t)p.y % 16) == 0 && p.ldy % 8 == 0) {
 #pragma unroll
-              for (int j = 0; j < 8; ++j) reinterpret_cast<uint4*>(y)[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
-            } else {
+          for (int c = 0; c < 2; ++c) {
+            if (vec) {
+              uint4 v[4];
 #pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                y[2 * j] = reinterpret_cast<const __nv_bfloat162*>(o)[j].x;
-                y[2 * j + 1] = reinterpret_cast<const __nv_bfloat162*>(o)[j].y;
+              for (int k = 0; k < 4; ++k) v[k] = make_uint4(o[16 * c + 4 * k], o[16 * c + 4 * k + 1], o[16 * c + 4 * k + 2], o[16 * c + 4 * k + 3]);
+              put64(out_buf, lane, v, first + 64 * c, row_bytes, n_rows);
+            } else if (lane < n_rows) {
+              __nv_bfloat16* y = reinterpret_cast<__nv_bfloat16*>(first + (size_t)lane * row_bytes) + 32 * c;
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                y[2 * j] = reinterpret_cast<const __nv_bfloat162*>(o)[16 * c + j].x;
+                y[2 * j + 1] = reinterpret_cast<const __nv_bfloat162*>(o)[16 * c + j].y;
               }
             }
           }
@@ -302,12 +334,11 @@ gemm_fp8_many_kernel(Params p, const __grid_constant__ CUtensorMap amap, const _
             q8[j] = inf ? pack4(no_infinity(a.x) * by, no_infinity(a.y) * by, no_infinity(b.x) * by, no_infinity(b.y) * by)
                         : pack4(a.x * by, a.y * by, b.x * by, b.y * by);
           }
-          if (live) {
-            uint4* y = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(p.y) + (size_t)row * p.ldy + n0 + c0);
+          uint4 v[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) y[j] = make_uint4(q8[4 * j], q8[4 * j + 1], q8[4 * j + 2], q8[4 * j + 3]);
-            if (h == 0) p.ys[(size_t)(n0 / 128) * p.ys_ld + row] = __uint_as_float(scale);
-          }
+          for (int k = 0; k < 4; ++k) v[k] = make_uint4(q8[4 * k], q8[4 * k + 1], q8[4 * k + 2], q8[4 * k + 3]);
+          put64(out_buf, lane, v, first, row_bytes, n_rows);
+          if (h == 0 && lane < n_rows) p.ys[(size_t)(n0 / 128) * p.ys_ld + row] = __uint_as_float(scale);
           asm volatile("bar.sync 1, 256;\n" ::: "memory");     // the next tile writes top_s again
         }
       }
@@ -329,67 +360,62 @@ gemm_fp8_many_kernel(Params p, const __grid_constant__ CUtensorMap amap, const _
   }
 }
 
-// The weights as [block][half][row][128] (half: gates and ups; see fp8::make_map): a copy brings a block of a tile.
-static int make_weight_map(CUtensorMap* map, const void* w, const Params& p, uint64_t ld, bool glu) {
-  tma::EncodeTiledFn fn = tma::encode_fn();
-  if (fn == nullptr) return -5;
-  const cuuint32_t halves = glu ? 2 : 1;
-  cuuint64_t dims[4] = {p.whole ? (uint64_t)BK : p.K, (uint64_t)p.N, halves, p.whole ? (uint64_t)p.k_blocks : 1};
-  cuuint64_t strides[3] = {ld, (uint64_t)p.N * ld, (uint64_t)(p.whole ? BK : ld)};
-  cuuint32_t box[4] = {BK, BN / halves, halves, 1};
-  cuuint32_t estr[4] = {1, 1, 1, 1};
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(w), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? 0 : -2;
-}
-
-template <int MODE>
-static int launch_mode(const Params& p, const CUtensorMap& amap, const CUtensorMap& bmap, cudaStream_t stream) {
+template <int MODE, bool GROUPS>
+static int launch_groups(const Params& p, const CUtensorMap& amap, const CUtensorMap& bmap, cudaStream_t stream) {
   static bool attr_set = false;
   if (!attr_set) {
-    const cudaError_t ce = cudaFuncSetAttribute(gemm_fp8_many_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
+    const cudaError_t ce = cudaFuncSetAttribute(gemm_fp8_many_kernel<MODE, GROUPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
     if (ce != cudaSuccess) return (int)ce;
     attr_set = true;
   }
-  const int tiles = p.m_tiles * p.n_tiles;
-  const cudaError_t ce = pe::launch(gemm_fp8_many_kernel<MODE>, dim3(tiles < pe::kSMs ? tiles : pe::kSMs), dim3(kThreads), kSmem, stream, p, amap, bmap);
+  // with groups: as many tiles of rows as there can be
+  const long long most = p.n_groups > 0 ? p.M / BM + (p.n_groups < p.M ? p.n_groups : p.M) : p.m_tiles, tiles = most * p.n_tiles;
+  const cudaError_t ce = pe::launch(gemm_fp8_many_kernel<MODE, GROUPS>, dim3((unsigned)(tiles < pe::kSMs ? tiles : pe::kSMs)), dim3(kThreads), kSmem, stream, p, amap, bmap);
   if (ce != cudaSuccess) return (int)ce;
   PE_LAUNCH_CHECK();
   return PE_OK;
 }
 
+template <int MODE>
+static int launch_mode(const Params& p, const CUtensorMap& amap, const CUtensorMap& bmap, cudaStream_t stream) {
+  return p.n_groups > 0 ? launch_groups<MODE, true>(p, amap, bmap, stream) : launch_groups<MODE, false>(p, amap, bmap, stream);
+}
+
 }  // namespace fp8many
 }  // namespace pe
 
-// The arguments of pe_gemm_fp8 (gemm_fp8.cu) without groups; with an activation N is a multiple of 128.  y_scales (or null): the outputs
-// are quantised again, y is e4m3 (ldy bytes between rows, a multiple of 16) and y_scales[b * ys_ld + m] their blocks' scales.
+// The arguments of pe_gemm_fp8 (gemm_fp8.cu); with an activation N is a multiple of 128.  y_scales (or null): the outputs are
+// quantised again, y is e4m3 (ldy bytes between rows, a multiple of 16) and y_scales[b * ys_ld + m] their blocks' scales.
 extern "C" int pe_gemm_fp8_many(const void* x, long long x_ld, const float* x_scales, long long xs_ld, const void* w, long long w_ld,
                                 const float* w_scales, void* y, long long ldy, float* y_scales, long long ys_ld, int M, int N, int K,
-                                int out_f32, int kind, float limit, float alpha, const float* bias, int* status, cudaStream_t stream) {
+                                int out_f32, int kind, float limit, float alpha, const float* bias, const float* row_weight,
+                                const int* offsets, int n_groups, int* status, cudaStream_t stream) {
   using namespace pe::fp8many;
-  if (M < 0 || N < 0 || K < 1 || kind < 0 || kind > 3) return PE_ERR_BAD_ARGUMENT;
+  if (M < 0 || N < 0 || K < 1 || kind < 0 || kind > 3 || n_groups < 0) return PE_ERR_BAD_ARGUMENT;
   if (M == 0 || N == 0) return PE_OK;
   if (x == nullptr || x_scales == nullptr || w == nullptr || w_scales == nullptr || y == nullptr) return PE_ERR_BAD_ARGUMENT;
-  if (x_ld < K || w_ld < K || xs_ld < M || ldy < N || (kind > 0 && out_f32) || (kind == 0 && (bias || y_scales))) return PE_ERR_BAD_ARGUMENT;
+  if (x_ld < K || w_ld < K || xs_ld < M || ldy < N || (kind > 0 && out_f32) || (kind == 0 && (bias || y_scales)) || (row_weight && (kind == 0 || n_groups == 0)))
+    return PE_ERR_BAD_ARGUMENT;
+  if ((n_groups > 0) != (offsets != nullptr)) return PE_ERR_BAD_ARGUMENT;
   if (((uintptr_t)x % 16) || ((uintptr_t)w % 16) || (x_ld % 16) || (w_ld % 16)) return PE_ERR_BAD_ARGUMENT;
   if (y_scales && ((ldy % 16) || ((uintptr_t)y % 16) || ys_ld < M)) return PE_ERR_BAD_ARGUMENT;
-  if ((kind > 0 && N % 128) || N > (1 << 28)) return PE_ERR_UNSUPPORTED_SIZE;
+  if ((kind > 0 && N % 128) || N > (1 << 28) || (long long)(n_groups > 0 ? n_groups : 1) * N > (1 << 29)) return PE_ERR_UNSUPPORTED_SIZE;
   Params p;
   p.M = M; p.N = N; p.K = K; p.k_blocks = (K + BK - 1) / BK; p.whole = K % BK == 0;
   p.xs = x_scales; p.xs_ld = xs_ld; p.ws = w_scales;
+  const int w_rows = kind > 0 ? 2 * N : N;
+  p.ws_group = (long long)((w_rows + 127) / 128) * p.k_blocks;
+  p.offsets = offsets; p.n_groups = n_groups; p.row_weight = row_weight;
   p.y = y; p.ldy = ldy; p.ys = y_scales; p.ys_ld = ys_ld;
   p.m_tiles = (M + BM - 1) / BM;
   p.n_tiles = kind > 0 ? N / (BN / 2) : (N + BN - 1) / BN;
   p.glu = pe::GluEpilogue{kind, limit, alpha, bias};
   p.status = status;
-  if ((long long)p.m_tiles * p.n_tiles > 0x7fffffffLL) return PE_ERR_UNSUPPORTED_SIZE;
+  if (((long long)p.m_tiles + n_groups) * p.n_tiles * p.k_blocks > 0x7fffffffLL) return PE_ERR_UNSUPPORTED_SIZE;
   CUtensorMap amap, bmap;
   int e = make_map(&amap, x, K, M, x_ld, BM, p.whole, 1);
-  if (e == 0) e = make_weight_map(&bmap, w, p, w_ld, kind > 0);
+  if (e == 0) e = make_weight_map(&bmap, w, K, N, w_ld, kind > 0, n_groups > 0 ? n_groups : 1, BN / (kind > 0 ? 2 : 1), p.whole, 1);
   if (e != 0) return e;
   if (kind == 0) return out_f32 ? launch_mode<kF32>(p, amap, bmap, stream) : launch_mode<kBf16>(p, amap, bmap, stream);
   return y_scales ? launch_mode<kGluFp8>(p, amap, bmap, stream) : launch_mode<kGlu>(p, amap, bmap, stream);
 }
-
-extern "C" int trace_get(long long* out) { return (int)cudaMemcpyFromSymbol(out, pe::fp8many::g_trace, sizeof(long long)*16*128); }

@@ -1710,28 +1710,39 @@ def linear_fp8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: to
     _count(1 if raw else 2)
 
 
-def gemm_fp8_gated_supported(rows: int, width: int, k: int) -> bool:
+def gemm_fp8_gated_supported(rows: int, width: int, k: int, groups: int = 0) -> bool:
     """Whether ``gemm_fp8_gated`` takes a product of so many rows and ``width`` gates (many rows, a multiple of 128 gates)."""
-    return bool(library().pe_gemm_fp8_many_takes(rows, width, k, 1))
+    return bool(library().pe_gemm_fp8_many_takes(rows, width, k, 1, groups))
 
 
 def gemm_fp8_gated(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, values: torch.Tensor,
-                   scales: torch.Tensor, status: torch.Tensor, glu=()) -> None:
-    """``gemm_fp8`` with an activation whose outputs, rounded to bfloat16, are quantised on the way out (csrc/gemm_fp8_many.cu): e4m3
-    ``values [M, N]`` and ``scales [fp8_blocks(N), M]``, the bits that ``quantize_rows_fp8`` of ``gemm_fp8``'s output gives."""
+                   scales: torch.Tensor, status: torch.Tensor, glu=(), offsets: Optional[torch.Tensor] = None,
+                   row_weight: Optional[torch.Tensor] = None) -> None:
+    """``gemm_fp8`` (with ``offsets`` ``moe_rows_gemm_fp8``) with an activation whose outputs, rounded to bfloat16, are quantised on the
+    way out (csrc/gemm_fp8_many.cu): e4m3 ``values [M, N]`` and ``scales [fp8_blocks(N), M]``, the bits that ``quantize_rows_fp8`` of
+    the other's output gives."""
     what = "gemm_fp8_gated"
     m, k = x.shape
-    n = values.shape[1]
-    _need(values.dim() == 2 and values.shape[0] == m and w.dim() == 2 and tuple(w.shape) == (2 * n, k) and w.dtype == FP8, f"{what}: shapes do not match")
-    _need(gemm_fp8_gated_supported(m, n, k) or m == 0, f"{what}: not for {m} rows and {n} gates")
-    _need(w.stride(1) == 1 and w.stride(0) % 16 == 0, f"{what}: rows of w must be neighbouring values, a multiple of 16 bytes apart")
-    _need(w_scales.dtype == torch.float32 and w_scales.is_contiguous() and tuple(w_scales.shape) == (fp8_blocks(2 * n), fp8_blocks(k)), f"{what}: scales of w")
+    n, groups = values.shape[1], 0
+    if offsets is not None:
+        groups = w.shape[0]
+        _need(w.dim() == 3 and offsets.dtype == torch.int32 and offsets.is_contiguous() and offsets.numel() == groups + 1
+              and (groups == 1 or w.stride(0) == w.shape[1] * w.stride(1)), f"{what}: w [groups, 2 N, K] one behind the other, offsets int32, one more")
+    _need(values.dim() == 2 and values.shape[0] == m and w.dim() == (2 if offsets is None else 3) and tuple(w.shape[-2:]) == (2 * n, k)
+          and w.dtype == FP8, f"{what}: shapes do not match")
+    _need(gemm_fp8_gated_supported(m, n, k, groups) or m == 0, f"{what}: not for {m} rows and {n} gates")
+    _need(w.stride(-1) == 1 and w.stride(-2) % 16 == 0, f"{what}: rows of w must be neighbouring values, a multiple of 16 bytes apart")
+    _need(w_scales.dtype == torch.float32 and w_scales.is_contiguous() and tuple(w_scales.shape) == (*w.shape[:-2], fp8_blocks(2 * n), fp8_blocks(k)),
+          f"{what}: scales of w")
+    _need(row_weight is None or (offsets is not None and row_weight.dtype == torch.float32 and row_weight.is_contiguous()
+                                 and row_weight.numel() >= m), f"{what}: row_weight float32, one per row, with offsets")
     x_ld, xs_ld = _fp8_ld(x, what), _fp8_scales_ld(x_scales, fp8_blocks(k), m, what)
     y_ld, ys_ld = _fp8_ld(values, what), _fp8_scales_ld(scales, fp8_blocks(n), m, what)
-    _on_current(what, x, x_scales, w, w_scales, values, scales, status)
+    _on_current(what, x, x_scales, w, w_scales, values, scales, status, offsets, row_weight)
     if m == 0:
         return
     kind, limit, alpha, bias = _glu_args(glu or None, n)
-    check(library().pe_gemm_fp8_many(x.data_ptr(), x_ld, x_scales.data_ptr(), xs_ld, w.data_ptr(), w.stride(0), w_scales.data_ptr(), values.data_ptr(), y_ld,
-                                     scales.data_ptr(), ys_ld, m, n, k, 0, kind, limit, alpha, bias, status.data_ptr(), _stream()), what)
+    check(library().pe_gemm_fp8_many(x.data_ptr(), x_ld, x_scales.data_ptr(), xs_ld, w.data_ptr(), w.stride(-2), w_scales.data_ptr(), values.data_ptr(),
+                                     y_ld, scales.data_ptr(), ys_ld, m, n, k, 0, kind, limit, alpha, bias, _ptr(row_weight), _ptr(offsets), groups,
+                                     status.data_ptr(), _stream()), what)
     _count(1)

@@ -325,6 +325,14 @@ class Runtime:
         ``row_weight``: as in ``ops.moe_rows_gemm_fp8``.  Rows that no expert has are left as they are."""
         if not self.is_cuda:
             raise KernelError("this package computes on a CUDA device only; there is no CPU path")
-        act = torch.empty((out.shape[0], down.shape[2]), dtype=torch.bfloat16, device=x.device)
-        self._float8_product(x, gate_up, act, glu or (), offsets, row_weight, row_token)
+        groups, hidden, inter = down.shape
+        m = out.shape[0]
+        if m > 64 * groups and ops.gemm_fp8_gated_supported(m, inter, hidden, groups):
+            rows = Float8Rows.quantize(x, row_token, offsets[-1:], self.status)
+            act = Float8Rows.empty(m, inter, x.device)
+            ops.gemm_fp8_gated(rows.values, rows.scales, gate_up.values, gate_up.scales, act.values, act.scales, self.status, glu or (), offsets,
+                               row_weight)
+        else:
+            act = torch.empty((m, inter), dtype=torch.bfloat16, device=x.device)
+            self._float8_product(x, gate_up, act, glu or (), offsets, row_weight, row_token)
         return self._float8_product(act, down, out, None, offsets)

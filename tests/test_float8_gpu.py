@@ -500,3 +500,43 @@ def test_feed_forward(pe, ops, f8, m, hidden, inter):
     rt.float8_feed_forward(rows, gate_up, down, again)
     assert torch.equal(out, again)
     rt.raise_on_status()
+
+
+# many rows an expert: none, one tile, some, with a last tile of one row
+@pytest.mark.parametrize("counts", [[0, 128, 300, 1], [700, 0, 0, 500], [129] * 5])
+@pytest.mark.parametrize("weighted,inter,hidden", [(False, 256, 384), (True, 128, 272), (False, 200, 272)])
+def test_experts_of_many_rows(pe, ops, f8, counts, weighted, inter, hidden):
+    """The run of them, rows taken by a map, against each expert's feed-forward alone in 64 bits' definition of its two products."""
+    from pytorch_engine_b200.parts.runtime import Runtime
+
+    rt, groups, m = Runtime(DEV, BF16), len(counts), sum(counts)
+    offsets = torch.tensor([sum(counts[:i]) for i in range(groups + 1)], dtype=torch.int32, device=DEV)
+    src = rows_of(90, hidden, BF16, 1) * 0.01
+    pick = torch.randint(0, 90, (m,), device=DEV, dtype=torch.int32)
+    gate_up, down = weight_of(f8, 2 * inter, hidden, 1, groups), weight_of(f8, hidden, inter, 2, groups)
+    rw = torch.rand(m, device=DEV) if weighted else None
+    out = torch.full((m + 4, hidden), 5.0, dtype=BF16, device=DEV)
+    row_weight = torch.cat([rw, rw[:4]]) if weighted else None
+    rt.float8_experts(src, offsets, gate_up, down, out, row_weight=row_weight,
+                      row_token=torch.cat([pick, torch.full((4,), 10 ** 6, dtype=torch.int32, device=DEV)]))
+    rt.raise_on_status()
+    assert bool((out[m:] == 5.0).all())
+    x = f8.Float8Rows.quantize(src[pick.long()])
+    act = torch.empty(m, inter, dtype=BF16, device=DEV)
+    ops.moe_rows_gemm_fp8(x.values, x.scales, offsets, gate_up.values, gate_up.scales, act, rt.status, glu=(), row_weight=rw)
+    x64, w64 = wide_rows(x), wide(gate_up)
+    r = f8.Float8Rows.quantize(act)
+    r64, d64 = wide_rows(r), wide(down)
+    for e in range(groups):
+        at = slice(int(offsets[e]), int(offsets[e + 1]))
+        if counts[e] == 0:
+            continue
+        sums, err = x64[at] @ w64[e].t(), sum_error(x64[at], w64[e])
+        if weighted:
+            f = rw[at, None].to(F64)
+            sums, err = sums * f, err * f + 2.0 ** -23 * (sums * f).abs()
+        g, u = sums[:, :inter], sums[:, inter:]
+        want = plain_glu("silu", g, u, 0, 1)
+        assert_within(act[at], want, glu_bound("silu", g, u, err[:, :inter], err[:, inter:], 0, 1, want))
+        want = r64[at] @ d64[e].t()
+        assert_within(out[at], want, sum_error(r64[at], d64[e]) + 2.0 ** -8 * want.abs())

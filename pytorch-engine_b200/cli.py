@@ -27,6 +27,8 @@ def build_parser() -> argparse.ArgumentParser:
                      help="write the random model (config.json + model.safetensors) to DIR and exit")
     src.add_argument("--list-presets", action="store_true")
     p.add_argument("--dtype", choices=["bf16", "bfloat16", "fp32", "float32"], default="bf16")
+    p.add_argument("--weights", choices=["stored", "float8"], default="stored",
+                   help="float8: projections in 8-bit floating point, a scale for each 128 x 128 elements (bfloat16 runs)")
     p.add_argument("--ctx", type=int, default=None, help="max context window (default: the model's)")
     p.add_argument("--max-batch", type=int, default=64, help="most sequences decoded together")
     p.add_argument("--max-step-tokens", type=int, default=65536, help="most prompt tokens fed in one step (0: no limit)")
@@ -109,7 +111,8 @@ def main(argv=None) -> int:
         return 2
     kw = dict(dtype=args.dtype, max_context_len=args.ctx, max_batch=args.max_batch,
               max_step_tokens=args.max_step_tokens or None,
-              enable_cuda_graph=not args.no_cuda_graph, verbose=not args.json)
+              enable_cuda_graph=not args.no_cuda_graph, weight_format=None if args.weights == "stored" else args.weights,
+              verbose=not args.json)
     engine = Engine(args.model, **kw) if args.model else Engine.from_random(cfg, args.seed, **kw)
     params = SamplingParams(max_tokens=args.max_tokens, temperature=args.temperature, top_k=args.top_k,
                             top_p=args.top_p, min_p=args.min_p, repetition_penalty=args.repetition_penalty,

@@ -78,13 +78,17 @@ class Engine:
                  max_slots: Optional[int] = None, max_step_tokens: Optional[int] = 65536,
                  enable_cuda_graph: bool = True, device: str = "cuda:0",
                  config: Optional[ModelConfig] = None, weights: Optional[Dict[str, torch.Tensor]] = None,
-                 verbose: bool = False) -> None:
+                 weight_format: Optional[str] = None, verbose: bool = False) -> None:
         """``model_path``: a folder with config.json and model.safetensors.  ``max_context_len``: the
         longest sequence (default: the configuration's ``max_position_embeddings``).
         ``max_cache_tokens``: how many tokens all live sequences may hold together, each rounded up
         to 64 (default: ``max_batch`` sequences of full length, capped by free memory).
         ``max_step_tokens``: the most prompt tokens that generation feeds in one step (None: no limit); the
-        buffers of a step, beside the cache, grow with its tokens (about 100 KB per token at the 8B shape)."""
+        buffers of a step, beside the cache, grow with its tokens (about 100 KB per token at the 8B shape).
+        ``weight_format``: None (as stored) or "float8": the projections of attention, gated feed-forwards and routed experts are
+        quantised to e4m3 with a scale for each 128 x 128 elements when the model is built, and their inputs, in blocks of 128
+        features, in every step (bfloat16 runs only).  A checkpoint whose matrices are stored so (``name_scale_inv`` beside
+        ``name``) keeps them without it."""
         t0 = time.perf_counter()
         if not torch.cuda.is_available():
             raise KernelError("no CUDA device is visible: this engine runs on a B200 (sm_100a) only and has no CPU path")
@@ -100,6 +104,11 @@ class Engine:
         arch = architecture(config.architecture)
         self.plan = arch.plan(config)
         self.runtime = Runtime(self.device, self.dtype)
+        if weight_format not in (None, "float8"):
+            raise ValueError(f"weight_format must be None or 'float8', got {weight_format!r}")
+        if weight_format == "float8" and not self.runtime.takes_float8():
+            raise ValueError("weight_format 'float8' needs dtype bfloat16")
+        self.runtime.float8 = weight_format == "float8"
         self.max_context_len = int(max_context_len or config.max_positions)
         if self.max_context_len > config.max_positions:
             raise ValueError(f"max_context_len {self.max_context_len} exceeds the model's max_position_embeddings "

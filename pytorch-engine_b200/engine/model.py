@@ -12,6 +12,7 @@ from typing import Dict, Optional
 
 import torch
 
+from ..parts.float8 import Float8Weight
 from ..parts.registry import lookup
 from ..parts.spec import CacheRequest, ModelPlan, PartSpec
 
@@ -19,8 +20,11 @@ from ..parts.spec import CacheRequest, ModelPlan, PartSpec
 def _build_part(role: str, spec: PartSpec, weights: Dict[str, torch.Tensor], runtime, **extra):
     cls = lookup(role, spec.kind)
     local = {}
+    takes = getattr(cls, "takes_float8_weight", None) or (lambda name: name in getattr(cls, "float8_weights", ()))
     for name in cls.weight_decls(spec.params):
-        local[name] = weights[spec.weights[name]]
+        w = weights[spec.weights[name]]
+        # a checkpoint's 8-bit matrix for a part that has no product with such a weight: its numbers
+        local[name] = w.dequantize(runtime.dtype) if type(w) is Float8Weight and not takes(name) else w
     accepted = inspect.signature(cls.__init__).parameters
     extra = {k: v for k, v in extra.items() if k in accepted}
     return cls(spec.params, local, runtime, **extra)
@@ -140,9 +144,10 @@ class DecoderModel:
         def visit(obj):
             nonlocal total
             for v in vars(obj).values():
-                if isinstance(v, torch.Tensor) and v.data_ptr() not in seen:
-                    seen.add(v.data_ptr())
-                    total += v.numel() * v.element_size()
+                for t in (v.values, v.scales) if type(v) is Float8Weight else (v,):
+                    if isinstance(t, torch.Tensor) and t.data_ptr() not in seen:
+                        seen.add(t.data_ptr())
+                        total += t.numel() * t.element_size()
 
         visit(self.embedding)
         visit(self.final_norm)

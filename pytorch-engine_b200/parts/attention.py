@@ -14,7 +14,8 @@ from typing import Dict, Optional
 import torch
 
 from ..kernels import ops
-from .linear import fuse_rows
+from .float8 import Float8Weight
+from .linear import projection, wide
 from .registry import register
 from .spec import CacheRequest, WeightDecl
 
@@ -71,6 +72,9 @@ class GQAttention:
             decls["o_bias"] = WeightDecl((h,))
         return decls
 
+    # weights that may be 8-bit (parts/float8.py)
+    float8_weights = ("q_proj", "k_proj", "v_proj", "g_proj", "o_proj")
+
     @classmethod
     def cache_request(cls, params) -> Optional[CacheRequest]:
         d = int(params["head_dim"])
@@ -124,9 +128,10 @@ class GQAttention:
         if self.output_gate == "sigmoid_head":    # rows of the product stay 16-byte aligned
             rows = sum(t.shape[0] for t in fused)
             if rows % 8:
+                fused = [wide(t) for t in fused]
                 fused.append(torch.zeros((8 - rows % 8, self.hidden), dtype=fused[0].dtype, device=fused[0].device))
-        self.qkv = fuse_rows(runtime, fused)
-        self.o_proj = runtime.adopt(weights["o_proj"])
+        self.qkv = projection(runtime, fused)
+        self.o_proj = projection(runtime, [weights["o_proj"]])
         self.q_norm = self.k_norm = None
         if params.get("qk_norm", False):
             self.q_norm = runtime.adopt(weights["q_norm"], torch.float32)
@@ -195,7 +200,13 @@ class GQAttention:
 
     def chains(self) -> bool:
         """Whether ``forward`` takes a ``residual`` (parts/block.py, PreNormBlock)."""
-        return not self.general and ops.gemm_smallm_weight(self.qkv) and ops.gemm_smallm_weight(self.o_proj)
+        return (not self.general and type(self.qkv) is torch.Tensor and type(self.o_proj) is torch.Tensor
+                and ops.gemm_smallm_weight(self.qkv) and ops.gemm_smallm_weight(self.o_proj))
+
+    @property
+    def reads_float8(self) -> bool:
+        """Whether ``forward`` takes its rows as ``Float8Rows`` (parts/block.py, PreNormBlock)."""
+        return type(self.qkv) is Float8Weight
 
     def forward(self, x, ctx, view, writes_cache: bool = True, residual=None):
         """``x``: the normed rows; with ``residual`` (few rows) they may be ``ChainedRows``, and the output projection goes where
@@ -380,7 +391,7 @@ class GQAttention:
         """Whether this step's q|k|v product takes norm, rotation and append into its epilogue: the many-row tcgen05
         pair kernel must be the one that runs (as ``Runtime.linear`` would decide), the position encoding one that
         it can apply (rotary tables over the whole head, or none), the head size 128."""
-        if rt.gemm_backend is not None or not rt.fuse_qkv_rope or not rt.pair_gemm or not rt.takes_large_gemm(x, self.qkv):
+        if type(self.qkv) is Float8Weight or rt.gemm_backend is not None or not rt.fuse_qkv_rope or not rt.pair_gemm or not rt.takes_large_gemm(x, self.qkv):
             return False
         if self.position is not None and not self.fused_position:
             return False

@@ -8,6 +8,7 @@ from typing import Optional
 import torch
 
 from ..kernels import ops
+from .float8 import Float8Rows
 from .registry import register
 
 
@@ -146,15 +147,23 @@ class PreNormBlock:
         if chained and isinstance(pending, ChainedRows) and pending.norm is self.mixer_norm:
             x = pending
         else:
-            x = ctx.buffer("block.normed", tuple(stream.shape), rt.dtype)
-            self.mixer_norm.add_forward(stream, pending, x)
+            x = self.normed(self.mixer_norm, self.mixer, stream, pending, ctx)
         kw = {} if writes_cache else {"writes_cache": False}
         if chained:
             rows = self.mixer.forward(x, ctx, view, residual=Residual(stream, self.ffn_norm, ctx), **kw)
             return self.ffn.forward(rows, ctx, residual=Residual(stream, getattr(ctx, "following_norm", None), ctx))
         mixed = self.mixer.forward(x, ctx, view, **kw)
-        self.ffn_norm.add_forward(stream, mixed, x)
-        return self.ffn.forward(x, ctx)
+        return self.ffn.forward(self.normed(self.ffn_norm, self.ffn, stream, mixed, ctx), ctx)
+
+    def normed(self, norm, part, stream: torch.Tensor, pending, ctx):
+        """``norm`` of the stream with ``pending`` added, for ``part``: in 8 bits if it reads them and the norm writes them."""
+        if getattr(part, "reads_float8", False) and hasattr(norm, "add_forward_float8"):
+            rows = Float8Rows.of_buffers(ctx, "block.normed", *stream.shape)
+            if norm.add_forward_float8(stream, pending, rows):
+                return rows
+        x = ctx.buffer("block.normed", tuple(stream.shape), self.runtime.dtype)
+        norm.add_forward(stream, pending, x)
+        return x
 
 
 @register("arrangement", "post_norm")

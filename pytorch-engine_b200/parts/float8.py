@@ -43,6 +43,12 @@ class Float8Rows:
         return cls(_padded_empty((rows, width), device), torch.empty((fp8_blocks(width), rows), dtype=torch.float32, device=device))
 
     @classmethod
+    def of_buffers(cls, ctx, name: str, rows: int, width: int) -> "Float8Rows":
+        """Rows in the step's buffers ``name`` (one name, one set of rows at a time)."""
+        values = ctx.buffer(name + ".values", (rows, (width + 15) // 16 * 16), FP8)[:, :width]
+        return cls(values, ctx.buffer(name + ".scales", (fp8_blocks(width), rows), torch.float32))
+
+    @classmethod
     def quantize(cls, x: torch.Tensor, row_map: Optional[torch.Tensor] = None, live: Optional[torch.Tensor] = None,
                  status: Optional[torch.Tensor] = None) -> "Float8Rows":
         """``x [rows, K]`` in new storage (``row_map``, ``live``: see ``ops.quantize_rows_fp8``)."""

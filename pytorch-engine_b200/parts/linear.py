@@ -1,9 +1,11 @@
 """Helpers for parts that own projection matrices."""
 from __future__ import annotations
 
-from typing import Sequence
+from typing import Iterable, Sequence, Union
 
 import torch
+
+from .float8 import Float8Weight
 
 
 def fuse_rows(runtime, tensors: Sequence[torch.Tensor]) -> torch.Tensor:
@@ -11,3 +13,28 @@ def fuse_rows(runtime, tensors: Sequence[torch.Tensor]) -> torch.Tensor:
     (q|k|v and gate|up, as the reference does: pygguf_engine/quant_kernels.py:1874-1893)."""
     parts = [t.to(device=runtime.device, dtype=runtime.dtype) for t in tensors]
     return torch.cat(parts, dim=0).contiguous()
+
+
+def wide(tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """A weight as numbers of 16 or 32 bits: a checkpoint's 8-bit matrix times its scales, any other tensor as it is."""
+    return tensor.dequantize(dtype) if type(tensor) is Float8Weight else tensor
+
+
+def projection(runtime, tensors: Sequence) -> Union[torch.Tensor, Float8Weight]:
+    """A part's projection, the given matrices under each other: as ``fuse_rows`` makes it, or 8-bit.  A checkpoint's 8-bit
+    matrices stay as they are where the run takes them (``runtime.takes_float8``) and each but the last ends with a block of rows;
+    with ``runtime.float8`` everything else is quantised when the model is built."""
+    stored = [type(t) is Float8Weight for t in tensors]
+    if runtime.takes_float8():
+        if all(stored) and Float8Weight.stacks_rows(tensors):
+            return Float8Weight.cat_rows([t.to(runtime.device) for t in tensors]) if len(tensors) > 1 else tensors[0].to(runtime.device)
+        if runtime.float8:
+            return Float8Weight.quantize(fuse_rows(runtime, [wide(t) for t in tensors]))
+    if len(tensors) == 1 and not stored[0]:
+        return runtime.adopt(tensors[0])
+    return fuse_rows(runtime, [wide(t, runtime.dtype) for t in tensors])
+
+
+def quantized_stack(matrices: Iterable[torch.Tensor]) -> Float8Weight:
+    """Matrices of one shape, each quantised (or 8-bit already), as one weight ``[G, N, K]``."""
+    return Float8Weight.stack([m if type(m) is Float8Weight else Float8Weight.quantize(m) for m in matrices])

@@ -27,6 +27,8 @@ from typing import Dict
 import torch
 
 from ..kernels import ops
+from .float8 import Float8Weight
+from .linear import quantized_stack, wide
 from .registry import register
 from .spec import WeightDecl
 from .swiglu import SwiGLU
@@ -49,6 +51,11 @@ class RoutedExperts:
     [I, H]``, ``e<i>.down [H, I]``, and ``shared.gate, shared.up, shared.down`` with a shared expert."""
 
     graph_safe = True  # launches only; nothing in forward() waits for the device
+
+    @staticmethod
+    def takes_float8_weight(name: str) -> bool:
+        """Every expert's matrices may be 8-bit (parts/float8.py); the router is not."""
+        return "." in name
 
     @classmethod
     def weight_decls(cls, params) -> Dict[str, WeightDecl]:
@@ -100,10 +107,22 @@ class RoutedExperts:
             self.router_bias = runtime.adopt(weights["router_bias"], torch.float32)
         else:
             self.correction = runtime.adopt(weights["correction"], torch.float32)
-        if self.n_experts:
-            self.gate_up = torch.stack([torch.cat([weights[f"e{e}.gate"], weights[f"e{e}.up"]]).to(device=dev, dtype=dt)
-                                        for e in range(self.n_experts)]).contiguous()
-            self.down = torch.stack([weights[f"e{e}.down"].to(device=dev, dtype=dt) for e in range(self.n_experts)]).contiguous()
+        # 8-bit experts: quantised here, or the checkpoint's where every matrix is 8-bit and gates end with a block of rows
+        names = [f"e{e}.{n}" for e in range(self.n_experts) for n in ("gate", "up", "down")]
+        stored = bool(names) and all(type(weights[n]) is Float8Weight for n in names) and self.intermediate % ops.FP8_BLOCK == 0
+        self.float8 = bool(names) and runtime.takes_float8() and (runtime.float8 or stored)
+        if self.float8 and stored:
+            mine = {n: weights[n].to(dev) for n in names}
+            self.gate_up = Float8Weight.stack([Float8Weight.cat_rows([mine[f"e{e}.gate"], mine[f"e{e}.up"]]) for e in range(self.n_experts)])
+            self.down = Float8Weight.stack([mine[f"e{e}.down"] for e in range(self.n_experts)])
+        elif self.n_experts:
+            mine = {n: wide(weights[n], dt) for n in names}
+            gate_up = (torch.cat([mine[f"e{e}.gate"], mine[f"e{e}.up"]]).to(device=dev, dtype=dt) for e in range(self.n_experts))
+            down = (mine[f"e{e}.down"].to(device=dev, dtype=dt) for e in range(self.n_experts))
+            if self.float8:
+                self.gate_up, self.down = quantized_stack(gate_up), quantized_stack(down)
+            else:
+                self.gate_up, self.down = torch.stack(list(gate_up)).contiguous(), torch.stack(list(down)).contiguous()
         # the library's product over row groups takes bfloat16 rows that start on 16-byte boundaries
         self.library_product = (runtime.dtype == torch.bfloat16 and hasattr(torch, "_grouped_mm") and self.hidden % 8 == 0
                                 and self.intermediate % 8 == 0)
@@ -120,7 +139,7 @@ class RoutedExperts:
         experts, every expert runs on every row (all experts' gate|up rows as one stacked matrix, the down products as
         one grouped launch), and the sum takes the chosen ones."""
         rt = self.runtime
-        if not (self.n_experts and rt.dtype == torch.bfloat16 and rt.gemm_backend is None and rt.own_small_gemm
+        if not (self.n_experts and not self.float8 and rt.dtype == torch.bfloat16 and rt.gemm_backend is None and rt.own_small_gemm
                 and n <= rt.small_gemm_rows and 6 * n * self.top >= self.n_experts):
             return False
         return (self.hidden % 16 == 0 and self.intermediate % 8 == 0
@@ -170,7 +189,9 @@ class RoutedExperts:
         row_weight = ctx.buffer("moe.row_weight", (n * top,), torch.float32) if self.on_input else None
         ops.moe_group(chosen, n, top, self.n_experts, offsets, row_token, pair_row, weight, row_weight)
         rows = ctx.buffer("moe.rows", (n * top, self.hidden), rt.dtype)
-        if self.n_experts and self.library_product and n * top > LIBRARY_ROWS and rt.gemm_backend is None:
+        if self.float8:
+            rt.float8_experts(x, offsets, self.gate_up, self.down, rows, (self.activation, self.limit, self.alpha, None), row_weight, row_token)
+        elif self.n_experts and self.library_product and n * top > LIBRARY_ROWS and rt.gemm_backend is None:
             # many rows: the rows in expert order, then the library's product over row groups (bfloat16, float32 sums)
             xs = ctx.buffer("moe.xs", (n * top, self.hidden), rt.dtype)
             ops.moe_gather_rows(x, row_token, offsets, self.n_experts, xs)

@@ -7,6 +7,7 @@ from typing import Dict, Optional
 import torch
 
 from ..kernels import ops
+from .float8 import Float8Rows
 from .registry import register
 from .spec import WeightDecl
 
@@ -45,6 +46,14 @@ class RMSNorm:
             return out
         ops.rmsnorm_residual(residual, delta, self.weight, out, self.eps, rows)
         return out
+
+    def add_forward_float8(self, residual: torch.Tensor, delta: Optional[torch.Tensor], out: Float8Rows) -> bool:
+        """``add_forward`` whose rows go to an 8-bit product: the same values, quantised in the same kernel.  False (and nothing
+        done) for a width or a kind of delta that the kernel does not take."""
+        if not (ops.rmsnorm_residual_fp8_supported(self.dim) and (delta is None or (type(delta) is torch.Tensor and delta.dtype == torch.bfloat16))):
+            return False
+        ops.rmsnorm_residual_fp8(residual, delta, self.weight, out.values, out.scales, self.eps)
+        return True
 
     def forward(self, x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         out = torch.empty_like(x) if out is None else out

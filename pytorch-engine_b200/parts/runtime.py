@@ -128,6 +128,8 @@ class Runtime:
         # q/k-norm, rotation and cache append in the epilogue of the q|k|v product where the pair kernel runs it
         # (PE_B200_FUSE_QKV_ROPE=0 keeps them kernels of their own, for comparisons)
         self.fuse_qkv_rope = os.environ.get("PE_B200_FUSE_QKV_ROPE", "1") != "0"
+        # true: projections of attention, feed-forwards and experts are quantised to 8 bits when the model is built (parts/float8.py)
+        self.float8 = False
 
     # ---- weights -------------------------------------------------------------------------
     def adopt(self, tensor: torch.Tensor, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
@@ -140,6 +142,11 @@ class Runtime:
             got = tensor.to(device=self.device, dtype=dtype).contiguous()
             self._adopted[key] = got
         return got
+
+    def takes_float8(self) -> bool:
+        """Whether products may have 8-bit weights: in a bfloat16 run on a CUDA device (a float32 run is there to show what
+        rounding hides; it gets a checkpoint's 8-bit matrices times their scales)."""
+        return self.is_cuda and self.dtype == torch.bfloat16 and self.gemm_backend is None
 
     def forget_adopted(self) -> None:
         self._adopted.clear()

@@ -7,7 +7,8 @@ from typing import Dict
 import torch
 
 from ..kernels import ops
-from .linear import fuse_rows
+from .float8 import Float8Weight
+from .linear import projection
 from .registry import register
 from .spec import WeightDecl
 
@@ -23,6 +24,7 @@ class SwiGLU:
     library product they are a kernel of their own."""
 
     graph_safe = True  # launches only; nothing in forward() waits for the device
+    float8_weights = ("gate_proj", "up_proj", "down_proj")   # that may be 8-bit (parts/float8.py)
 
     @classmethod
     def weight_decls(cls, params) -> Dict[str, WeightDecl]:
@@ -41,8 +43,11 @@ class SwiGLU:
             raise ValueError(f"activation {self.activation!r} is not built ({', '.join(sorted(ops.GLU_KINDS))} are)")
         self.limit = float(params.get("limit") or 0.0)
         self.alpha = float(params.get("alpha") or 1.0)
-        self.gate_up = fuse_rows(runtime, [weights["gate_proj"], weights["up_proj"]])
-        self.down = runtime.adopt(weights["down_proj"])
+        self.gate_up = projection(runtime, [weights["gate_proj"], weights["up_proj"]])
+        self.down = projection(runtime, [weights["down_proj"]])
+        self.float8 = type(self.gate_up) is Float8Weight and type(self.down) is Float8Weight
+        if not self.float8:      # a checkpoint that has only one of the two in 8 bits, or gates that end inside a block
+            self.gate_up, self.down = (w.dequantize(runtime.dtype) if type(w) is Float8Weight else w for w in (self.gate_up, self.down))
         self.bias = self.out_bias = None
         self.out_bias_deferred = False
         if params.get("bias", False):
@@ -60,9 +65,14 @@ class SwiGLU:
         self.out_bias_deferred = True
         return self.out_bias
 
+    @property
+    def reads_float8(self) -> bool:
+        """Whether ``forward`` takes its rows as ``Float8Rows`` (parts/block.py, PreNormBlock)."""
+        return self.float8
+
     def chains(self) -> bool:
         """Whether ``forward`` takes a ``residual`` (parts/block.py, PreNormBlock)."""
-        return self.out_bias is None and ops.gemm_smallm_weight(self.gate_up) and ops.gemm_smallm_weight(self.down)
+        return not self.float8 and self.out_bias is None and ops.gemm_smallm_weight(self.gate_up) and ops.gemm_smallm_weight(self.down)
 
     def forward(self, x, ctx, residual=None):
         rt = self.runtime
@@ -71,6 +81,12 @@ class SwiGLU:
             ops.gemm_smallm_scaled(x.x, self.gate_up, act, x.squares, x.norm.eps, pair_offset=self.intermediate, glu=self.glu)
             return residual.add_product(act, self.down)
         n = x.shape[0]
+        if self.float8:
+            delta = ctx.buffer("ffn.delta", (n, self.hidden), rt.dtype)
+            rt.float8_feed_forward(x, self.gate_up, self.down, delta, self.glu)
+            if self.out_bias is not None and not self.out_bias_deferred:
+                delta.add_(self.out_bias)
+            return delta
         act = ctx.buffer("ffn.act", (n, self.intermediate), rt.dtype)
         if rt.takes_small_gemm(x, self.gate_up):
             # few rows: gate|up product with the activation in its epilogue

@@ -12,6 +12,10 @@ become int32.  A tensor's role decides what it may be stored as: a matrix, an em
 stored as integers is refused, and so is an integer table stored as floats (the reference refuses tensor
 types it does not know, pygguf_engine/gguf_parser.py:250-256).
 
+A matrix may be stored in 8-bit floating point (``F8_E4M3``) with a tensor ``name + "_scale_inv"`` beside it: the numbers that its
+blocks of 128 x 128 elements are multiplied by, 32- or 16-bit floats ``[blocks of rows, blocks of columns]``.  It is kept so
+(``parts/float8.py``); a part that has no product with such a weight, and a float32 run, get its numbers.
+
 Tensors the plan does not name are errors, with two exceptions that the plan itself declares:
 ``plan.duplicates`` (a name that may be in the file if it holds the same values as another tensor: a tied
 model whose file also stores ``lm_head.weight``) and ``plan.ignored`` (name patterns of buffers that carry
@@ -29,6 +33,7 @@ from typing import Dict, List, Optional, Tuple
 
 import torch
 
+from ..parts.float8 import Float8Weight
 from ..parts.registry import lookup
 from ..parts.spec import ModelPlan, WeightDecl
 
@@ -79,6 +84,8 @@ _FLOAT_KEEP = {torch.float32: torch.float32, torch.float64: torch.float32,
                torch.bfloat16: torch.bfloat16, torch.float16: torch.bfloat16}
 _INT_TYPES = (torch.int8, torch.int16, torch.int32, torch.int64, torch.uint8)
 _FLOAT_TAGS = ("F32", "F64", "F16", "BF16")
+_FLOAT8_TAG = "F8_E4M3"
+SCALE_SUFFIX = "_scale_inv"      # of the tensor that holds an 8-bit matrix's scales
 _INT_TAGS = ("I8", "I16", "I32", "I64", "U8")
 
 
@@ -128,13 +135,20 @@ def load_weights(folder: str, plan: ModelPlan, device="cpu", dtype: Optional[tor
                 sl = fh.get_slice(name)
                 where[name] = (path, tuple(sl.get_shape()), sl.get_dtype())
     missing = sorted(n for n in want if n not in where)
-    extra = [n for n in where if n not in want]
+    # 8-bit matrices and the scales beside them
+    scale_of = {n: n + SCALE_SUFFIX for n in want if n in where and where[n][2] == _FLOAT8_TAG and want[n].role == "matrix"}
+    missing = sorted(missing + [s for s in scale_of.values() if s not in where])
+    scales = {s for s in scale_of.values() if s in where}
+    extra = [n for n in where if n not in want and n not in scales]
     check_equal = sorted(n for n in extra if n in duplicates and duplicates[n] in want)
     unexpected = sorted(n for n in extra if n not in check_equal and not any(fnmatch.fnmatchcase(n, pat) for pat in ignored))
     wrong = sorted((n, where[n][1], tuple(want[n].shape)) for n in want
                    if n in where and not want[n].fits(where[n][1]))
-    bad_dtype = sorted((n, where[n][2], want[n].role, " / ".join(usable_tags(want[n].role))) for n in want
-                       if n in where and where[n][2] not in usable_tags(want[n].role))
+    wrong += sorted((s, where[s][1], tuple(-(-d // 128) for d in where[n][1])) for n, s in scale_of.items()
+                    if s in where and len(where[n][1]) == 2 and tuple(where[s][1]) != tuple(-(-d // 128) for d in where[n][1]))
+    bad_dtype = sorted([(n, where[n][2], want[n].role, " / ".join(usable_tags(want[n].role))) for n in want
+                        if n in where and n not in scale_of and where[n][2] not in usable_tags(want[n].role)]
+                       + [(s, where[s][2], "scale", " / ".join(_FLOAT_TAGS)) for s in scales if where[s][2] not in _FLOAT_TAGS])
     conflicting = []
     for n in check_equal:
         other = duplicates[n]
@@ -150,11 +164,14 @@ def load_weights(folder: str, plan: ModelPlan, device="cpu", dtype: Optional[tor
         raise WeightError(folder, missing, unexpected, wrong, bad_dtype, conflicting)
     out: Dict[str, torch.Tensor] = {}
     by_file: Dict[str, List[str]] = {}
-    for name in want:
+    for name in [*want, *scales]:
         by_file.setdefault(where[name][0], []).append(name)
     for path, names in by_file.items():
         with safe_open(path, framework="pt", device="cpu") as fh:
             for name in names:
                 t = fh.get_tensor(name)
-                out[name] = t.to(device=device, dtype=stored_dtype(t.dtype, dtype))
+                kept = torch.float32 if name in scales else t.dtype if name in scale_of else stored_dtype(t.dtype, dtype)
+                out[name] = t.to(device=device, dtype=kept)
+    for name, scale in scale_of.items():
+        out[name] = Float8Weight(out[name], out.pop(scale).contiguous())
     return out

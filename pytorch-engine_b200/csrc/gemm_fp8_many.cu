@@ -83,7 +83,7 @@ gemm_fp8_many_kernel(Params p, const __grid_constant__ CUtensorMap amap, const _
   __shared__ float top_s[2][BM];
   __shared__ uint32_t tmem_holder;
   __shared__ volatile int failed;
-  __shared__ int started[2];
+  __shared__ int started[2], issued;
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int kPerTile = GLU ? BN / 2 : BN;     // outputs of a row in a tile
@@ -97,10 +97,10 @@ gemm_fp8_many_kernel(Params p, const __grid_constant__ CUtensorMap amap, const _
       tma::mbar_init(&acc_full[b], 1);
       tma::mbar_init(&acc_empty[b], 8);   // the epilogue's warps
     }
-    failed = 0;
+    failed = issued = 0;
     tma::fence_barrier_init();
   }
-  if (warp == 2) tmem_alloc<1>(&tmem_holder, kTmemCols);
+  if (warp == 2) tmem_alloc(&tmem_holder, kTmemCols);
   fence_before_sync();
   pdl_wait_block();
   pdl_launch_dependents();
@@ -156,7 +156,6 @@ gemm_fp8_many_kernel(Params p, const __grid_constant__ CUtensorMap amap, const _
         for (int stage = 0; stage < STAGES; ++stage) {
           const int it = it0 + stage, half = stage & 1;
           if (it >= total) break;
-          if (!tma::mbar_wait(&full_bar[stage], (it / STAGES) & 1)) failed = 1;
           if (!tma::mbar_wait(&full_bar[stage], (it / STAGES) & 1) || !tma::mbar_wait(&acc_empty[half], ((it >> 1) & 1) ^ 1)) {
             report(p.status, kStatusWaitTimedOut, 91, (int)blockIdx.x, it);
             failed = 1;
@@ -169,6 +168,7 @@ gemm_fp8_many_kernel(Params p, const __grid_constant__ CUtensorMap amap, const _
             umma(tmem_base + half * BN, smem_desc(sa + k * 32), smem_desc(sb + k * 32), idesc, k > 0 ? 1u : 0u);
           umma_commit(&acc_full[half]);
           umma_commit(&empty_bar[stage]);
+          issued = it + 1;
         }
       }
     }
@@ -347,16 +347,18 @@ gemm_fp8_many_kernel(Params p, const __grid_constant__ CUtensorMap amap, const _
   if (warp < 2 && lane == 0) started[warp] = loaded;
   fence_before_sync();
   __syncthreads();
-  if (failed && threadIdx.x == 0) {       // copies still on their way to this block's shared memory
-    const int last = max(started[0], started[1]);
-    for (int i = max(0, last - STAGES); i < last; ++i) {
-      if (i >= started[0] || i >= started[1]) tma::mbar_arrive(&full_bar[i % STAGES]);     // for the operand that was not asked for
-      tma::mbar_wait(&full_bar[i % STAGES], (i / STAGES) & 1);
-    }
-  }
   if (warp == 2) {
+    if (failed && lane == 0) {            // MMAs that still read this block's shared memory, copies still on their way to it
+      for (int i = max(0, issued - STAGES); i < issued; ++i) tma::mbar_wait(&empty_bar[i % STAGES], (i / STAGES) & 1);
+      const int last = max(started[0], started[1]);
+      for (int i = max(0, last - STAGES); i < last; ++i) {
+        if (i >= started[0] || i >= started[1]) tma::mbar_arrive(&full_bar[i % STAGES]);     // for the operand that was not asked for
+        tma::mbar_wait(&full_bar[i % STAGES], (i / STAGES) & 1);
+      }
+    }
+    __syncwarp();
     fence_after_sync();
-    tmem_dealloc<1>(tmem_base, kTmemCols);
+    tmem_dealloc(tmem_base, kTmemCols);
   }
 }
 
@@ -393,6 +395,7 @@ extern "C" int pe_gemm_fp8_many(const void* x, long long x_ld, const float* x_sc
   using namespace pe::fp8many;
   if (M < 0 || N < 0 || K < 1 || kind < 0 || kind > 3 || n_groups < 0) return PE_ERR_BAD_ARGUMENT;
   if (M == 0 || N == 0) return PE_OK;
+  if (M > kMostRows || K > kMostRows) return PE_ERR_UNSUPPORTED_SIZE;
   if (x == nullptr || x_scales == nullptr || w == nullptr || w_scales == nullptr || y == nullptr) return PE_ERR_BAD_ARGUMENT;
   if (x_ld < K || w_ld < K || xs_ld < M || ldy < N || (kind > 0 && out_f32) || (kind == 0 && (bias || y_scales)) || (row_weight && (kind == 0 || n_groups == 0)))
     return PE_ERR_BAD_ARGUMENT;

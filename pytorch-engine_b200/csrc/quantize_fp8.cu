@@ -126,7 +126,8 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* x, long lon
 }
 
 // One thread block for 128 x 128 elements, which it holds in registers between the maximum and the conversion.  Its successor
-// in the stream may not start early: it may be a product that asks for these values before it waits.
+// in the stream may not start early: it may be a product that asks for these values before it waits (which only the dependents of a
+// grid with launch_dependents must do).
 template <typename T>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) quantize_weight_kernel(const T* w, long long w_ld, uint8_t* values, long long v_ld,
                                                                                     float* scales, int N, int K, bool vec) {
@@ -238,6 +239,7 @@ extern "C" int pe_quantize_rows_fp8(int dtype, const void* x, long long x_ld, co
   if (x == nullptr || values == nullptr || scales == nullptr || x_ld < K || v_ld < K || s_ld < M || x_rows < 1 || (!row_map && M > x_rows))
     return PE_ERR_BAD_ARGUMENT;
   if (((uintptr_t)values % 16) || (v_ld % 16)) return PE_ERR_BAD_ARGUMENT;
+  if (M > kMostRows || K > kMostRows) return PE_ERR_UNSUPPORTED_SIZE;
   if (dtype == PE_BF16) return launch_rows((const __nv_bfloat16*)x, x_ld, row_map, n_live, (uint8_t*)values, v_ld, scales, s_ld, M, K, x_rows, status, stream);
   if (dtype == PE_F32) return launch_rows((const float*)x, x_ld, row_map, n_live, (uint8_t*)values, v_ld, scales, s_ld, M, K, x_rows, status, stream);
   return PE_ERR_UNSUPPORTED_DTYPE;
@@ -251,6 +253,7 @@ extern "C" int pe_quantize_weight_fp8(int dtype, const void* w, long long w_ld, 
   if (N == 0 || K == 0) return PE_OK;
   if (w == nullptr || values == nullptr || scales == nullptr || w_ld < K || v_ld < K) return PE_ERR_BAD_ARGUMENT;
   if (((uintptr_t)values % 16) || (v_ld % 16)) return PE_ERR_BAD_ARGUMENT;
+  if (N > kMostRows || K > kMostRows) return PE_ERR_UNSUPPORTED_SIZE;
   const long long cells = (long long)((N + BLOCK - 1) / BLOCK) * ((K + BLOCK - 1) / BLOCK);
   if (cells > 0x7fffffffLL) return PE_ERR_UNSUPPORTED_SIZE;
   cudaError_t e;

@@ -1684,6 +1684,8 @@ def linear_fp8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: to
     """``quantize_rows_fp8`` of ``x`` (bfloat16 or float32, ``row_map`` as there), then ``gemm_fp8``, or with ``offsets``
     ``moe_rows_gemm_fp8``.  A handful of bfloat16 rows are quantised inside the product
     (``FP8_INSIDE_ROWS``)."""
+    if x.dim() != 2:
+        raise KernelError("linear_fp8: x must be a matrix")
     src_rows, k = x.shape
     x_ld, x_step = x.stride()
     if src_rows <= 1:

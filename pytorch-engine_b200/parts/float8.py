@@ -93,6 +93,8 @@ class Float8Weight:
     @classmethod
     def quantize(cls, w: torch.Tensor) -> "Float8Weight":
         """A matrix ``[N, K]`` on a CUDA device, quantised into new storage."""
+        if w.dim() != 2:
+            raise ValueError(f"a matrix is quantised, got {list(w.shape)}")
         values = _padded_empty(w.shape, w.device)
         scales = torch.empty((fp8_blocks(w.shape[0]), fp8_blocks(w.shape[1])), dtype=torch.float32, device=w.device)
         ops.quantize_weight_fp8(w, values, scales)

@@ -328,14 +328,16 @@ class Runtime:
     def float8_experts(self, x, offsets: torch.Tensor, gate_up: Float8Weight, down: Float8Weight, out: torch.Tensor, glu=None,
                        row_weight: Optional[torch.Tensor] = None, row_token: Optional[torch.Tensor] = None) -> torch.Tensor:
         """``float8_feed_forward`` with weights ``[experts, ...]`` for rows grouped by expert: rows ``offsets[e] .. offsets[e + 1]`` of
-        ``out [rows, hidden]`` come from expert e.  ``x``: the rows in that order, or with ``row_token`` (int32) rows to take them from.
-        ``row_weight``: as in ``ops.moe_rows_gemm_fp8``.  Rows that no expert has are left as they are."""
+        ``out [rows, hidden]`` come from expert e.  ``x``: the rows in that order (bfloat16, float32 or ``Float8Rows``), or with
+        ``row_token`` (int32) rows to take them from.  ``row_weight``: as in ``ops.moe_rows_gemm_fp8``.  Rows that no expert has are left as they are."""
         if not self.is_cuda:
             raise KernelError("this package computes on a CUDA device only; there is no CPU path")
+        if row_token is not None and type(x) is Float8Rows:
+            raise KernelError("rows taken from others are given in bfloat16 or float32, not quantised already")
         groups, hidden, inter = down.shape
         m = out.shape[0]
         if m > 64 * groups and ops.gemm_fp8_gated_supported(m, inter, hidden, groups):
-            rows = Float8Rows.quantize(x, row_token, offsets[-1:], self.status)
+            rows = x if type(x) is Float8Rows else Float8Rows.quantize(x, row_token, offsets[-1:], self.status)
             act = Float8Rows.empty(m, inter, x.device)
             ops.gemm_fp8_gated(rows.values, rows.scales, gate_up.values, gate_up.scales, act.values, act.scales, self.status, glu or (), offsets,
                                row_weight)

@@ -540,3 +540,88 @@ def test_experts_of_many_rows(pe, ops, f8, counts, weighted, inter, hidden):
         assert_within(act[at], want, glu_bound("silu", g, u, err[:, :inter], err[:, inter:], 0, 1, want))
         want = r64[at] @ d64[e].t()
         assert_within(out[at], want, sum_error(r64[at], d64[e]) + 2.0 ** -8 * want.abs())
+
+
+@pytest.mark.parametrize("counts", [[0, 3, 40, 1], [700, 0, 0, 500]])
+def test_experts_of_quantized_rows(pe, ops, f8, counts):
+    """Rows that are quantised already give the bits of the rows they come from; they cannot be taken by a map."""
+    from pytorch_engine_b200.parts.runtime import KernelError, Runtime
+
+    rt, groups, m, hidden, inter = Runtime(DEV, BF16), len(counts), sum(counts), 384, 256
+    offsets = torch.tensor([sum(counts[:i]) for i in range(groups + 1)], dtype=torch.int32, device=DEV)
+    x = rows_of(m, hidden, BF16, 1)
+    gate_up, down = weight_of(f8, 2 * inter, hidden, 1, groups), weight_of(f8, hidden, inter, 2, groups)
+    want, got = torch.empty(m, hidden, dtype=BF16, device=DEV), torch.empty(m, hidden, dtype=BF16, device=DEV)
+    rt.float8_experts(x, offsets, gate_up, down, want)
+    rows = f8.Float8Rows.quantize(x)
+    rt.float8_experts(rows, offsets, gate_up, down, got)
+    rt.raise_on_status()
+    assert torch.equal(got, want)
+    with pytest.raises(KernelError):
+        rt.float8_experts(rows, offsets, gate_up, down, got, row_token=torch.arange(m, dtype=torch.int32, device=DEV))
+
+
+def test_two_streams_at_once(pe, f8):
+    """Feed-forwards of two streams and of their graphs share weights and a status word, and nothing else."""
+    from pytorch_engine_b200.parts.runtime import Runtime
+
+    rt, hidden, inter = Runtime(DEV, BF16), 512, 384
+    gate_up, down = weight_of(f8, 2 * inter, hidden, 1), weight_of(f8, hidden, inter, 2)
+    sizes = (5, 300)
+    x = [rows_of(m, hidden, BF16, m) for m in sizes]
+    want = [torch.empty(m, hidden, dtype=BF16, device=DEV) for m in sizes]
+    for a, y in zip(x, want):
+        rt.float8_feed_forward(a, gate_up, down, y)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sizes]
+    out = [torch.zeros_like(y) for y in want]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for s, a, y in zip(streams, x, out):
+            with torch.cuda.stream(s):
+                rt.float8_feed_forward(a, gate_up, down, y)
+    torch.cuda.synchronize()
+    for y, w in zip(out, want):
+        assert torch.equal(y, w)
+        y.zero_()
+    torch.cuda.synchronize()
+    graphs = []
+    for s, a, y in zip(streams, x, out):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=s):
+            rt.float8_feed_forward(a, gate_up, down, y)
+    for _ in range(20):
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for y, w in zip(out, want):
+        assert torch.equal(y, w)
+    rt.raise_on_status()
+
+
+def test_weight_quantized_right_before(ops, f8, status):
+    """A weight that the launch right in front of its product writes, in storage that held another."""
+    m, k, n = 8, 4096, 6144
+    x = rows_of(m, k, BF16, 1)
+    r = f8.Float8Rows.quantize(x)
+    mats = [rows_of(n, k, BF16, 2 + i) for i in range(3)]
+    want = torch.empty(m, n, dtype=BF16, device=DEV)
+    out, w = torch.empty_like(want), f8.Float8Weight.quantize(mats[0])
+    for i in range(12):
+        fresh = f8.Float8Weight.quantize(mats[i % 3])
+        torch.cuda.synchronize()
+        ops.gemm_fp8(r.values, r.scales, fresh.values, fresh.scales, want, status)
+        ops.quantize_weight_fp8(mats[i % 3], w.values, w.scales)
+        ops.gemm_fp8(r.values, r.scales, w.values, w.scales, out, status)
+        assert torch.equal(out, want)
+
+
+def test_shapes_refused(pe, ops, f8, status):
+    from pytorch_engine_b200.parts.runtime import KernelError
+
+    w, y = weight_of(f8, 64, 256), torch.empty(1, 64, dtype=BF16, device=DEV)
+    with pytest.raises(KernelError):
+        ops.linear_fp8(torch.zeros(256, dtype=BF16, device=DEV), w.values, w.scales, y, status)
+    with pytest.raises(ValueError):
+        f8.Float8Weight.quantize(torch.zeros(256, device=DEV))

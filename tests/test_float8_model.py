@@ -127,6 +127,16 @@ def test_ops_refuse_cpu_tensors(pe):
 
 
 # ---- refusals on the GPU -----------------------------------------------------------------------------------------------------
+def test_sizes_refused(pe):
+    """More rows than the tiles' 32-bit arithmetic holds: refused on the host, before anything is launched."""
+    lib, p, big = pe.kernels.library(), 256, (1 << 30) + 1
+    act = (0, 0, 0.0, 1.0, None)
+    assert lib.pe_gemm_fp8(p, 128, p, big, p, 128, p, p, 64, big, 64, 128, *act, None, None, 0, p, None) == -1
+    assert lib.pe_gemm_fp8_many(p, 128, p, big, p, 128, p, p, 64, None, 0, big, 64, 128, *act, None, None, 0, p, None) == -1
+    assert lib.pe_quantize_rows_fp8(1, p, 128, None, None, p, 128, p, big, big, 128, big, p, None) == -1
+    assert lib.pe_quantize_weight_fp8(1, p, 128, p, 128, p, big, 128, None) == -1
+
+
 @pytest.mark.gpu
 def test_op_refusals(pe):
     ops, f8 = pe.kernels.ops, pe.parts.float8

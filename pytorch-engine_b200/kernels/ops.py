@@ -1488,24 +1488,28 @@ def fp8_blocks(n: int) -> int:
 
 def _fp8_ld(t: torch.Tensor, what: str) -> int:
     """Bytes between the rows of ``t [rows, K]``; one row may start anywhere 16 divides."""
-    rows, width = t.shape
-    _need(t.dtype == FP8 and (t.stride(1) == 1 or width == 1), f"{what}: float8_e4m3fn rows of neighbouring values")
+    (rows, width), (step, one) = t.shape, t.stride()
+    if t.dtype is not FP8 or (one != 1 and width != 1):
+        raise KernelError(f"{what}: float8_e4m3fn rows of neighbouring values")
     if rows <= 1:
         return (width + 15) // 16 * 16
-    _need(t.stride(0) % 16 == 0, f"{what}: rows must lie a multiple of 16 bytes apart")
-    return t.stride(0)
+    if step % 16:
+        raise KernelError(f"{what}: rows must lie a multiple of 16 bytes apart")
+    return step
 
 
 def _fp8_scales_ld(scales: torch.Tensor, blocks: int, rows: int, what: str) -> int:
-    _need(scales.dtype == torch.float32 and scales.dim() == 2 and scales.shape[0] == blocks and scales.shape[1] == rows
-          and (scales.stride(1) == 1 or rows == 1), f"{what}: scales [blocks of {FP8_BLOCK} features, rows] float32")
-    return max(scales.stride(0), rows) if blocks > 1 else rows
+    strides = scales.stride()
+    if scales.dtype is not torch.float32 or scales.shape != (blocks, rows) or (strides[1] != 1 and rows != 1):
+        raise KernelError(f"{what}: scales [blocks of {FP8_BLOCK} features, rows] float32")
+    return max(strides[0], rows) if blocks > 1 else rows
 
 
 def _on_current(what: str, *tensors) -> None:
     here = _current_device()
     for t in tensors:
-        _need(t is None or t.get_device() == here, f"{what}: tensors must lie on the current CUDA device")
+        if t is not None and t.get_device() != here:
+            raise KernelError(f"{what}: tensors must lie on the current CUDA device")
 
 
 def quantize_rows_fp8(x: torch.Tensor, values: torch.Tensor, scales: torch.Tensor, row_map: Optional[torch.Tensor] = None,
@@ -1546,10 +1550,10 @@ def new_rows_fp8(x: torch.Tensor, row_map: Optional[torch.Tensor] = None, live: 
     if row_map is not None:
         m = row_map.numel()
     ld = (k + 15) // 16 * 16
-    values = torch.empty((m, ld), dtype=FP8, device=x.device)
-    scales = torch.empty(((k + 127) >> 7, m), dtype=torch.float32, device=x.device)
+    values = torch.empty_strided((m, k), (ld, 1), dtype=FP8, device=x.device)
+    scales = torch.empty((k + 127) >> 7, m, dtype=torch.float32, device=x.device)
     _quantize_rows(x, m, k, values.data_ptr(), ld, scales.data_ptr(), m, row_map, live, status)
-    return (values if ld == k else values[:, :k]), scales
+    return values, scales
 
 
 def quantize_weight_fp8(w: torch.Tensor, values: torch.Tensor, scales: torch.Tensor) -> None:
@@ -1558,13 +1562,13 @@ def quantize_weight_fp8(w: torch.Tensor, values: torch.Tensor, scales: torch.Ten
     _need(w.dim() == 2 and w.shape == values.shape and (w.stride(1) == 1 or w.shape[1] == 1), "quantize_weight_fp8: matrices of one shape")
     n, k = w.shape
     v_ld = _fp8_ld(values, "quantize_weight_fp8")
-    _need(scales.dtype == torch.float32 and scales.is_contiguous() and tuple(scales.shape) == (fp8_blocks(n), fp8_blocks(k)),
-          f"quantize_weight_fp8: scales [blocks of {FP8_BLOCK} rows, blocks of {FP8_BLOCK} features] float32")
+    if scales.dtype is not torch.float32 or not scales.is_contiguous() or scales.shape != (fp8_blocks(n), fp8_blocks(k)):
+        raise KernelError(f"quantize_weight_fp8: scales [blocks of {FP8_BLOCK} rows, blocks of {FP8_BLOCK} features] float32")
     _on_current("quantize_weight_fp8", w, values, scales)
     if n == 0 or k == 0:
         return
-    check(library().pe_quantize_weight_fp8(dtype_tag(w.dtype), _ptr(w), w.stride(0) if n > 1 else k, _ptr(values), v_ld, _ptr(scales),
-                                           n, k, _stream()), "quantize_weight_fp8")
+    check(library().pe_quantize_weight_fp8(dtype_tag(w.dtype), w.data_ptr(), w.stride(0) if n > 1 else k, values.data_ptr(), v_ld,
+                                           scales.data_ptr(), n, k, _stream()), "quantize_weight_fp8")
     _count(1)
 
 
@@ -1582,11 +1586,11 @@ def rmsnorm_residual_fp8(residual: torch.Tensor, delta: Optional[torch.Tensor], 
           and weight.numel() == dim, "rmsnorm_residual_fp8: stream and weight float32")
     _need(delta is None or (delta.dtype == torch.bfloat16 and delta.is_contiguous() and delta.shape == residual.shape),
           "rmsnorm_residual_fp8: delta must be bfloat16 of the stream's shape")
-    _need(tuple(values.shape) == (n, dim), "rmsnorm_residual_fp8: values must have the stream's shape")
+    _need(values.shape == residual.shape, "rmsnorm_residual_fp8: values must have the stream's shape")
     v_ld, s_ld = _fp8_ld(values, "rmsnorm_residual_fp8"), _fp8_scales_ld(scales, fp8_blocks(dim), n, "rmsnorm_residual_fp8")
     _on_current("rmsnorm_residual_fp8", residual, delta, weight, values, scales)
-    check(library().pe_rmsnorm_residual_fp8(_ptr(residual), _ptr(delta), _ptr(weight), _ptr(values), v_ld, _ptr(scales), s_ld, n, dim,
-                                            float(eps), _stream()), "rmsnorm_residual_fp8")
+    check(library().pe_rmsnorm_residual_fp8(residual.data_ptr(), None if delta is None else delta.data_ptr(), weight.data_ptr(), values.data_ptr(),
+                                            v_ld, scales.data_ptr(), s_ld, n, dim, float(eps), _stream()), "rmsnorm_residual_fp8")
     _count(1)
 
 

@@ -16,10 +16,13 @@ from ..kernels.ops import FP8, FP8_BLOCK, fp8_blocks
 
 def _padded_empty(shape, device) -> torch.Tensor:
     """Uninitialised e4m3 ``[..., K]`` whose rows start on 16-byte boundaries."""
-    *lead, k = shape
+    k = shape[-1]
     if k % 16 == 0:
-        return torch.empty((*lead, k), dtype=FP8, device=device)
-    return torch.empty((*lead, (k + 15) // 16 * 16), dtype=FP8, device=device)[..., :k]
+        return torch.empty(*shape, dtype=FP8, device=device)
+    strides = [1, (k + 15) // 16 * 16]
+    for n in reversed(shape[1:-1]):
+        strides.append(strides[-1] * n)
+    return torch.empty_strided(shape, strides[::-1], dtype=FP8, device=device)
 
 
 class Float8Rows:
@@ -40,7 +43,7 @@ class Float8Rows:
 
     @classmethod
     def empty(cls, rows: int, width: int, device) -> "Float8Rows":
-        return cls(_padded_empty((rows, width), device), torch.empty((fp8_blocks(width), rows), dtype=torch.float32, device=device))
+        return cls(_padded_empty((rows, width), device), torch.empty(fp8_blocks(width), rows, dtype=torch.float32, device=device))
 
     @classmethod
     def of_buffers(cls, ctx, name: str, rows: int, width: int) -> "Float8Rows":
@@ -96,7 +99,7 @@ class Float8Weight:
         if w.dim() != 2:
             raise ValueError(f"a matrix is quantised, got {list(w.shape)}")
         values = _padded_empty(w.shape, w.device)
-        scales = torch.empty((fp8_blocks(w.shape[0]), fp8_blocks(w.shape[1])), dtype=torch.float32, device=w.device)
+        scales = torch.empty(fp8_blocks(w.shape[0]), fp8_blocks(w.shape[1]), dtype=torch.float32, device=w.device)
         ops.quantize_weight_fp8(w, values, scales)
         return cls(values, scales)
 

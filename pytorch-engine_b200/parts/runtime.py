@@ -249,7 +249,7 @@ class Runtime:
             raise KernelError("this package computes on a CUDA device only; there is no CPU path")
         if type(weight) is Float8Weight:
             if out is None:
-                out = torch.empty((x.shape[0], weight.shape[0]), dtype=out_dtype or torch.bfloat16, device=x.device)
+                out = torch.empty(x.shape[0], weight.shape[0], dtype=out_dtype or torch.bfloat16, device=x.device)
             return self._float8_product(x, weight, out)
         if self.gemm_backend is not None:
             y = self.gemm_backend(x, weight, out, out_dtype)

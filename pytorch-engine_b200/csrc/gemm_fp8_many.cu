@@ -22,7 +22,7 @@
 // Every wait is bounded; one that runs out records kStatusWaitTimedOut, every role leaves its loop, copies still in flight are
 // waited for (bounded again) and tensor memory is freed.
 #include "api.h"
-#include "fp8.cuh"
+#include "fp8_out.cuh"
 
 namespace pe {
 namespace fp8many {
@@ -34,44 +34,18 @@ constexpr int STAGES = 4;        // of one k block
 constexpr int kBytesA = BM * BK, kBytesB = BN * BK, kStage = kBytesA + kBytesB;
 constexpr int kTmemCols = 512;
 constexpr int kRoles = 3, kThreads = 32 * (kRoles + 8);
-constexpr int kOutRow = 80, kOutWarp = 32 * kOutRow;      // what an epilogue warp has for 64 bytes of each of its rows on their way out
 constexpr size_t kSmem = 1024 + (size_t)STAGES * kStage + 8 * kOutWarp;
-
-enum Mode { kBf16 = 0, kF32 = 1, kGlu = 2, kGluFp8 = 3 };
 
 struct Params {
   int M, N, K, k_blocks;                // N: output columns
-  bool whole;
+  bool whole, unless_powers;
   const float* xs; long long xs_ld;
-  const float* ws; long long ws_group;  // per group [ceil(w rows / 128)][k_blocks]
+  const float* ws; long long ws_group, ws_all;  // per group [ceil(w rows / 128)][k_blocks]; of all groups
   const int* offsets; int n_groups;     // null, 0: one group of M rows
-  const float* row_weight;
-  void* y; long long ldy;
-  float* ys; long long ys_ld;           // kGluFp8: scales of the outputs, [block][row]
   int m_tiles, n_tiles;                 // m_tiles: without groups
-  GluEpilogue glu;
+  Output out;
   int* status;
 };
-
-// 64 bytes of each of a warp's 32 rows (a row a lane) to rows `row_bytes` apart, of which `n` are there: through shared memory, so that
-// four lanes store a row (a lane that stored its own row touched 32 lines with each instruction).  Rows of `buf` are 80 bytes, so that
-// the 16-byte accesses of eight lanes to eight rows fall into different banks.
-__device__ __forceinline__ void put64(char* buf, int lane, const uint4 (&v)[4], char* to, long long row_bytes, int n) {
-  uint4* mine = reinterpret_cast<uint4*>(buf + lane * kOutRow);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) mine[j] = v[j];
-  __syncwarp();
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = 8 * i + (lane >> 2), part = lane & 3;
-    if (r < n) *reinterpret_cast<uint4*>(to + (size_t)r * row_bytes + part * 16) = *reinterpret_cast<const uint4*>(buf + r * kOutRow + part * 16);
-  }
-  __syncwarp();
-}
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
 
 // GROUPS: rows grouped by expert, and weights on rows; the plain products keep kernels of their own, which have registers left.
 template <int MODE, bool GROUPS>
@@ -88,6 +62,11 @@ gemm_fp8_many_kernel(Params p, const __grid_constant__ CUtensorMap amap, const _
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int kPerTile = GLU ? BN / 2 : BN;     // outputs of a row in a tile
 
+  if (p.unless_powers && all_powers(p.ws, p.ws_all)) {     // gemm_fp8_pair.cu's kernel, launched before this one, has done it
+    pdl_wait_block();
+    pdl_launch_dependents();
+    return;
+  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       tma::mbar_init(&full_bar[s], 2);    // the two producers
@@ -237,111 +216,7 @@ gemm_fp8_many_kernel(Params p, const __grid_constant__ CUtensorMap amap, const _
         acc[2 * j] = f.x;
         acc[2 * j + 1] = f.y;
       }
-      // this warp's first row of y, and how many of its rows are there
-      const int es = MODE == kF32 ? 4 : MODE == kGluFp8 ? 1 : 2, n_rows = failed ? 0 : rows - quarter * 32;
-      const long long row_bytes = p.ldy * es;
-      char* first = reinterpret_cast<char*>(p.y) + (size_t)(m0 + quarter * 32) * row_bytes + (size_t)(n0 + c0) * es;
-      const bool vec = ((uintptr_t)p.y % 16) == 0 && row_bytes % 16 == 0;
-      if constexpr (!GLU) {
-        const int left = p.N - (n0 + c0);
-        constexpr int PER = 64 / (MODE == kF32 ? 4 : 2);        // outputs of a row that go together
-#pragma unroll
-        for (int j = 0; j < 128; j += PER) {
-          if (vec && j + PER <= left) {
-            uint4 v[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              if (MODE == kF32)
-                v[k] = make_uint4(__float_as_uint(acc[j + 4 * k]), __float_as_uint(acc[j + 4 * k + 1]), __float_as_uint(acc[j + 4 * k + 2]),
-                                  __float_as_uint(acc[j + 4 * k + 3]));
-              else
-                v[k] = make_uint4(pack2(acc[(j + 8 * k) & 127], acc[(j + 8 * k + 1) & 127]), pack2(acc[(j + 8 * k + 2) & 127], acc[(j + 8 * k + 3) & 127]),
-                                  pack2(acc[(j + 8 * k + 4) & 127], acc[(j + 8 * k + 5) & 127]), pack2(acc[(j + 8 * k + 6) & 127], acc[(j + 8 * k + 7) & 127]));
-            }
-            put64(out_buf, lane, v, first + j * es, row_bytes, n_rows);
-          } else if (lane < n_rows) {
-            char* y = first + (size_t)lane * row_bytes;
-#pragma unroll
-            for (int k = 0; k < PER; ++k) {
-              if (j + k < left) {
-                if (MODE == kF32) reinterpret_cast<float*>(y)[j + k] = acc[j + k];
-                else reinterpret_cast<__nv_bfloat16*>(y)[j + k] = __float2bfloat16_rn(acc[j + k]);
-              }
-            }
-          }
-        }
-      } else {
-        // N is a multiple of 128 here: the tile's outputs are all there
-        if (GROUPS && p.row_weight && live) {
-          const float w = p.row_weight[row];
-#pragma unroll
-          for (int j = 0; j < 128; ++j) acc[j] *= w;
-        }
-        uint32_t o[32];                   // 64 outputs as bfloat16
-        if (p.glu.kind == 1 && p.glu.bias == nullptr) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) o[j] = pack2(silu_mul_fast(acc[2 * j], acc[64 + 2 * j]), silu_mul_fast(acc[2 * j + 1], acc[64 + 2 * j + 1]));
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            float g[2] = {acc[2 * j], acc[2 * j + 1]}, u[2] = {acc[64 + 2 * j], acc[64 + 2 * j + 1]};
-            if (p.glu.bias) {
-              const int col = n0 + c0 + 2 * j;
-#pragma unroll
-              for (int k = 0; k < 2; ++k) {
-                g[k] += p.glu.bias[col + k];
-                u[k] += p.glu.bias[p.N + col + k];
-              }
-            }
-            o[j] = glu_fast_pair(p.glu, g[0], g[1], u[0], u[1]);
-          }
-        }
-        if (MODE == kGlu) {
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            if (vec) {
-              uint4 v[4];
-#pragma unroll
-              for (int k = 0; k < 4; ++k) v[k] = make_uint4(o[16 * c + 4 * k], o[16 * c + 4 * k + 1], o[16 * c + 4 * k + 2], o[16 * c + 4 * k + 3]);
-              put64(out_buf, lane, v, first + 64 * c, row_bytes, n_rows);
-            } else if (lane < n_rows) {
-              __nv_bfloat16* y = reinterpret_cast<__nv_bfloat16*>(first + (size_t)lane * row_bytes) + 32 * c;
-#pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                y[2 * j] = reinterpret_cast<const __nv_bfloat162*>(o)[16 * c + j].x;
-                y[2 * j + 1] = reinterpret_cast<const __nv_bfloat162*>(o)[16 * c + j].y;
-              }
-            }
-          }
-        } else {
-          float top = 0.f;
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const float2 f = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(o)[j]);
-            top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
-          }
-          top_s[h][r_tile] = top;         // the other half of the row's 128 outputs is another warp's
-          asm volatile("bar.sync 1, 256;\n" ::: "memory");
-          top = fmaxf(top_s[0][r_tile], top_s[1][r_tile]);
-          const uint32_t scale = scale_bits(top);
-          const float by = inverse_of(scale);
-          const bool inf = top == INFINITY;
-          uint32_t q8[16];
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float2 a = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(o)[2 * j]);
-            const float2 b = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(o)[2 * j + 1]);
-            q8[j] = inf ? pack4(no_infinity(a.x) * by, no_infinity(a.y) * by, no_infinity(b.x) * by, no_infinity(b.y) * by)
-                        : pack4(a.x * by, a.y * by, b.x * by, b.y * by);
-          }
-          uint4 v[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) v[k] = make_uint4(q8[4 * k], q8[4 * k + 1], q8[4 * k + 2], q8[4 * k + 3]);
-          put64(out_buf, lane, v, first, row_bytes, n_rows);
-          if (h == 0 && lane < n_rows) p.ys[(size_t)(n0 / 128) * p.ys_ld + row] = __uint_as_float(scale);
-          asm volatile("bar.sync 1, 256;\n" ::: "memory");     // the next tile writes top_s again
-        }
-      }
+      finish_tile<MODE, GROUPS>(p.out, acc, m0, rows, n0, h, quarter, lane, failed != 0, out_buf, top_s);
     }
   }
   if (warp < 2 && lane == 0) started[warp] = loaded;
@@ -384,15 +259,12 @@ static int launch_mode(const Params& p, const CUtensorMap& amap, const CUtensorM
 }
 
 }  // namespace fp8many
-}  // namespace pe
 
-// The arguments of pe_gemm_fp8 (gemm_fp8.cu); with an activation N is a multiple of 128.  y_scales (or null): the outputs are
-// quantised again, y is e4m3 (ldy bytes between rows, a multiple of 16) and y_scales[b * ys_ld + m] their blocks' scales.
-extern "C" int pe_gemm_fp8_many(const void* x, long long x_ld, const float* x_scales, long long xs_ld, const void* w, long long w_ld,
-                                const float* w_scales, void* y, long long ldy, float* y_scales, long long ys_ld, int M, int N, int K,
-                                int out_f32, int kind, float limit, float alpha, const float* bias, const float* row_weight,
-                                const int* offsets, int n_groups, int* status, cudaStream_t stream) {
-  using namespace pe::fp8many;
+int fp8::gemm_many(bool unless_powers, const void* x, long long x_ld, const float* x_scales, long long xs_ld, const void* w, long long w_ld,
+                   const float* w_scales, void* y, long long ldy, float* y_scales, long long ys_ld, int M, int N, int K, int out_f32,
+                   int kind, float limit, float alpha, const float* bias, const float* row_weight, const int* offsets, int n_groups,
+                   int* status, cudaStream_t stream) {
+  using namespace fp8many;
   if (M < 0 || N < 0 || K < 1 || kind < 0 || kind > 3 || n_groups < 0) return PE_ERR_BAD_ARGUMENT;
   if (M == 0 || N == 0) return PE_OK;
   if (M > kMostRows || K > kMostRows) return PE_ERR_UNSUPPORTED_SIZE;
@@ -408,11 +280,12 @@ extern "C" int pe_gemm_fp8_many(const void* x, long long x_ld, const float* x_sc
   p.xs = x_scales; p.xs_ld = xs_ld; p.ws = w_scales;
   const int w_rows = kind > 0 ? 2 * N : N;
   p.ws_group = (long long)((w_rows + 127) / 128) * p.k_blocks;
-  p.offsets = offsets; p.n_groups = n_groups; p.row_weight = row_weight;
-  p.y = y; p.ldy = ldy; p.ys = y_scales; p.ys_ld = ys_ld;
+  p.ws_all = p.ws_group * (n_groups > 0 ? n_groups : 1);
+  p.unless_powers = unless_powers;
+  p.offsets = offsets; p.n_groups = n_groups;
   p.m_tiles = (M + BM - 1) / BM;
   p.n_tiles = kind > 0 ? N / (BN / 2) : (N + BN - 1) / BN;
-  p.glu = pe::GluEpilogue{kind, limit, alpha, bias};
+  p.out = Output{N, y, ldy, y_scales, ys_ld, row_weight, pe::GluEpilogue{kind, limit, alpha, bias}};
   p.status = status;
   if (((long long)p.m_tiles + n_groups) * p.n_tiles * p.k_blocks > 0x7fffffffLL) return PE_ERR_UNSUPPORTED_SIZE;
   CUtensorMap amap, bmap;
@@ -421,4 +294,16 @@ extern "C" int pe_gemm_fp8_many(const void* x, long long x_ld, const float* x_sc
   if (e != 0) return e;
   if (kind == 0) return out_f32 ? launch_mode<kF32>(p, amap, bmap, stream) : launch_mode<kBf16>(p, amap, bmap, stream);
   return y_scales ? launch_mode<kGluFp8>(p, amap, bmap, stream) : launch_mode<kGlu>(p, amap, bmap, stream);
+}
+
+}  // namespace pe
+
+// The arguments of pe_gemm_fp8 (gemm_fp8.cu); with an activation N is a multiple of 128.  y_scales (or null): the outputs are
+// quantised again, y is e4m3 (ldy bytes between rows, a multiple of 16) and y_scales[b * ys_ld + m] their blocks' scales.
+extern "C" int pe_gemm_fp8_many(const void* x, long long x_ld, const float* x_scales, long long xs_ld, const void* w, long long w_ld,
+                                const float* w_scales, void* y, long long ldy, float* y_scales, long long ys_ld, int M, int N, int K,
+                                int out_f32, int kind, float limit, float alpha, const float* bias, const float* row_weight,
+                                const int* offsets, int n_groups, int* status, cudaStream_t stream) {
+  return pe::fp8::gemm_many(false, x, x_ld, x_scales, xs_ld, w, w_ld, w_scales, y, ldy, y_scales, ys_ld, M, N, K, out_f32, kind, limit, alpha,
+                            bias, row_weight, offsets, n_groups, status, stream);
 }

@@ -26,12 +26,13 @@ def _padded_empty(shape, device) -> torch.Tensor:
 
 
 class Float8Rows:
-    """``values [M, K]`` (e4m3) and ``scales [fp8_blocks(K), M]`` (float32)."""
+    """``values [M, K]`` (e4m3) and ``scales [fp8_blocks(K), M]`` (float32).  ``powers``: the scales are powers of two, as this
+    package's conversions make them (``empty`` and ``of_buffers`` are for those to fill)."""
 
-    __slots__ = ("values", "scales")
+    __slots__ = ("values", "scales", "powers")
 
-    def __init__(self, values: torch.Tensor, scales: torch.Tensor) -> None:
-        self.values, self.scales = values, scales
+    def __init__(self, values: torch.Tensor, scales: torch.Tensor, powers: bool = False) -> None:
+        self.values, self.scales, self.powers = values, scales, powers
 
     @property
     def shape(self) -> torch.Size:
@@ -43,40 +44,46 @@ class Float8Rows:
 
     @classmethod
     def empty(cls, rows: int, width: int, device) -> "Float8Rows":
-        return cls(_padded_empty((rows, width), device), torch.empty(fp8_blocks(width), rows, dtype=torch.float32, device=device))
+        return cls(_padded_empty((rows, width), device), torch.empty(fp8_blocks(width), rows, dtype=torch.float32, device=device), True)
 
     @classmethod
     def of_buffers(cls, ctx, name: str, rows: int, width: int) -> "Float8Rows":
         """Rows in the step's buffers ``name`` (one name, one set of rows at a time)."""
         values = ctx.buffer(name + ".values", (rows, (width + 15) // 16 * 16), FP8)[:, :width]
-        return cls(values, ctx.buffer(name + ".scales", (fp8_blocks(width), rows), torch.float32))
+        return cls(values, ctx.buffer(name + ".scales", (fp8_blocks(width), rows), torch.float32), True)
 
     @classmethod
     def quantize(cls, x: torch.Tensor, row_map: Optional[torch.Tensor] = None, live: Optional[torch.Tensor] = None,
                  status: Optional[torch.Tensor] = None) -> "Float8Rows":
         """``x [rows, K]`` in new storage (``row_map``, ``live``: see ``ops.quantize_rows_fp8``)."""
-        return cls(*ops.new_rows_fp8(x, row_map, live, status))
+        return cls(*ops.new_rows_fp8(x, row_map, live, status), True)
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         s = self.scales.repeat_interleave(FP8_BLOCK, 0)[:self.values.shape[1]].t()
         return (self.values.to(torch.float32) * s).to(dtype)
 
 
+def _all_powers(weights) -> Optional[bool]:
+    known = [w.powers for w in weights]
+    return False if False in known else None if None in known else True
+
+
 class Float8Weight:
     """``values [N, K]`` (e4m3) and ``scales [fp8_blocks(N), fp8_blocks(K)]`` (float32); or several such matrices stacked in
-    front, ``[G, N, K]`` and ``[G, ...]``.  Rows start on 16-byte boundaries (``aligned`` makes it so)."""
+    front, ``[G, N, K]`` and ``[G, ...]``.  Rows start on 16-byte boundaries (``to`` makes it so).  ``powers``: whether all scales are
+    powers of two; None: not known (a product of many rows then looks, ``to`` does it once)."""
 
-    __slots__ = ("values", "scales")
+    __slots__ = ("values", "scales", "powers")
     dtype = FP8
 
-    def __init__(self, values: torch.Tensor, scales: torch.Tensor) -> None:
+    def __init__(self, values: torch.Tensor, scales: torch.Tensor, powers: Optional[bool] = None) -> None:
         shape = values.shape
         if values.dtype is not FP8 or scales.dtype is not torch.float32:
             raise ValueError(f"an 8-bit weight is float8_e4m3fn with float32 scales, got {values.dtype} and {scales.dtype}")
         want = (*shape[:-2], (shape[-2] + 127) >> 7, (shape[-1] + 127) >> 7)
         if scales.shape != want:
             raise ValueError(f"an 8-bit weight {list(values.shape)} has scales {list(want)}, got {list(scales.shape)}")
-        self.values, self.scales = values, scales
+        self.values, self.scales, self.powers = values, scales, powers
 
     @property
     def shape(self) -> torch.Size:
@@ -91,7 +98,7 @@ class Float8Weight:
 
     def __getitem__(self, i: int) -> "Float8Weight":
         """One of several stacked matrices."""
-        return Float8Weight(self.values[i], self.scales[i])
+        return Float8Weight(self.values[i], self.scales[i], self.powers or None)
 
     @classmethod
     def quantize(cls, w: torch.Tensor) -> "Float8Weight":
@@ -101,7 +108,7 @@ class Float8Weight:
         values = _padded_empty(w.shape, w.device)
         scales = torch.empty(fp8_blocks(w.shape[0]), fp8_blocks(w.shape[1]), dtype=torch.float32, device=w.device)
         ops.quantize_weight_fp8(w, values, scales)
-        return cls(values, scales)
+        return cls(values, scales, True)
 
     @classmethod
     def stack(cls, weights: Sequence["Float8Weight"]) -> "Float8Weight":
@@ -110,7 +117,7 @@ class Float8Weight:
         values = _padded_empty((len(weights), *first.shape), first.device)
         for i, w in enumerate(weights):
             values[i].copy_(w.values)
-        return cls(values, torch.stack([w.scales for w in weights]).contiguous())
+        return cls(values, torch.stack([w.scales for w in weights]).contiguous(), _all_powers(weights))
 
     @staticmethod
     def stacks_rows(weights: Sequence["Float8Weight"]) -> bool:
@@ -127,15 +134,19 @@ class Float8Weight:
         for w in weights:
             values[at:at + w.shape[0]].copy_(w.values)
             at += w.shape[0]
-        return cls(values, torch.cat([w.scales for w in weights]).contiguous())
+        return cls(values, torch.cat([w.scales for w in weights]).contiguous(), _all_powers(weights))
 
     def to(self, device) -> "Float8Weight":
-        """On ``device``, with rows on 16-byte boundaries."""
-        if self.values.device == torch.device(device) and self.values.stride(-2) % 16 == 0 and self.values.data_ptr() % 16 == 0:
-            return Float8Weight(self.values, self.scales.contiguous())
-        values = _padded_empty(self.shape, device)
-        values.copy_(self.values)
-        return Float8Weight(values, self.scales.to(device).contiguous())
+        """On ``device``, with rows on 16-byte boundaries, and ``powers`` known (for which the host waits for the device)."""
+        values, scales = self.values, self.scales.to(device).contiguous()
+        if values.device != torch.device(device) or values.stride(-2) % 16 or values.data_ptr() % 16:
+            values = _padded_empty(self.shape, device)
+            values.copy_(self.values)
+        powers = self.powers
+        if powers is None:
+            bits = scales.view(torch.int32)
+            powers = bool(((bits & 0x7fffff) == 0).logical_and_(bits > 0).logical_and_(bits != 0x7f800000).all())
+        return Float8Weight(values, scales, powers)
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         n, k = self.shape[-2:]

@@ -349,10 +349,10 @@ int pe_linear_fp8(int dtype, const void* x, long long x_ld, const int* row_map, 
 int pe_gemm_fp8_many_takes(int M, int N, int K, int kind, int n_groups);
 
 // gemm_fp8_many.cu
-int pe_gemm_fp8_pair_takes(int M, int N, int K, int kind, int n_groups, int known);
+int pe_gemm_fp8_pair_takes(int M, int N, int K, int kind, int n_groups);
 int pe_gemm_fp8_pair(const void* x, long long x_ld, const float* x_scales, long long xs_ld, const void* w, long long w_ld,
     const float* w_scales, void* y, long long ldy, float* y_scales, long long ys_ld, int M, int N, int K, int out_f32, int kind,
-    float limit, float alpha, const float* bias, const float* row_weight, const int* offsets, int n_groups, int check, int* status,
+    float limit, float alpha, const float* bias, const float* row_weight, const int* offsets, int n_groups, int* status,
     cudaStream_t stream);
 int pe_gemm_fp8_many(const void* x, long long x_ld, const float* x_scales, long long xs_ld, const void* w, long long w_ld,
     const float* w_scales, void* y, long long ldy, float* y_scales, long long ys_ld, int M, int N, int K, int out_f32, int kind,

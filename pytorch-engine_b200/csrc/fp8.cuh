@@ -28,16 +28,6 @@ __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
 }
 __device__ __forceinline__ float no_infinity(float x) { return fabsf(x) == INFINITY ? __uint_as_float(0x7fffffffu) : x; }
 
-// Whether all `n` scales are powers of two (positive and normal); all threads of the block take part.
-__device__ __forceinline__ bool all_powers(const float* scales, long long n) {
-  bool odd = false;
-  for (long long i = threadIdx.x; i < n; i += blockDim.x) {
-    const uint32_t b = __float_as_uint(scales[i]);
-    odd = odd || (b & 0x807fffffu) != 0 || b == 0 || b == 0x7f800000u;
-  }
-  return !__syncthreads_or(odd);
-}
-
 // ---- copies and clusters -----------------------------------------------------------------------------------------------
 // Rows of bytes, `ld` bytes apart, as [block][row][128]: a copy brings `kbs` blocks of `box_rows` rows as 128-byte swizzled tiles
 // one behind the other.  Where the rows are not whole blocks (`whole` false) the view is [1][row][width] and a copy brings one block

@@ -19,12 +19,6 @@ struct Output {
   GluEpilogue glu;
 };
 
-// gemm_fp8_many.cu: pe_gemm_fp8_many; with `unless_powers` only where some of the weights' scales are no powers of two.
-int gemm_many(bool unless_powers, const void* x, long long x_ld, const float* x_scales, long long xs_ld, const void* w, long long w_ld,
-              const float* w_scales, void* y, long long ldy, float* y_scales, long long ys_ld, int M, int N, int K, int out_f32, int kind,
-              float limit, float alpha, const float* bias, const float* row_weight, const int* offsets, int n_groups, int* status,
-              cudaStream_t stream);
-
 // 64 bytes of each of a warp's 32 rows (a row a lane) to rows `row_bytes` apart, of which `n` are there: through shared memory, so that
 // four lanes store a row (a lane that stored its own row touched 32 lines with each instruction).  Rows of `buf` are 80 bytes, so that
 // the 16-byte accesses of eight lanes to eight rows fall into different banks.

@@ -174,13 +174,14 @@ gemm_fp8_kernel(Params p, const __grid_constant__ CUtensorMap wmap, const __grid
       const uint32_t base = tma::smem_addr(smem);
       // Unrolled over the stages: an MMA's descriptors are registers that it reads when it starts, and a loop that writes the same
       // ones again waits for that (a stage of two blocks of 16 rows took 1,290 cycles, of which the MMAs are some 500).
-      for (int i0 = 0; i0 < n_st && !failed; i0 += STAGES) {
+      bool ok = true;
+      for (int i0 = 0; i0 < n_st && ok; i0 += STAGES) {
 #pragma unroll
         for (int stage = 0; stage < STAGES; ++stage) {
           const int i = i0 + stage, n = n_kb - i * KBS;
           if (n <= 0) break;
-          if ((i >= STAGES && !tma::mbar_wait(&read_bar[stage], ((i / STAGES) & 1) ^ 1)) ||
-              !tma::mbar_wait(&full_bar[stage], (i / STAGES) & 1)) {
+          ok = tma::mbar_wait_both(&read_bar[stage], ((i / STAGES) & 1) ^ 1, &full_bar[stage], (i / STAGES) & 1);
+          if (!ok) {
             report(p.status, kStatusWaitTimedOut, 71, tile, i);
             failed = 1;
             break;
@@ -514,22 +515,21 @@ extern "C" int pe_gemm_fp8_many_takes(int M, int N, int K, int kind, int n_group
   return 11 * ((tiles + pe::kSMs - 1) / pe::kSMs) * k_blocks <= 10LL * c.waves_blocks ? 1 : 0;
 }
 
-// Whether a product whose rows' scales are powers of two runs in pairs of SMs (gemm_fp8_pair.cu): where they take less.  A block of K
-// takes a pair 0.43 us for 256 x 256, and its launch 1.5 us more than the others'; weights whose scales have to be looked at (`known` 0)
-// 3 us again, and they fall back on tiles of 128 x 256 (us, other tiles : pairs; 4,096 x 6,144: 128 rows 15.4 : 17.3, 192 rows 21.9 : 17.3,
-// 1,024 rows 43.4 : 31.3; 12,288 x 4,096: 256 rows 33.0 : 43.4, 320 rows 55.6 : 43.0; 4,096 x 2 * 12,288 gated: 256 rows 48.6 : 36.9,
-// 320 rows 47.8 : 48.0, 2,048 rows 246 : 162).  Of groups half are taken to fill their last tile and half not to have it.
-extern "C" int pe_gemm_fp8_pair_takes(int M, int N, int K, int kind, int n_groups, int known) {
+// Whether a product whose scales are powers of two runs in pairs of SMs (gemm_fp8_pair.cu): where they take less.  A block of K takes a
+// pair 0.43 us for 256 x 256, and its launch 1.5 us more than the others' (us, other tiles : pairs; 4,096 x 6,144: 128 rows 15.4 : 17.3,
+// 192 rows 21.9 : 17.3, 1,024 rows 43.4 : 31.3; 12,288 x 4,096: 256 rows 33.0 : 43.4, 320 rows 55.6 : 43.0; 4,096 x 2 * 12,288 gated:
+// 256 rows 48.6 : 36.9, 320 rows 47.8 : 48.0, 2,048 rows 233 : 160).  Of groups half are taken to fill their last tile and half not to
+// have it.
+extern "C" int pe_gemm_fp8_pair_takes(int M, int N, int K, int kind, int n_groups) {
   if (N < 1 || K < 1 || M < 1 || M > pe::fp8::kMostRows || K > pe::fp8::kMostRows || (kind > 0 && N % 128)) return 0;
   if ((n_groups > 0 ? (M + n_groups - 1) / n_groups : M) <= 64) return 0;
   const int many = pe_gemm_fp8_many_takes(M, N, K, kind, n_groups);
-  if (!known && !many) return 0;
   const long long k_blocks = (K + pe::fp8::BK - 1) / pe::fp8::BK, n_tiles = kind > 0 ? N / 128 : (N + 255) / 256;
   const long long pairs = (((M + 255LL) / 256 + n_groups / 2) * n_tiles + pe::kSMs / 2 - 1) / (pe::kSMs / 2);
   const long long m_tiles = (M + 127LL) / 128 + n_groups / 2;
   const long long others = many ? 60 * ((m_tiles * n_tiles + pe::kSMs - 1) / pe::kSMs) * k_blocks
                                 : 55 * pe::fp8::cut_of((int)(m_tiles * 128), N, (int)k_blocks, 0, 128, kind > 0).waves_blocks;
-  return 43 * pairs * k_blocks + (known ? 150 : 450) <= others ? 1 : 0;
+  return 43 * pairs * k_blocks + 150 <= others ? 1 : 0;
 }
 
 // Whether bfloat16 rows are quantised inside the product: up to 16 rows (of an average group).

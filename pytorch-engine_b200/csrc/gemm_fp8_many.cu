@@ -38,9 +38,9 @@ constexpr size_t kSmem = 1024 + (size_t)STAGES * kStage + 8 * kOutWarp;
 
 struct Params {
   int M, N, K, k_blocks;                // N: output columns
-  bool whole, unless_powers;
+  bool whole;
   const float* xs; long long xs_ld;
-  const float* ws; long long ws_group, ws_all;  // per group [ceil(w rows / 128)][k_blocks]; of all groups
+  const float* ws; long long ws_group;  // per group [ceil(w rows / 128)][k_blocks]
   const int* offsets; int n_groups;     // null, 0: one group of M rows
   int m_tiles, n_tiles;                 // m_tiles: without groups
   Output out;
@@ -62,11 +62,6 @@ gemm_fp8_many_kernel(Params p, const __grid_constant__ CUtensorMap amap, const _
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int kPerTile = GLU ? BN / 2 : BN;     // outputs of a row in a tile
 
-  if (p.unless_powers && all_powers(p.ws, p.ws_all)) {     // gemm_fp8_pair.cu's kernel, launched before this one, has done it
-    pdl_wait_block();
-    pdl_launch_dependents();
-    return;
-  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       tma::mbar_init(&full_bar[s], 2);    // the two producers
@@ -259,12 +254,15 @@ static int launch_mode(const Params& p, const CUtensorMap& amap, const CUtensorM
 }
 
 }  // namespace fp8many
+}  // namespace pe
 
-int fp8::gemm_many(bool unless_powers, const void* x, long long x_ld, const float* x_scales, long long xs_ld, const void* w, long long w_ld,
-                   const float* w_scales, void* y, long long ldy, float* y_scales, long long ys_ld, int M, int N, int K, int out_f32,
-                   int kind, float limit, float alpha, const float* bias, const float* row_weight, const int* offsets, int n_groups,
-                   int* status, cudaStream_t stream) {
-  using namespace fp8many;
+// The arguments of pe_gemm_fp8 (gemm_fp8.cu); with an activation N is a multiple of 128.  y_scales (or null): the outputs are
+// quantised again, y is e4m3 (ldy bytes between rows, a multiple of 16) and y_scales[b * ys_ld + m] their blocks' scales.
+extern "C" int pe_gemm_fp8_many(const void* x, long long x_ld, const float* x_scales, long long xs_ld, const void* w, long long w_ld,
+                                const float* w_scales, void* y, long long ldy, float* y_scales, long long ys_ld, int M, int N, int K,
+                                int out_f32, int kind, float limit, float alpha, const float* bias, const float* row_weight,
+                                const int* offsets, int n_groups, int* status, cudaStream_t stream) {
+  using namespace pe::fp8many;
   if (M < 0 || N < 0 || K < 1 || kind < 0 || kind > 3 || n_groups < 0) return PE_ERR_BAD_ARGUMENT;
   if (M == 0 || N == 0) return PE_OK;
   if (M > kMostRows || K > kMostRows) return PE_ERR_UNSUPPORTED_SIZE;
@@ -280,8 +278,6 @@ int fp8::gemm_many(bool unless_powers, const void* x, long long x_ld, const floa
   p.xs = x_scales; p.xs_ld = xs_ld; p.ws = w_scales;
   const int w_rows = kind > 0 ? 2 * N : N;
   p.ws_group = (long long)((w_rows + 127) / 128) * p.k_blocks;
-  p.ws_all = p.ws_group * (n_groups > 0 ? n_groups : 1);
-  p.unless_powers = unless_powers;
   p.offsets = offsets; p.n_groups = n_groups;
   p.m_tiles = (M + BM - 1) / BM;
   p.n_tiles = kind > 0 ? N / (BN / 2) : (N + BN - 1) / BN;
@@ -294,16 +290,4 @@ int fp8::gemm_many(bool unless_powers, const void* x, long long x_ld, const floa
   if (e != 0) return e;
   if (kind == 0) return out_f32 ? launch_mode<kF32>(p, amap, bmap, stream) : launch_mode<kBf16>(p, amap, bmap, stream);
   return y_scales ? launch_mode<kGluFp8>(p, amap, bmap, stream) : launch_mode<kGlu>(p, amap, bmap, stream);
-}
-
-}  // namespace pe
-
-// The arguments of pe_gemm_fp8 (gemm_fp8.cu); with an activation N is a multiple of 128.  y_scales (or null): the outputs are
-// quantised again, y is e4m3 (ldy bytes between rows, a multiple of 16) and y_scales[b * ys_ld + m] their blocks' scales.
-extern "C" int pe_gemm_fp8_many(const void* x, long long x_ld, const float* x_scales, long long xs_ld, const void* w, long long w_ld,
-                                const float* w_scales, void* y, long long ldy, float* y_scales, long long ys_ld, int M, int N, int K,
-                                int out_f32, int kind, float limit, float alpha, const float* bias, const float* row_weight,
-                                const int* offsets, int n_groups, int* status, cudaStream_t stream) {
-  return pe::fp8::gemm_many(false, x, x_ld, x_scales, xs_ld, w, w_ld, w_scales, y, ldy, y_scales, ys_ld, M, N, K, out_f32, kind, limit, alpha,
-                            bias, row_weight, offsets, n_groups, status, stream);
 }

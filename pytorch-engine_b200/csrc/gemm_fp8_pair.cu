@@ -14,9 +14,6 @@
 // A tile's sums take half of tensor memory, and with scales there is no room for two: the epilogue's eight warps fetch all of it into
 // registers and hand it back before they convert or store anything.
 //
-// Weights whose scales are not known to be powers of two are looked over first, before the kernel waits for its predecessor; if one is
-// not, nothing is done here and gemm_fp8_many.cu's kernel, launched behind this one, does it.
-//
 // Roles: warps 0 and 1 copy x and the weights, warp 2 allocates tensor memory and (in the pair's first block) issues the MMAs, warp 3
 // prepares scales, warps 4 to 11 are the epilogue.  Every wait is bounded; one that runs out records kStatusWaitTimedOut, every role
 // leaves its loop, what is in flight is waited for (bounded again) and tensor memory is freed.
@@ -43,9 +40,9 @@ static_assert(kChunk % KBS == 0, "a stage's scales are of one chunk");
 
 struct Params {
   int M, K, k_blocks;
-  bool whole, check;                    // check: the weights' scales may be any
+  bool whole;
   const float* xs; long long xs_ld;
-  const float* ws; long long ws_group, ws_all;   // of a group, of all
+  const float* ws; long long ws_group;  // per group [ceil(w rows / 128)][k_blocks]
   int w_rows;
   const int* offsets; int n_groups;     // null, 0: one group of M rows
   int m_tiles, n_tiles;                 // m_tiles: without groups
@@ -127,11 +124,6 @@ gemm_fp8_pair_kernel(Params p, const __grid_constant__ CUtensorMap amap, const _
   const bool leader = rank == 0;
   constexpr int kPerTile = GLU ? BN / 2 : BN;     // outputs of a row in a tile
 
-  if (p.check && !all_powers(p.ws, p.ws_all)) {
-    pdl_wait_block();
-    pdl_launch_dependents();
-    return;                             // both blocks of the pair, and all pairs: nothing has been set up
-  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       tma::mbar_init(&full_bar[s], 2);    // the leader's: its producer, bytes of both blocks, and its scales
@@ -401,12 +393,11 @@ static int launch_mode(const Params& p, const CUtensorMap& amap, const CUtensorM
 }  // namespace fp8pair
 }  // namespace pe
 
-// The arguments of pe_gemm_fp8_many; the rows' scales are powers of two.  `check`: whether the weights' are is not known; where they
-// are not, gemm_fp8_many.cu's kernel computes the product.
+// The arguments of pe_gemm_fp8_many; all scales are powers of two (of others the exponent is taken).
 extern "C" int pe_gemm_fp8_pair(const void* x, long long x_ld, const float* x_scales, long long xs_ld, const void* w, long long w_ld,
                                 const float* w_scales, void* y, long long ldy, float* y_scales, long long ys_ld, int M, int N, int K,
                                 int out_f32, int kind, float limit, float alpha, const float* bias, const float* row_weight,
-                                const int* offsets, int n_groups, int check, int* status, cudaStream_t stream) {
+                                const int* offsets, int n_groups, int* status, cudaStream_t stream) {
   using namespace pe::fp8pair;
   if (M < 0 || N < 0 || K < 1 || kind < 0 || kind > 3 || n_groups < 0) return PE_ERR_BAD_ARGUMENT;
   if (M == 0 || N == 0) return PE_OK;
@@ -420,11 +411,10 @@ extern "C" int pe_gemm_fp8_pair(const void* x, long long x_ld, const float* x_sc
   const int groups = n_groups > 0 ? n_groups : 1;
   if ((kind > 0 && N % 128) || N > (1 << 28) || (long long)groups * N > (1 << 29)) return PE_ERR_UNSUPPORTED_SIZE;
   Params p;
-  p.M = M; p.K = K; p.k_blocks = (K + BK - 1) / BK; p.whole = K % BK == 0; p.check = check != 0;
+  p.M = M; p.K = K; p.k_blocks = (K + BK - 1) / BK; p.whole = K % BK == 0;
   p.xs = x_scales; p.xs_ld = xs_ld; p.ws = w_scales;
   p.w_rows = kind > 0 ? 2 * N : N;
   p.ws_group = (long long)((p.w_rows + 127) / 128) * p.k_blocks;
-  p.ws_all = p.ws_group * groups;
   p.offsets = offsets; p.n_groups = n_groups;
   p.m_tiles = (M + 2 * BM - 1) / (2 * BM);
   p.n_tiles = kind > 0 ? N / (BN / 2) : (N + BN - 1) / BN;
@@ -436,9 +426,6 @@ extern "C" int pe_gemm_fp8_pair(const void* x, long long x_ld, const float* x_sc
   if (e == 0) e = make_weight_map(&bmap, w, K, p.w_rows, w_ld, false, groups, BM, p.whole, KBS);
   if (e != 0) return e;
 #define PE_PAIR(MODE) (n_groups > 0 ? launch_mode<MODE, true>(p, amap, bmap, stream) : launch_mode<MODE, false>(p, amap, bmap, stream))
-  e = kind == 0 ? (out_f32 ? PE_PAIR(kF32) : PE_PAIR(kBf16)) : y_scales ? PE_PAIR(kGluFp8) : PE_PAIR(kGlu);
+  return kind == 0 ? (out_f32 ? PE_PAIR(kF32) : PE_PAIR(kBf16)) : y_scales ? PE_PAIR(kGluFp8) : PE_PAIR(kGlu);
 #undef PE_PAIR
-  if (e != PE_OK || !check) return e;
-  return gemm_many(true, x, x_ld, x_scales, xs_ld, w, w_ld, w_scales, y, ldy, y_scales, ys_ld, M, N, K, out_f32, kind, limit, alpha, bias,
-                   row_weight, offsets, n_groups, status, stream);
 }

@@ -141,8 +141,8 @@ _SIGNATURES = {
     "pe_rmsnorm_residual_fp8": [P, P, P, P, L, P, L, I, I, F, P],
     "pe_gemm_fp8": [P, L, P, L, P, L, P, P, L, I, I, I, I, I, F, F, P, P, P, I, P, P],
     "pe_gemm_fp8_many_takes": [I, I, I, I, I],
-    "pe_gemm_fp8_pair_takes": [I, I, I, I, I, I],
-    "pe_gemm_fp8_pair": [P, L, P, L, P, L, P, P, L, P, L, I, I, I, I, I, F, F, P, P, P, I, I, P, P],
+    "pe_gemm_fp8_pair_takes": [I, I, I, I, I],
+    "pe_gemm_fp8_pair": [P, L, P, L, P, L, P, P, L, P, L, I, I, I, I, I, F, F, P, P, P, I, P, P],
     "pe_gemm_fp8_many": [P, L, P, L, P, L, P, P, L, P, L, I, I, I, I, I, F, F, P, P, P, I, P, P],
     "pe_linear_fp8": [I, P, L, P, I, P, P, L, P, P, L, I, I, I, I, I, F, F, P, P, P, I, P, P],
     "pe_latent_prepare": [I, P, L, P, L, I, I, I, I, P, F, P, P, I, I, I, P, P, P, P, I, I, P, P, P, I, P, P],

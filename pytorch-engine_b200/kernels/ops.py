@@ -1647,23 +1647,22 @@ def _fp8_product(what: str, m: int, k: int, w, w_scales, out, glu, offsets, row_
     return n, w_ld, groups, (0, 0.0, 1.0, None) if glu is None else _glu_args(glu or None, n)
 
 
-def fp8_pair_takes(rows: int, width: int, k: int, glu, groups: int, powers) -> bool:
-    """Whether a product of rows whose scales are powers of two runs on pairs of SMs (csrc/gemm_fp8_pair.cu).  ``powers``: whether the
-    weight's scales are (None: not known)."""
-    return rows > 64 and powers is not False and bool(library().pe_gemm_fp8_pair_takes(rows, width, k, 0 if glu is None else 1, groups, 0 if powers is None else 1))
+def fp8_pair_takes(rows: int, width: int, k: int, glu, groups: int) -> bool:
+    """Whether a product whose scales are all powers of two runs on pairs of SMs (csrc/gemm_fp8_pair.cu)."""
+    return rows > 64 and bool(library().pe_gemm_fp8_pair_takes(rows, width, k, 0 if glu is None else 1, groups))
 
 
-def _gemm_fp8(what: str, x, x_scales, w, w_scales, out, status, glu, offsets, row_weight, row_powers, powers) -> None:
+def _gemm_fp8(what: str, x, x_scales, w, w_scales, out, status, glu, offsets, row_weight, powers) -> None:
     m, k = x.shape
     n, w_ld, groups, act = _fp8_product(what, m, k, w, w_scales, out, glu, offsets, row_weight, x, x_scales, status)
     x_ld, xs_ld = _fp8_ld(x, what), _fp8_scales_ld(x_scales, fp8_blocks(k), m, what)
     if m == 0 or n == 0:
         return
-    if row_powers and m > 64 and (row_weight is None or groups) and fp8_pair_takes(m, n, k, glu, groups, powers):
+    if powers and m > 64 and (row_weight is None or groups) and fp8_pair_takes(m, n, k, glu, groups):
         check(library().pe_gemm_fp8_pair(x.data_ptr(), x_ld, x_scales.data_ptr(), xs_ld, w.data_ptr(), w_ld, w_scales.data_ptr(), out.data_ptr(),
                                          out.stride(0), None, 0, m, n, k, 1 if out.dtype == torch.float32 else 0, *act, _ptr(row_weight),
-                                         _ptr(offsets), groups, 1 if powers is None else 0, status.data_ptr(), _stream()), what)
-        _count(2 if powers is None else 1)
+                                         _ptr(offsets), groups, status.data_ptr(), _stream()), what)
+        _count(1)
         return
     check(library().pe_gemm_fp8(x.data_ptr(), x_ld, x_scales.data_ptr(), xs_ld, w.data_ptr(), w_ld, w_scales.data_ptr(), out.data_ptr(),
                                 out.stride(0) if m > 1 else n, m, n, k, 1 if out.dtype == torch.float32 else 0, *act,
@@ -1673,7 +1672,7 @@ def _gemm_fp8(what: str, x, x_scales, w, w_scales, out, status, glu, offsets, ro
 
 
 def gemm_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor,
-             status: torch.Tensor, glu=None, row_powers: bool = False, powers: Optional[bool] = None) -> None:
+             status: torch.Tensor, glu=None, powers: bool = False) -> None:
     """``out[m, n] = sum_b x_scales[b, m] * w_scales[n // 128, b] * sum_{k in block b} x[m, k] w[n, k]`` of e4m3 ``x [M, K]`` and
     ``w [N, K]`` (csrc/gemm_fp8.cu), summed in float32; ``out`` bfloat16 or float32.  Rows of ``x`` and ``w`` lie a multiple of 16
     bytes apart and start on such boundaries.
@@ -1681,29 +1680,29 @@ def gemm_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales:
     ``glu``: ``w`` holds gate rows, then as many up rows (``out [M, N / 2]``, bfloat16), and ``out = act(gate, up)``; ``()`` is SiLU,
     else (kind of ``GLU_KINDS``, limit, alpha, float32 bias ``[N]`` or None).
 
-    ``row_powers``: the caller knows that ``x_scales`` are powers of two, as this module's conversions make them; many rows are then
-    faster where ``w_scales`` are too (``powers``: None if that is not known).  The sums of K are taken in another order there.
+    ``powers``: the caller knows that all scales are powers of two, as this module's conversions make them.  Many rows are then up to
+    1.5 times as fast (csrc/gemm_fp8_pair.cu); the sums of K are taken in another order there.
 
     ``w`` is a weight: the kernel starts to read it while the one launched before it is still running, so that one must
     not be what writes it (``quantize_weight_fp8`` may be: it lets nothing start early)."""
-    _gemm_fp8("gemm_fp8", x, x_scales, w, w_scales, out, status, glu, None, None, row_powers, powers)
+    _gemm_fp8("gemm_fp8", x, x_scales, w, w_scales, out, status, glu, None, None, powers)
 
 
 def moe_rows_gemm_fp8(x: torch.Tensor, x_scales: torch.Tensor, offsets: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor,
                       out: torch.Tensor, status: torch.Tensor, glu=None, row_weight: Optional[torch.Tensor] = None,
-                      row_powers: bool = False, powers: Optional[bool] = None) -> None:
+                      powers: bool = False) -> None:
     """``gemm_fp8`` for rows grouped by expert: rows ``offsets[g] .. offsets[g + 1]`` (int32, on the device) go through ``w[g]`` of ``w
     [groups, N, K]``, ``w_scales [groups, blocks, blocks]``.  Rows from ``offsets[groups]`` on are left as they are.  ``row_weight``
     (float32, one per row) multiplies both sums of an output before its activation."""
-    _gemm_fp8("moe_rows_gemm_fp8", x, x_scales, w, w_scales, out, status, glu, offsets, row_weight, row_powers, powers)
+    _gemm_fp8("moe_rows_gemm_fp8", x, x_scales, w, w_scales, out, status, glu, offsets, row_weight, powers)
 
 
 def linear_fp8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor, status: torch.Tensor, glu=None,
                offsets: Optional[torch.Tensor] = None, row_weight: Optional[torch.Tensor] = None,
-               row_map: Optional[torch.Tensor] = None, powers: Optional[bool] = None) -> None:
+               row_map: Optional[torch.Tensor] = None, powers: bool = False) -> None:
     """``quantize_rows_fp8`` of ``x`` (bfloat16 or float32, ``row_map`` as there), then ``gemm_fp8``, or with ``offsets``
     ``moe_rows_gemm_fp8``.  A handful of bfloat16 rows are quantised inside the product
-    (``FP8_INSIDE_ROWS``).  ``powers``: as there."""
+    (``FP8_INSIDE_ROWS``).  ``powers``: the scales of ``w`` are powers of two (see ``gemm_fp8``)."""
     if x.dim() != 2:
         raise KernelError("linear_fp8: x must be a matrix")
     src_rows, k = x.shape
@@ -1719,9 +1718,9 @@ def linear_fp8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: to
     n, w_ld, groups, act = _fp8_product("linear_fp8", m, k, w, w_scales, out, glu, offsets, row_weight, x, status, row_map)
     if m == 0 or n == 0:
         return
-    if m > 64 and (row_weight is None or groups) and fp8_pair_takes(m, n, k, glu, groups, powers):
+    if powers and m > 64 and (row_weight is None or groups) and fp8_pair_takes(m, n, k, glu, groups):
         values, scales = new_rows_fp8(x, row_map, None if offsets is None else offsets[-1:], status)
-        _gemm_fp8("linear_fp8", values, scales, w, w_scales, out, status, glu, offsets, row_weight, True, powers)
+        _gemm_fp8("linear_fp8", values, scales, w, w_scales, out, status, glu, offsets, row_weight, True)
         return
     px, scratch = x.data_ptr(), None
     raw = (m <= FP8_INSIDE_ROWS * (groups or 1) and w.numel() <= FP8_INSIDE_BYTES and row_map is None and x.dtype is torch.bfloat16
@@ -1736,14 +1735,14 @@ def linear_fp8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: to
     _count(1 if raw else 2)
 
 
-def gemm_fp8_gated_supported(rows: int, width: int, k: int, groups: int = 0, row_powers: bool = False, powers: Optional[bool] = None) -> bool:
+def gemm_fp8_gated_supported(rows: int, width: int, k: int, groups: int = 0, powers: bool = False) -> bool:
     """Whether ``gemm_fp8_gated`` takes a product of so many rows and ``width`` gates (many rows, a multiple of 128 gates)."""
-    return bool(library().pe_gemm_fp8_many_takes(rows, width, k, 1, groups)) or (row_powers and fp8_pair_takes(rows, width, k, (), groups, powers))
+    return bool(library().pe_gemm_fp8_many_takes(rows, width, k, 1, groups)) or (powers and fp8_pair_takes(rows, width, k, (), groups))
 
 
 def gemm_fp8_gated(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, values: torch.Tensor,
                    scales: torch.Tensor, status: torch.Tensor, glu=(), offsets: Optional[torch.Tensor] = None,
-                   row_weight: Optional[torch.Tensor] = None, row_powers: bool = False, powers: Optional[bool] = None) -> None:
+                   row_weight: Optional[torch.Tensor] = None, powers: bool = False) -> None:
     """``gemm_fp8`` (with ``offsets`` ``moe_rows_gemm_fp8``) with an activation whose outputs, rounded to bfloat16, are quantised on the
     way out (csrc/gemm_fp8_many.cu): e4m3 ``values [M, N]`` and ``scales [fp8_blocks(N), M]``, the bits that ``quantize_rows_fp8`` of
     the other's output gives."""
@@ -1756,7 +1755,7 @@ def gemm_fp8_gated(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_s
               and (groups == 1 or w.stride(0) == w.shape[1] * w.stride(1)), f"{what}: w [groups, 2 N, K] one behind the other, offsets int32, one more")
     _need(values.dim() == 2 and values.shape[0] == m and w.dim() == (2 if offsets is None else 3) and tuple(w.shape[-2:]) == (2 * n, k)
           and w.dtype == FP8, f"{what}: shapes do not match")
-    _need(gemm_fp8_gated_supported(m, n, k, groups, row_powers, powers) or m == 0, f"{what}: not for {m} rows and {n} gates")
+    _need(gemm_fp8_gated_supported(m, n, k, groups, powers) or m == 0, f"{what}: not for {m} rows and {n} gates")
     _need(w.stride(-1) == 1 and w.stride(-2) % 16 == 0, f"{what}: rows of w must be neighbouring values, a multiple of 16 bytes apart")
     _need(w_scales.dtype == torch.float32 and w_scales.is_contiguous() and tuple(w_scales.shape) == (*w.shape[:-2], fp8_blocks(2 * n), fp8_blocks(k)),
           f"{what}: scales of w")
@@ -1770,9 +1769,6 @@ def gemm_fp8_gated(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_s
     kind, limit, alpha, bias = _glu_args(glu or None, n)
     args = (x.data_ptr(), x_ld, x_scales.data_ptr(), xs_ld, w.data_ptr(), w.stride(-2), w_scales.data_ptr(), values.data_ptr(), y_ld,
             scales.data_ptr(), ys_ld, m, n, k, 0, kind, limit, alpha, bias, _ptr(row_weight), _ptr(offsets), groups)
-    if row_powers and fp8_pair_takes(m, n, k, glu, groups, powers):
-        check(library().pe_gemm_fp8_pair(*args, 1 if powers is None else 0, status.data_ptr(), _stream()), what)
-        _count(2 if powers is None else 1)
-    else:
-        check(library().pe_gemm_fp8_many(*args, status.data_ptr(), _stream()), what)
-        _count(1)
+    run = library().pe_gemm_fp8_pair if powers and fp8_pair_takes(m, n, k, glu, groups) else library().pe_gemm_fp8_many
+    check(run(*args, status.data_ptr(), _stream()), what)
+    _count(1)

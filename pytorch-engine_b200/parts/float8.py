@@ -71,7 +71,7 @@ def _all_powers(weights) -> Optional[bool]:
 class Float8Weight:
     """``values [N, K]`` (e4m3) and ``scales [fp8_blocks(N), fp8_blocks(K)]`` (float32); or several such matrices stacked in
     front, ``[G, N, K]`` and ``[G, ...]``.  Rows start on 16-byte boundaries (``to`` makes it so).  ``powers``: whether all scales are
-    powers of two; None: not known (a product of many rows then looks, ``to`` does it once)."""
+    powers of two, which makes products of many rows faster; None: not known (``to`` finds out)."""
 
     __slots__ = ("values", "scales", "powers")
     dtype = FP8

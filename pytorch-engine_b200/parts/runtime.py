@@ -301,11 +301,11 @@ class Runtime:
 
     def _float8_product(self, x, weight: Float8Weight, out: torch.Tensor, glu=None, offsets=None, row_weight=None, row_map=None) -> torch.Tensor:
         if type(x) is not Float8Rows:
-            ops.linear_fp8(x, weight.values, weight.scales, out, self.status, glu, offsets, row_weight, row_map, weight.powers)
+            ops.linear_fp8(x, weight.values, weight.scales, out, self.status, glu, offsets, row_weight, row_map, bool(weight.powers))
         elif offsets is None:
-            ops.gemm_fp8(x.values, x.scales, weight.values, weight.scales, out, self.status, glu, x.powers, weight.powers)
+            ops.gemm_fp8(x.values, x.scales, weight.values, weight.scales, out, self.status, glu, bool(x.powers and weight.powers))
         else:
-            ops.moe_rows_gemm_fp8(x.values, x.scales, offsets, weight.values, weight.scales, out, self.status, glu, row_weight, x.powers, weight.powers)
+            ops.moe_rows_gemm_fp8(x.values, x.scales, offsets, weight.values, weight.scales, out, self.status, glu, row_weight, bool(x.powers and weight.powers))
         return out
 
     def float8_feed_forward(self, x, gate_up: Float8Weight, down: Float8Weight, out: torch.Tensor, glu=None) -> torch.Tensor:
@@ -315,13 +315,13 @@ class Runtime:
         if not self.is_cuda:
             raise KernelError("this package computes on a CUDA device only; there is no CPU path")
         m, (hidden, inter) = x.shape[0], down.shape
-        row_powers = type(x) is not Float8Rows or x.powers
-        if m > 64 and ops.gemm_fp8_gated_supported(m, inter, hidden, 0, row_powers, gate_up.powers):
+        powers = bool(gate_up.powers and (type(x) is not Float8Rows or x.powers))
+        if m > 64 and ops.gemm_fp8_gated_supported(m, inter, hidden, 0, powers):
             # many rows: the activation leaves the product's epilogue quantised
             rows = x if type(x) is Float8Rows else Float8Rows.quantize(x)
             act = Float8Rows.empty(m, inter, x.device)
             ops.gemm_fp8_gated(rows.values, rows.scales, gate_up.values, gate_up.scales, act.values, act.scales, self.status, glu or (),
-                               row_powers=row_powers, powers=gate_up.powers)
+                               powers=powers)
         else:
             act = torch.empty((m, inter), dtype=torch.bfloat16, device=x.device)
             self._float8_product(x, gate_up, act, glu or ())
@@ -338,12 +338,12 @@ class Runtime:
             raise KernelError("rows taken from others are given in bfloat16 or float32, not quantised already")
         groups, hidden, inter = down.shape
         m = out.shape[0]
-        row_powers = type(x) is not Float8Rows or x.powers
-        if m > 64 * groups and ops.gemm_fp8_gated_supported(m, inter, hidden, groups, row_powers, gate_up.powers):
+        powers = bool(gate_up.powers and (type(x) is not Float8Rows or x.powers))
+        if m > 64 * groups and ops.gemm_fp8_gated_supported(m, inter, hidden, groups, powers):
             rows = x if type(x) is Float8Rows else Float8Rows.quantize(x, row_token, offsets[-1:], self.status)
             act = Float8Rows.empty(m, inter, x.device)
             ops.gemm_fp8_gated(rows.values, rows.scales, gate_up.values, gate_up.scales, act.values, act.scales, self.status, glu or (), offsets,
-                               row_weight, row_powers, gate_up.powers)
+                               row_weight, powers)
         else:
             act = torch.empty((m, inter), dtype=torch.bfloat16, device=x.device)
             self._float8_product(x, gate_up, act, glu or (), offsets, row_weight, row_token)

@@ -285,7 +285,7 @@ extern "C" int pe_rmsnorm_residual_fp8(float* residual, const void* delta, const
   int threads = dim >= 2048 ? 512 : (dim >= 512 ? 256 : 128);
   if (n_rows <= 64 && dim > 2048) threads = 1024;
   cudaError_t e;
-  if (smem > 48 * 1024) {
+  if (smem > 47 * 1024) {              // with the static part beyond the 48 KB that need no asking
     e = cudaFuncSetAttribute(rmsnorm_residual_fp8_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return (int)e;
   }

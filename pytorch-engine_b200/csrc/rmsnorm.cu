@@ -379,7 +379,7 @@ __global__ void __launch_bounds__(1024) rmsnorm_of_sum_vec4_kernel(float* __rest
 
 template <typename K>
 static int set_smem(K kernel, size_t bytes) {
-  if (bytes > 48 * 1024) {
+  if (bytes > 47 * 1024) {             // with the kernels' static part beyond the 48 KB that need no asking
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
     if (e != cudaSuccess) return (int)e;
   }

@@ -225,6 +225,24 @@ def test_norm(ops, f8, n, dim, delta):
     assert torch.equal(r.values.to(F32), want.values.to(F32)) and torch.equal(r.scales, want.scales)
 
 
+@pytest.mark.parametrize("n,dim", [(2, 12032), (3, 12256), (3, 12260), (70, 12288), (2, 12292), (1, 51200)])
+def test_norm_wide(ops, f8, n, dim):
+    """Rows about as wide as the shared memory that a kernel may have without asking, and the widest."""
+    g = torch.Generator(device=DEV).manual_seed(n)
+    stream, w = torch.randn(n, dim, generator=g, device=DEV) * 3, torch.randn(dim, generator=g, device=DEV)
+    d = torch.randn(n, dim, generator=g, device=DEV).to(BF16)
+    two, out = stream.clone(), torch.empty(n, dim, dtype=BF16, device=DEV)
+    ops.rmsnorm_residual(two, d, w, out, 1e-6)
+    want, r = f8.Float8Rows.quantize(out), f8.Float8Rows.empty(n, dim, DEV)
+    ops.rmsnorm_residual_fp8(stream, d, w, r.values, r.scales, 1e-6)
+    assert torch.equal(stream, two)
+    assert torch.equal(r.values.to(F32), want.values.to(F32)) and torch.equal(r.scales, want.scales)
+    x64 = two.to(F64)
+    y64 = x64 * torch.rsqrt((x64 * x64).mean(1, keepdim=True) + 1e-6) * w.to(F64)
+    # sums of squares: dim terms; the root, two products: 4 roundings; then bfloat16
+    assert_within(out, y64, ((dim + 8) * 2.0 ** -24 + 2.0 ** -8) * y64.abs())
+
+
 # ---- products --------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("out_dtype", [F32, BF16])
 @pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 128, 128), (3, 129, 130), (16, 300, 1040), (17, 64, 2000), (33, 1111, 384),

@@ -156,7 +156,9 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) quantize_weight_k
 }
 
 // rmsnorm.cu's norm (with its residual add) whose result, rounded to bfloat16, is quantised on the way out: what rmsnorm.cu's
-// kernel and the one above would give, without the bfloat16 rows between them.  A warp's 32 x 4 features are one block.
+// kernel and the one above would give, without the bfloat16 rows between them.  The sum of squares is taken in rmsnorm.cu's order, four
+// features a thread; the rest with eight a thread, for which the sixteen lanes of a block need a step less than 32 would (2,011 x 4,096:
+// 14.6 us, with four 16.1; asking for several of a thread's features at once made it 19).
 __global__ void __launch_bounds__(1024) rmsnorm_residual_fp8_kernel(float* residual, const __nv_bfloat16* delta,
                                                                     const float* __restrict__ weight, uint8_t* values,
                                                                     long long v_ld, float* scales, long long s_ld, int dim,
@@ -164,8 +166,11 @@ __global__ void __launch_bounds__(1024) rmsnorm_residual_fp8_kernel(float* resid
   extern __shared__ float row_buf[];  // dim floats
   __shared__ float red[32];
   const int c0 = threadIdx.x * 4;
-  float4 w0 = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (c0 < dim) w0 = *reinterpret_cast<const float4*>(weight + c0);   // the weight does not come from the kernel before this one
+  // the weight does not come from the kernel before this one
+  float4 w0[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if ((int)threadIdx.x * 8 + 4 * i < dim) w0[i] = *reinterpret_cast<const float4*>(weight + threadIdx.x * 8 + 4 * i);
   pdl_wait_block();
   pdl_launch_dependents();
   const int r = blockIdx.x;
@@ -185,23 +190,27 @@ __global__ void __launch_bounds__(1024) rmsnorm_residual_fp8_kernel(float* resid
     ss += h.x * h.x + h.y * h.y + h.z * h.z + h.w * h.w;
   }
   const float inv = rsqrtf(block_sum(ss, red) / (float)dim + eps);
-  // whole warps stay in the loop for the shuffles
-  for (int c = c0; c - (int)(threadIdx.x & 31) * 4 < dim; c += blockDim.x * 4) {
-    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (c < dim) {
-      const float4 h = *reinterpret_cast<const float4*>(row_buf + c);
-      const float4 w = c == c0 ? w0 : *reinterpret_cast<const float4*>(weight + c);
-      const float2 lo = __bfloat1622float2(__floats2bfloat162_rn(h.x * inv * w.x, h.y * inv * w.y));
-      const float2 hi = __bfloat1622float2(__floats2bfloat162_rn(h.z * inv * w.z, h.w * inv * w.w));
-      y = make_float4(lo.x, lo.y, hi.x, hi.y);
-    }
-    const float a = warp_max(fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))));
+  // from here on eight features a thread, sixteen lanes a block; whole warps stay in the loop for the shuffles
+  for (int c = threadIdx.x * 8; c - (int)(threadIdx.x & 31) * 8 < dim; c += blockDim.x * 8) {
+    uint32_t y[4] = {0, 0, 0, 0};         // bfloat16 pairs
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (c + 4 * i < dim) {
+        const float4 h = *reinterpret_cast<const float4*>(row_buf + c + 4 * i);
+        const float4 w = c == (int)threadIdx.x * 8 ? w0[i] : *reinterpret_cast<const float4*>(weight + c + 4 * i);
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(h.x * inv * w.x, h.y * inv * w.y), hi = __floats2bfloat162_rn(h.z * inv * w.z, h.w * inv * w.w);
+        y[2 * i] = *reinterpret_cast<const uint32_t*>(&lo);
+        y[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&hi);
+      }
+    Raw8<__nv_bfloat16> v;
+    v.v = make_uint4(y[0], y[1], y[2], y[3]);
+    float a = v.top();
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
     if (c >= dim) continue;
     const uint32_t s = scale_bits(a);
-    const float by = inverse_of(s);
-    if (a == INFINITY) y = make_float4(no_infinity(y.x), no_infinity(y.y), no_infinity(y.z), no_infinity(y.w));
-    *reinterpret_cast<uint32_t*>(values + (size_t)r * v_ld + c) = pack4(y.x * by, y.y * by, y.z * by, y.w * by);
-    if ((threadIdx.x & 31) == 0) scales[(size_t)(c / BLOCK) * s_ld + r] = __uint_as_float(s);
+    store8<__nv_bfloat16>(values + (size_t)r * v_ld, c, dim, v, s, a);
+    if ((threadIdx.x & 15) == 0) scales[(size_t)(c / BLOCK) * s_ld + r] = __uint_as_float(s);
   }
 }
 

@@ -116,7 +116,7 @@ gemm_fp8_pair_kernel(Params p, const __grid_constant__ CUtensorMap amap, const _
   __shared__ float top_s[2][BM];
   __shared__ uint32_t tmem_holder;
   __shared__ volatile int failed;
-  __shared__ int issued;
+  __shared__ int started, fed, issued;    // stages whose copies were started, whose scales were, whose MMAs were
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   char* scales_s = smem + STAGES * kStage;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -135,7 +135,7 @@ gemm_fp8_pair_kernel(Params p, const __grid_constant__ CUtensorMap amap, const _
     }
     tma::mbar_init(&acc_full, 1);         // a commit, delivered to both blocks
     tma::mbar_init(&acc_empty, 16);       // the leader's: the epilogue warps of both blocks
-    failed = issued = 0;
+    failed = started = fed = issued = 0;
     tma::fence_barrier_init();
   }
   if (warp == 2) tmem_alloc2(&tmem_holder, kTmemCols);
@@ -188,6 +188,7 @@ gemm_fp8_pair_kernel(Params p, const __grid_constant__ CUtensorMap amap, const _
       }
       ok = __all_sync(0xffffffffu, ok);
     }
+    if (lane == 0) started = g;
     if (!ok) {
       if (lane == 0) report(p.status, kStatusWaitTimedOut, 100, (int)blockIdx.x, g);
       failed = 1;
@@ -218,10 +219,12 @@ gemm_fp8_pair_kernel(Params p, const __grid_constant__ CUtensorMap amap, const _
           if (!ok) break;
           if (st * KBS % kChunk == 0) {
             commit_one(&full_bar[stage]);
+            fed = g + 1;
             if (++c < chunks) ok = copy_up(c);
             if (!ok) break;
           } else {
             tma::mbar_arrive(&full_bar[stage]);
+            fed = g + 1;
           }
         }
       }
@@ -349,8 +352,13 @@ gemm_fp8_pair_kernel(Params p, const __grid_constant__ CUtensorMap amap, const _
   __syncwarp();
   fence_before_sync();
   __syncthreads();
-  if (failed && leader && threadIdx.x == 64)
+  if (failed && leader && threadIdx.x == 64) {   // MMAs that still read both blocks' shared memory, copies still on their way to it
     for (int i = max(0, issued - STAGES); i < issued; ++i) tma::mbar_wait(&empty_bar[i % STAGES], (i / STAGES) & 1);
+    for (int i = max(0, started - STAGES); i < started; ++i) {
+      if (i >= fed) tma::mbar_arrive(&full_bar[i % STAGES]);
+      tma::mbar_wait(&full_bar[i % STAGES], (i / STAGES) & 1);
+    }
+  }
   __syncwarp();
   cluster_sync();
   if (warp == 2) {

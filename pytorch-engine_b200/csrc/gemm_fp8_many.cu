@@ -10,7 +10,8 @@
 //
 // What bounds it is the way round a half of tensor memory: MMAs, commit, eight warps that read it, their arrival, the next MMAs.
 // Two SMs on one tile (cta_group::2) load a third less but have that way lead through the other SM: 1,750 cycles a block and
-// half, one SM 1,050.
+// half, one SM 1,050.  (Where the scales are powers of two there is no way round: gemm_fp8_pair.cu.)  2,048 x 4,096 x 6,144 64 us,
+// 2,048 x 4,096 to 2 * 12,288 gated 233 us, 1.77 PFLOP/s.
 //
 // GLU: the tile's weight rows are 128 gates and the 128 ups that belong to them, a thread owns 64 of each, and act(gate, up),
 // rounded to bfloat16, goes out as it is or quantised again: the tile's 128 outputs of a row are one block, whose largest

@@ -8,14 +8,20 @@
 // SMs share a tile of 256 x 256 (cta_group::2), each with half of both operands in its shared memory.
 //
 // Scales lie in tensor memory too.  One warp turns the float32 scales of four k blocks into bytes, a word of them for each row of x
-// and for the two blocks of weight rows, as 32 lanes x 16 bytes for 128 rows; the issuing thread copies them up (tcgen05.cp) in front
-// of the MMAs that use them, byte i for the i-th of the four blocks.
+// and for the two blocks of weight rows, as 32 lanes x 16 bytes for 128 rows; tcgen05.cp copies them up in front of the MMAs that use
+// them, byte i for the i-th of the four blocks.
+//
+// What bounds it is the thread that issues the MMAs: a stage's eight run 1,024 cycles, and each load from shared memory takes that
+// thread some 200 while they do.  So it waits for one barrier a stage and commits once; scales have a thread of their own, which copies
+// them up and arrives for the stage.  (With waits for scales and the copies in the issuing thread: 1,330 cycles a stage, 2,048 x 4,096 x
+// 6,144 52 us; as it is 46.)  2,048 x 4,096 to 2 * 12,288 gated 160 us, 2.57 PFLOP/s, of which the power cap takes a part; in tiles of
+// 128 x 256 with a multiply-add an output and block 233.
 //
 // A tile's sums take half of tensor memory, and with scales there is no room for two: the epilogue's eight warps fetch all of it into
 // registers and hand it back before they convert or store anything.
 //
-// Roles: warps 0 and 1 copy x and the weights, warp 2 allocates tensor memory and (in the pair's first block) issues the MMAs, warp 3
-// prepares scales, warps 4 to 11 are the epilogue.  Every wait is bounded; one that runs out records kStatusWaitTimedOut, every role
+// Roles: warp 0 copies x and the weights, warp 1 (in the pair's first block) copies scales up, warp 2 allocates tensor memory and (in
+// the first block) issues the MMAs, warp 3 prepares scales, warps 4 to 11 are the epilogue.  Every wait is bounded; one that runs out records kStatusWaitTimedOut, every role
 // leaves its loop, what is in flight is waited for (bounded again) and tensor memory is freed.
 #include "api.h"
 #include "fp8_out.cuh"

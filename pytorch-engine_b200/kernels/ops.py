@@ -1596,8 +1596,8 @@ def rmsnorm_residual_fp8(residual: torch.Tensor, delta: Optional[torch.Tensor], 
 
 # Up to so many rows, and so many bytes of weights, a product quantises bfloat16 rows itself (csrc/gemm_fp8.cu, RAW): each of its
 # blocks converts all rows of its share of K, which hides behind few weights.  Inside : in front, us on the device: 1 row, 4,096 x
-# 6,144 weights 9.5 : 10.2; 8 rows, 4,096 x 4,096 8.5 : 9.2, 4,096 x 6,144 10.6 : 10.3 (and 5 us less for the host), 12,288 x 4,096
-# 15.2 : 13.9, 4,096 x 24,576 28.6 : 21.3; 16 rows, 4,096 x 6,144 11.9 : 10.5.
+# 6,144 weights 9.1 : 9.7; 8 rows, 4,096 x 4,096 8.5 : 8.9, 4,096 x 6,144 10.4 : 10.0 (and 5 us less for the host), 12,288 x 4,096
+# 15.0 : 13.6, 4,096 x 24,576 28.5 : 20.8; 16 rows, 4,096 x 6,144 11.9 : 10.3.
 FP8_INSIDE_ROWS, FP8_INSIDE_BYTES = 8, 32 << 20
 
 

@@ -769,3 +769,56 @@ def test_feed_forward_of_powers(pe, ops, f8, m, hidden, inter):
     want = r64 @ d64.t()
     assert_within(out, want, sum_error(r64, d64) + 2.0 ** -8 * want.abs())
     rt.raise_on_status()
+
+
+def test_more_than_two_to_the_31(ops, f8, status):
+    """Outputs, rows and values that pass 2^31 elements and 2^32 bytes, in every kernel that writes many of them."""
+    m, n, k = 66000, 33024, 128
+    x = rows_of(m, k, BF16, 1)
+    rows = f8.Float8Rows.quantize(x)
+    picks = torch.tensor([0, 1, 32767, 32768, 65071, m - 129, m - 128, m - 1], device=DEV)
+    x64 = wide_rows(f8.Float8Rows(rows.values[picks], rows.scales[:, picks].contiguous()))
+    out = torch.empty(m, n, dtype=BF16, device=DEV)
+    for w, powers in ((weight_of(f8, n, k, 1), False), (power_weight(f8, n, k, 1), True)):
+        out.fill_(3.0)
+        ops.gemm_fp8(rows.values, rows.scales, w.values, w.scales, out, status, powers=powers)
+        w64 = wide(w)
+        want = x64 @ w64.t()
+        assert_within(out[picks], want, sum_error(x64, w64) + 2.0 ** -8 * want.abs())
+    wide_row = f8.Float8Rows.quantize(out)              # [66000, 33024] again
+    again = f8.Float8Rows.quantize(out[picks])
+    assert torch.equal(wide_row.values[picks].to(F32), again.values.to(F32)) and torch.equal(wide_row.scales[:, picks], again.scales)
+    rest = m % 128                                       # the last block of rows
+    tall, last = f8.Float8Weight.quantize(out), f8.Float8Weight.quantize(out[-rest:])
+    assert torch.equal(tall.values[-rest:].to(F32), last.values.to(F32)) and torch.equal(tall.scales[-1:], last.scales)
+
+
+def test_pairs_on_two_streams(pe, f8):
+    """Pairs of SMs for two streams at once, beside products of few rows, and their graphs."""
+    from pytorch_engine_b200.parts.runtime import Runtime
+
+    rt, hidden, inter = Runtime(DEV, BF16), 1024, 2816
+    gate_up, down = power_weight(f8, 2 * inter, hidden, 1).to(DEV), power_weight(f8, hidden, inter, 2).to(DEV)
+    sizes = (1500, 7, 2100)
+    x = [rows_of(m, hidden, BF16, m) * 0.01 for m in sizes]
+    want = [torch.empty(m, hidden, dtype=BF16, device=DEV) for m in sizes]
+    for a, y in zip(x, want):
+        rt.float8_feed_forward(a, gate_up, down, y)
+    streams, out = [torch.cuda.Stream() for _ in sizes], [torch.zeros_like(y) for y in want]
+    graphs = []
+    torch.cuda.synchronize()
+    for s, a, y in zip(streams, x, out):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=s):
+            rt.float8_feed_forward(a, gate_up, down, y)
+    for i in range(20):
+        for s, a, y, g in zip(streams, x, out, graphs):
+            with torch.cuda.stream(s):
+                if i % 2:
+                    rt.float8_feed_forward(a, gate_up, down, y)
+                else:
+                    g.replay()
+    torch.cuda.synchronize()
+    for y, w in zip(out, want):
+        assert torch.equal(y, w)
+    rt.raise_on_status()

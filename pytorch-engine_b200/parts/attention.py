@@ -128,7 +128,7 @@ class GQAttention:
         if self.output_gate == "sigmoid_head":    # rows of the product stay 16-byte aligned
             rows = sum(t.shape[0] for t in fused)
             if rows % 8:
-                fused = [wide(t) for t in fused]
+                fused = [wide(t, runtime.dtype) for t in fused]
                 fused.append(torch.zeros((8 - rows % 8, self.hidden), dtype=fused[0].dtype, device=fused[0].device))
         self.qkv = projection(runtime, fused)
         self.o_proj = projection(runtime, [weights["o_proj"]])

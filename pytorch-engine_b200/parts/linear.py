@@ -15,8 +15,9 @@ def fuse_rows(runtime, tensors: Sequence[torch.Tensor]) -> torch.Tensor:
     return torch.cat(parts, dim=0).contiguous()
 
 
-def wide(tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """A weight as numbers of 16 or 32 bits: a checkpoint's 8-bit matrix times its scales, any other tensor as it is."""
+def wide(tensor, dtype: torch.dtype) -> torch.Tensor:
+    """A weight as numbers of 16 or 32 bits: a checkpoint's 8-bit matrix times its scales, in the run's ``dtype``; any other tensor
+    as it is."""
     return tensor.dequantize(dtype) if type(tensor) is Float8Weight else tensor
 
 
@@ -29,7 +30,7 @@ def projection(runtime, tensors: Sequence) -> Union[torch.Tensor, Float8Weight]:
         if all(stored) and Float8Weight.stacks_rows(tensors):
             return Float8Weight.cat_rows([t.to(runtime.device) for t in tensors]) if len(tensors) > 1 else tensors[0].to(runtime.device)
         if runtime.float8:
-            return Float8Weight.quantize(fuse_rows(runtime, [wide(t) for t in tensors]))
+            return Float8Weight.quantize(fuse_rows(runtime, [wide(t, runtime.dtype) for t in tensors]))
     if len(tensors) == 1 and not stored[0]:
         return runtime.adopt(tensors[0])
     return fuse_rows(runtime, [wide(t, runtime.dtype) for t in tensors])

@@ -15,7 +15,7 @@ import torch
 
 from ..kernels import ops
 from .float8 import Float8Weight
-from .linear import projection, wide
+from .linear import projection
 from .registry import register
 from .spec import CacheRequest, WeightDecl
 
@@ -125,12 +125,8 @@ class GQAttention:
         fused = [weights["q_proj"], weights["k_proj"], weights["v_proj"]]
         if self.output_gate:
             fused.append(weights["g_proj"])       # q | k | v | gate: one product over the mixer's input
-        if self.output_gate == "sigmoid_head":    # rows of the product stay 16-byte aligned
-            rows = sum(t.shape[0] for t in fused)
-            if rows % 8:
-                fused = [wide(t, runtime.dtype) for t in fused]
-                fused.append(torch.zeros((8 - rows % 8, self.hidden), dtype=fused[0].dtype, device=fused[0].device))
-        self.qkv = projection(runtime, fused)
+        # with a gate per head too, rows of the product stay 16-byte aligned
+        self.qkv = projection(runtime, fused, 8 if self.output_gate == "sigmoid_head" else 1)
         self.o_proj = projection(runtime, [weights["o_proj"]])
         self.q_norm = self.k_norm = None
         if params.get("qk_norm", False):

@@ -136,6 +136,18 @@ class Float8Weight:
             at += w.shape[0]
         return cls(values, torch.cat([w.scales for w in weights]).contiguous(), _all_powers(weights))
 
+    def with_zero_rows(self, rows: int) -> "Float8Weight":
+        """The matrix with so many rows of zeros behind its last one, in whose block they must still lie."""
+        if rows == 0:
+            return self
+        n, k = self.shape
+        if fp8_blocks(n + rows) != fp8_blocks(n):
+            raise ValueError(f"{rows} more rows do not fit the last block of an 8-bit weight {list(self.shape)}")
+        values = _padded_empty((n + rows, k), self.device)
+        values[:n].copy_(self.values)
+        values[n:].view(torch.uint8).zero_()
+        return Float8Weight(values, self.scales, self.powers)
+
     def to(self, device) -> "Float8Weight":
         """On ``device``, with rows on 16-byte boundaries, and ``powers`` known (for which the host waits for the device)."""
         values, scales = self.values, self.scales.to(device).contiguous()

@@ -81,3 +81,39 @@ def test_a_float32_model_holds_the_numbers(pe, arch, key):
         assert set(a) == set(b)
         for n in b:
             assert a[n].dtype == b[n].dtype and torch.equal(a[n], b[n]), n
+
+
+class OfWidth8:
+    """What ``projection`` asks of a runtime, with 8-bit products."""
+    device, dtype, float8 = torch.device("cpu"), BF16, False
+
+    def takes_float8(self):
+        return True
+
+
+@pytest.mark.parametrize("rows", [(256, 128, 128, 6), (256, 128, 128, 8), (128, 128, 128, 1), (128, 128, 121), (127,), (128, 125)])
+@pytest.mark.parametrize("k", [54, 144])
+def test_a_padded_projection_stays_in_8_bits(pe, rows, k):
+    """Stored matrices that end with a block of rows are put under each other as they are, with zeros behind the last."""
+    from pytorch_engine_b200.parts.linear import projection
+
+    f8 = pe.parts.float8
+    g = torch.Generator().manual_seed(sum(rows))
+    mats = [f8.Float8Weight(torch.randn(n, k, generator=g).mul(40).clamp(-448, 448).to(E4M3), torch.rand(blocks(n), blocks(k), generator=g)) for n in rows]
+    got = projection(OfWidth8(), mats, 8)
+    assert type(got) is f8.Float8Weight and got.shape == (-(-sum(rows) // 8) * 8, k)
+    assert torch.equal(got.dequantize()[:sum(rows)], torch.cat([m.dequantize() for m in mats]))
+    assert bool((got.dequantize()[sum(rows):] == 0).all()) and got.values.stride(0) % 16 == 0
+
+
+def test_rows_that_end_inside_a_block(pe):
+    """Then the matrices' numbers are used; and zeros are not put where they would begin a block."""
+    from pytorch_engine_b200.parts.linear import projection
+
+    f8 = pe.parts.float8
+    mats = [f8.Float8Weight(torch.ones(n, 40).to(E4M3), torch.full((blocks(n), 1), 0.3)) for n in (100, 30)]
+    got = projection(OfWidth8(), mats, 8)
+    assert got.dtype == BF16 and got.shape == (136, 40)
+    assert torch.equal(got[:130], torch.cat([m.dequantize(BF16) for m in mats])) and bool((got[130:] == 0).all())
+    with pytest.raises(ValueError):
+        f8.Float8Weight(torch.ones(128, 40).to(E4M3), torch.ones(1, 1)).with_zero_rows(1)

@@ -105,6 +105,17 @@ inline cudaError_t launch_after(void (*kernel)(KArgs...), dim3 grid, dim3 block,
   return launch_as(false, kernel, grid, block, smem, stream, args...);
 }
 
+// Dynamic shared memory for a kernel: what comes, with the kernel's own static arrays, to more than 48 KB has to be asked for.  The
+// kernels that call this have less than 1 KB of their own (512 bytes at the most).
+template <typename K>
+inline int allow_smem(K kernel, size_t bytes) {
+  if (bytes > 47 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e != cudaSuccess) return (int)e;
+  }
+  return 0;
+}
+
 // ---- element conversion ----------------------------------------------------------------------
 template <typename T> __device__ __forceinline__ float to_f32(T v);
 template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }

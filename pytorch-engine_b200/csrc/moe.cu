@@ -566,10 +566,8 @@ extern "C" int pe_moe_rows_gemm(int dtype, int out_dtype, const void* x, long lo
 #define PE_MOE_LAUNCH(T, TOut)                                                                                          \
   do {                                                                                                                  \
     auto kernel = pe::moe_rows_gemm_kernel<T, TOut>;                                                                     \
-    if (smem > 48 * 1024) {                                                                                             \
-      cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);             \
-      if (e != cudaSuccess) return (int)e;                                                                              \
-    }                                                                                                                   \
+    const int e = pe::allow_smem(kernel, smem);                                                                         \
+    if (e != 0) return e;                                                                                               \
     pe::launch(kernel, grid, dim3(256), smem, stream, (const T*)x, x_ld, row_map, offsets, n_groups, (const T*)w,       \
                w_group_stride, (TOut*)out, out_ld, n_out, k_dim, glu, limit, alpha, vec_ok, row_weight);                \
   } while (0)

@@ -243,10 +243,8 @@ static int launch_streams(const StreamArgs& a, cudaStream_t stream) {
                    al(a.out, a.norm ? 4 * sizeof(T) : 16);
   auto go = [&](auto kern, int threads, size_t smem) -> int {
     if (smem > 200 * 1024) return PE_ERR_UNSUPPORTED_SIZE;
-    if (smem > 48 * 1024) {
-      cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-      if (e != cudaSuccess) return (int)e;
-    }
+    const int e = allow_smem(kern, smem);
+    if (e != 0) return e;
     pe::launch(kern, a.n_rows, threads, smem, stream, a);
     PE_LAUNCH_CHECK();
     return PE_OK;
@@ -270,6 +268,15 @@ static int launch_streams(const StreamArgs& a, cudaStream_t stream) {
   return go(streams_any_kernel<T>, 256, row_bytes + (size_t)(a.s * a.s + 2 * a.s) * sizeof(float));
 }
 
+template <typename T>
+static int launch_layernorm(const T* x, const float* w, T* out, int n_rows, int width, float eps, size_t smem, cudaStream_t stream) {
+  const int e = allow_smem(layernorm_rows_kernel<T>, smem);
+  if (e != 0) return e;
+  pe::launch(layernorm_rows_kernel<T>, n_rows, 256, smem, stream, x, w, out, n_rows, width, eps);
+  PE_LAUNCH_CHECK();
+  return PE_OK;
+}
+
 }  // namespace pe
 
 extern "C" int pe_stream_mix(int dtype, const float* single, float* x, const void* y, const float* bias, const float* mix,
@@ -291,13 +298,7 @@ extern "C" int pe_layernorm(int dtype, const void* x, const float* w, void* out,
   if (n_rows <= 0) return PE_OK;
   const size_t smem = (size_t)width * sizeof(float);
   if (width <= 0 || smem > 48 * 1024) return PE_ERR_UNSUPPORTED_SIZE;
-  if (dtype == PE_F32)
-    pe::launch(pe::layernorm_rows_kernel<float>, n_rows, 256, smem, stream, (const float*)x, w, (float*)out, n_rows, width, eps);
-  else if (dtype == PE_BF16)
-    pe::launch(pe::layernorm_rows_kernel<__nv_bfloat16>, n_rows, 256, smem, stream, (const __nv_bfloat16*)x, w, (__nv_bfloat16*)out,
-               n_rows, width, eps);
-  else
-    return PE_ERR_UNSUPPORTED_DTYPE;
-  PE_LAUNCH_CHECK();
-  return PE_OK;
+  if (dtype == PE_F32) return pe::launch_layernorm((const float*)x, w, (float*)out, n_rows, width, eps, smem, stream);
+  if (dtype == PE_BF16) return pe::launch_layernorm((const __nv_bfloat16*)x, w, (__nv_bfloat16*)out, n_rows, width, eps, smem, stream);
+  return PE_ERR_UNSUPPORTED_DTYPE;
 }

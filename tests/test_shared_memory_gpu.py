@@ -32,10 +32,54 @@ def experts(ops, g, dtype, out_dtype):
     return out, want, (k + 1) * 2.0 ** -24 * size + STEP[out_dtype] * want.abs()       # k products added in any order
 
 
+def norm_bound(width, x64, w64, want, dtype):
+    """A layer norm's: the mean is off by width * 2^-24 of the mean magnitude, so is every difference; the squares' sum by
+    (width + 4) * 2^-24 of itself and by the differences' error; root, quotient, two products: 8 more roundings."""
+    mean = x64.mean(1, keepdim=True)
+    sigma = ((x64 - mean) ** 2).mean(1, keepdim=True).sqrt()
+    e = (width + 2) * 2.0 ** -24 * x64.abs().mean(1, keepdim=True)
+    return (2 * e / sigma + 8 * 2.0 ** -24 + (width + 4) * 2.0 ** -24) * (want.abs() + w64.abs()) + STEP[dtype] * want.abs()
+
+
+def layer_norm(ops, g, dtype, width):
+    x, w = randn(g, 3, width).to(dtype), randn(g, width)
+    out = torch.empty_like(x)
+    ops.layernorm(x, w, out, 1e-5)
+    x64, w64 = x.to(F64), w.to(F64)
+    d = x64 - x64.mean(1, keepdim=True)
+    want = d / torch.sqrt((d * d).mean(1, keepdim=True) + 1e-5) * w64
+    return out, want, norm_bound(width, x64, w64, want, dtype)
+
+
+def streams(ops, g, dtype, s, width):
+    """stream_mix: a row, and with nine streams the mix beside it."""
+    x, w, read = randn(g, 2, s, width), randn(g, width), torch.rand(s, generator=g, device=DEV) + 0.5
+    y, write = randn(g, 2, width).to(dtype), randn(g, s)
+    mix = randn(g, s, s)
+    out = torch.empty(2, width, dtype=dtype, device=DEV)
+    before, y64 = x.to(F64), y.to(F64)
+    ops.stream_mix(None, x, y, None, mix, write, read, "layer", w, 1e-5, out)
+    now = torch.einsum("it,niw->ntw", mix.to(F64), before) + write.to(F64)[None, :, None] * y64[:, None]
+    row = torch.einsum("i,niw->nw", read.to(F64), now)
+    d = row - row.mean(1, keepdim=True)
+    sigma = torch.sqrt((d * d).mean(1, keepdim=True) + 1e-5)
+    want = d / sigma * w.to(F64)
+    # the row itself: s sums of s + 1 terms, each term a product
+    size = torch.einsum("i,niw->nw", read.to(F64).abs(), torch.einsum("it,niw->ntw", mix.to(F64).abs(), before.abs())
+                        + write.to(F64).abs()[None, :, None] * y64.abs()[:, None])
+    bound = norm_bound(width, row, w.to(F64), want, dtype) + (2 * s + 4) * 2.0 ** -24 * size / sigma * w.to(F64).abs()
+    return out, want, bound
+
+
 CASES = {
     "experts float32": lambda ops, g: experts(ops, g, F32, F32),
     "experts bfloat16": lambda ops, g: experts(ops, g, BF16, BF16),
     "experts bfloat16 to float32": lambda ops, g: experts(ops, g, BF16, F32),
+    "layer norm 12257 float32": lambda ops, g: layer_norm(ops, g, F32, 12257),
+    "layer norm 12288 bfloat16": lambda ops, g: layer_norm(ops, g, BF16, 12288),
+    "one stream 12260 bfloat16": lambda ops, g: streams(ops, g, BF16, 1, 12260),
+    "two streams 12288 float32": lambda ops, g: streams(ops, g, F32, 2, 12288),
+    "nine streams 12189 float32": lambda ops, g: streams(ops, g, F32, 9, 12189),
 }
 
 

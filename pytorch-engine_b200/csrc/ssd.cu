@@ -359,12 +359,10 @@ static int ssd_run(const SsdArgs& a, cudaStream_t stream) {
   auto k0 = ssd_kernel<T, 0, NR, SPLIT, CONST>;
   auto k1 = ssd_kernel<T, 1, NR, SPLIT, CONST>;
   auto k3 = ssd_kernel<T, 3, NR, SPLIT, CONST>;
-  if (smem > 48 * 1024) {
-    cudaError_t e = cudaFuncSetAttribute(k0, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k1, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k3, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return (int)e;
-  }
+  int e = allow_smem(k0, smem);
+  if (e == 0) e = allow_smem(k1, smem);
+  if (e == 0) e = allow_smem(k3, smem);
+  if (e != 0) return e;
   if (a.chunk > 0) {
     launch(k1, dim3(a.heads, a.n_seqs, a.max_chunks), dim3(threads), smem, stream, a);
     const size_t unit = (size_t)n * dv;

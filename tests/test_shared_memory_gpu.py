@@ -71,6 +71,36 @@ def streams(ops, g, dtype, s, width):
     return out, want, bound
 
 
+def state_space(ops, g, n, dv, chunk):
+    """ssd_recurrence: tokens of 32 staged at a time, beside their steps and decays."""
+    heads, t = 2, 70
+    xbc, dt = randn(g, t, heads * dv + 2 * n), randn(g, t, heads)
+    bias, A_log, D = randn(g, heads), randn(g, heads) * 0.3, randn(g, heads)
+    y, S = torch.empty(t, heads * dv, device=DEV), torch.zeros(1, heads, n, dv, device=DEV)
+    chunks = -(-t // chunk) if chunk else 1
+    scratch = torch.empty(ops.ssd_scratch_floats(1, heads, n, dv, chunks), device=DEV) if chunk else None
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=DEV)
+    status = i32(0, 0, 0, 0)
+    ops.ssd_recurrence(xbc, dt, bias, A_log, D, y, S, i32(0), i32(0, t), 1, t, heads, 1, n, dv, status, chunk, chunks, scratch)
+    assert status.tolist()[0] == 0
+    x64, step = xbc.to(F64), torch.nn.functional.softplus(dt.to(F64) + bias.to(F64))
+    B, C = x64[:, heads * dv:heads * dv + n], x64[:, heads * dv + n:]
+    want, size = torch.zeros(t, heads * dv, dtype=F64, device=DEV), torch.zeros(t, heads * dv, dtype=F64, device=DEV)
+    for h in range(heads):
+        at = slice(h * dv, (h + 1) * dv)
+        s = torch.zeros(n, dv, dtype=F64, device=DEV)
+        a = s.clone()
+        for i in range(t):
+            f = torch.exp(-torch.exp(A_log[h].to(F64)) * step[i, h])
+            s = f * s + step[i, h] * torch.outer(B[i], x64[i, at])
+            a = f * a + step[i, h] * torch.outer(B[i].abs(), x64[i, at].abs())
+            want[i, at] = s.T @ C[i] + D[h].to(F64) * x64[i, at]
+            size[i, at] = a.T @ C[i].abs() + (D[h].to(F64) * x64[i, at]).abs()
+    # a state's term has gone through at most t steps of 4 roundings (decay and step are functions good to 2^-20 of their value,
+    # a decay's through its exponent of at most some 16), the output is a sum of n + 1
+    return y, want, (t * (4 * 2.0 ** -24 + 16 * 2.0 ** -20) + (n + 2) * 2.0 ** -24) * size
+
+
 CASES = {
     "experts float32": lambda ops, g: experts(ops, g, F32, F32),
     "experts bfloat16": lambda ops, g: experts(ops, g, BF16, BF16),
@@ -80,6 +110,10 @@ CASES = {
     "one stream 12260 bfloat16": lambda ops, g: streams(ops, g, BF16, 1, 12260),
     "two streams 12288 float32": lambda ops, g: streams(ops, g, F32, 2, 12288),
     "nine streams 12189 float32": lambda ops, g: streams(ops, g, F32, 9, 12189),
+    "state space 64 x 240": lambda ops, g: state_space(ops, g, 64, 240, 0),
+    "state space 64 x 240 in chunks": lambda ops, g: state_space(ops, g, 64, 240, 32),
+    "state space 16 x 352": lambda ops, g: state_space(ops, g, 16, 352, 0),
+    "state space 16 x 352 in chunks": lambda ops, g: state_space(ops, g, 16, 352, 32),
 }
 
 

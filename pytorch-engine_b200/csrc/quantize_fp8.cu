@@ -5,7 +5,8 @@
 //
 // The scale is a power of two: x / s is then exact, so a block's values do not depend on how a quotient is rounded, and a
 // power of two costs e4m3 nothing but its smallest values (its relative precision is the same in every binade).  A NaN stays a
-// NaN and does not count for the block's maximum; an infinity becomes a NaN (e4m3 has none), and with it the block's scale is 2^120.
+// NaN and does not count for the block's maximum (a block of nothing else has a block of zeros' scale); an infinity becomes a NaN
+// (e4m3 has none), and with it the block's scale is 2^120.
 //
 // Scales of rows are stored by block, [blocks, rows]: the products (gemm_fp8.cu) read one block's scales of many rows at a time.
 #include "api.h"
@@ -22,10 +23,10 @@ template <typename T> struct Raw8;
 template <> struct Raw8<__nv_bfloat16> {
   uint4 v;
   __device__ __forceinline__ float top() const {
-    // the largest magnitudes two at a time; a NaN loses against a number
+    // the largest magnitudes two at a time; a NaN loses against a number, eight of them against the 0
     const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
     const __nv_bfloat162 m = __hmax2(__hmax2(__habs2(h[0]), __habs2(h[1])), __hmax2(__habs2(h[2]), __habs2(h[3])));
-    return fmaxf(__low2float(m), __high2float(m));
+    return fmaxf(fmaxf(__low2float(m), __high2float(m)), 0.f);
   }
   __device__ __forceinline__ void get(float (&f)[8]) const {
     const uint32_t u[4] = {v.x, v.y, v.z, v.w};
@@ -39,8 +40,8 @@ template <> struct Raw8<__nv_bfloat16> {
 template <> struct Raw8<float> {
   float4 v[2];
   __device__ __forceinline__ float top() const {
-    return fmaxf(fmaxf(fmaxf(fabsf(v[0].x), fabsf(v[0].y)), fmaxf(fabsf(v[0].z), fabsf(v[0].w))),
-                 fmaxf(fmaxf(fabsf(v[1].x), fabsf(v[1].y)), fmaxf(fabsf(v[1].z), fabsf(v[1].w))));
+    return fmaxf(fmaxf(fmaxf(fmaxf(fabsf(v[0].x), fabsf(v[0].y)), fmaxf(fabsf(v[0].z), fabsf(v[0].w))),
+                       fmaxf(fmaxf(fabsf(v[1].x), fabsf(v[1].y)), fmaxf(fabsf(v[1].z), fabsf(v[1].w)))), 0.f);
   }
   __device__ __forceinline__ void get(float (&f)[8]) const {
     f[0] = v[0].x; f[1] = v[0].y; f[2] = v[0].z; f[3] = v[0].w; f[4] = v[1].x; f[5] = v[1].y; f[6] = v[1].z; f[7] = v[1].w;

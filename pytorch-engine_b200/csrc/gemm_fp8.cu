@@ -222,7 +222,7 @@ gemm_fp8_kernel(Params p, const __grid_constant__ CUtensorMap wmap, const __grid
         if (at + 8 <= p.K) {
           r.v[q] = *reinterpret_cast<const uint4*>(x);
         } else {
-          __nv_bfloat16 e[8];
+          alignas(16) __nv_bfloat16 e[8];
 #pragma unroll
           for (int k = 0; k < 8; ++k) e[k] = at + k < p.K ? x[k] : __float2bfloat16_rn(0.f);
           r.v[q] = *reinterpret_cast<const uint4*>(e);

@@ -53,7 +53,7 @@ __device__ __forceinline__ Raw8<T> load8(const T* row, int c, int K, bool vec) {
   if (vec && c + 8 <= K) {
     r = *reinterpret_cast<const Raw8<T>*>(row + c);
   } else {
-    T e[8];
+    alignas(16) T e[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) e[i] = c + i < K ? row[c + i] : from_f32<T>(0.f);
     r = *reinterpret_cast<const Raw8<T>*>(e);

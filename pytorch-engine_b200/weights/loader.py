@@ -12,9 +12,9 @@ become int32.  A tensor's role decides what it may be stored as: a matrix, an em
 stored as integers is refused, and so is an integer table stored as floats (the reference refuses tensor
 types it does not know, pygguf_engine/gguf_parser.py:250-256).
 
-A matrix may be stored in 8-bit floating point (``F8_E4M3``) with a tensor ``name + "_scale_inv"`` beside it: the numbers that its
-blocks of 128 x 128 elements are multiplied by, 32- or 16-bit floats ``[blocks of rows, blocks of columns]``.  It is kept so
-(``parts/float8.py``); a part that has no product with such a weight, and a float32 run, get its numbers.
+A matrix (of two dimensions) may be stored in 8-bit floating point (``F8_E4M3``) with a tensor ``name + "_scale_inv"`` beside it:
+the numbers that its blocks of 128 x 128 elements are multiplied by, 32- or 16-bit floats ``[blocks of rows, blocks of columns]``.
+It is kept so (``parts/float8.py``); a part that has no product with such a weight, and a float32 run, get its numbers.
 
 Tensors the plan does not name are errors, with two exceptions that the plan itself declares:
 ``plan.duplicates`` (a name that may be in the file if it holds the same values as another tensor: a tied
@@ -135,8 +135,9 @@ def load_weights(folder: str, plan: ModelPlan, device="cpu", dtype: Optional[tor
                 sl = fh.get_slice(name)
                 where[name] = (path, tuple(sl.get_shape()), sl.get_dtype())
     missing = sorted(n for n in want if n not in where)
-    # 8-bit matrices and the scales beside them
-    scale_of = {n: n + SCALE_SUFFIX for n in want if n in where and where[n][2] == _FLOAT8_TAG and want[n].role == "matrix"}
+    # 8-bit matrices and the scales beside them; a vector or a stack of matrices in 8 bits is as unusable as any other
+    scale_of = {n: n + SCALE_SUFFIX for n in want if n in where and where[n][2] == _FLOAT8_TAG and want[n].role == "matrix"
+                and len(where[n][1]) == len(want[n].shape) == 2}
     missing = sorted(missing + [s for s in scale_of.values() if s not in where])
     scales = {s for s in scale_of.values() if s in where}
     extra = [n for n in where if n not in want and n not in scales]
@@ -145,7 +146,7 @@ def load_weights(folder: str, plan: ModelPlan, device="cpu", dtype: Optional[tor
     wrong = sorted((n, where[n][1], tuple(want[n].shape)) for n in want
                    if n in where and not want[n].fits(where[n][1]))
     wrong += sorted((s, where[s][1], tuple(-(-d // 128) for d in where[n][1])) for n, s in scale_of.items()
-                    if s in where and len(where[n][1]) == 2 and tuple(where[s][1]) != tuple(-(-d // 128) for d in where[n][1]))
+                    if s in where and tuple(where[s][1]) != tuple(-(-d // 128) for d in where[n][1]))
     bad_dtype = sorted([(n, where[n][2], want[n].role, " / ".join(usable_tags(want[n].role))) for n in want
                         if n in where and n not in scale_of and where[n][2] not in usable_tags(want[n].role)]
                        + [(s, where[s][2], "scale", " / ".join(_FLOAT_TAGS)) for s in scales if where[s][2] not in _FLOAT_TAGS])

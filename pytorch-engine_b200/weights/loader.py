@@ -155,7 +155,8 @@ def load_weights(folder: str, plan: ModelPlan, device="cpu", dtype: Optional[tor
         other = duplicates[n]
         if other not in where:
             continue
-        if where[n][1] != where[other][1]:
+        # (two 8-bit tensors are not compared: what they stand for is in their scales)
+        if where[n][1] != where[other][1] or _FLOAT8_TAG in (where[n][2], where[other][2]):
             conflicting.append((n, other))
             continue
         with safe_open(where[n][0], framework="pt", device="cpu") as fa, safe_open(where[other][0], framework="pt", device="cpu") as fb:

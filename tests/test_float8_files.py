@@ -54,3 +54,13 @@ def test_a_matrix_stored_as_something_else(pe, tmp_path):
         e = refused(pe, folder, plan, {**whole, name: whole[name].to(E4M3).reshape(shape), name + "_scale_inv": torch.ones(1, 1)})
         assert [w[0] for w in e.wrong_shape] == [name] and [b[0] for b in e.bad_dtype] == [name]
 
+
+def test_a_duplicate_in_8_bits(pe, tmp_path):
+    """A tied model whose file stores the head too, one or both in 8 bits."""
+    cfg = pe.Qwen3Config.from_dict(TEST_CONFIGS["A"])
+    folder, plan, whole = written(pe, tmp_path, cfg)
+    name, head = "model.embed_tokens.weight", "lm_head.weight"
+    eight = whole[name].to(E4M3)
+    e = refused(pe, folder, plan, {**whole, name: eight, head: eight.clone()})
+    assert [b[0] for b in e.bad_dtype] == [name] and e.conflicting == [(head, name)]
+    assert refused(pe, folder, plan, {**whole, head: eight}).conflicting == [(head, name)]

@@ -21,9 +21,12 @@
 // registers and hand it back before they convert or store anything.
 //
 // Roles: warp 0 copies x and the weights, warp 1 (in the pair's first block) copies scales up, warp 2 allocates tensor memory and (in
-// the first block) issues the MMAs, warp 3 prepares scales, warps 4 to 11 are the epilogue.  Every wait is bounded; one that runs out records kStatusWaitTimedOut, every role
-// leaves its loop, what is in flight is waited for (bounded again) and tensor memory is freed.
+// the first block) issues the MMAs, warp 3 prepares scales, warps 4 to 11 are the epilogue.
+//
+// Every wait is bounded; one that runs out records kStatusWaitTimedOut and every role leaves its loop.  The blocks then tell each other
+// how far they came, and both stay until MMAs, copies of scales and both blocks' copies have finished (bounded again; drain.h).
 #include "api.h"
+#include "drain.h"
 #include "fp8_out.cuh"
 
 namespace pe {
@@ -83,6 +86,9 @@ __device__ __forceinline__ void commit_both(uint64_t* bar) {
 __device__ __forceinline__ void commit_one(uint64_t* bar) {        // in this block only
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(tma::smem_addr(bar)) : "memory");
 }
+__device__ __forceinline__ void st_cluster(uint32_t addr, int v) {
+  asm volatile("st.shared::cluster.s32 [%0], %1;\n" ::"r"(addr), "r"(v) : "memory");
+}
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(bar) : "memory");
 }
@@ -118,11 +124,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 gemm_fp8_pair_kernel(Params p, const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap) {
   constexpr bool GLU = MODE == kGlu || MODE == kGluFp8;
   extern __shared__ char smem_raw[];
-  __shared__ uint64_t full_bar[STAGES], empty_bar[STAGES], sf_full[SLOTS], sf_empty[SLOTS], acc_full, acc_empty;
+  __shared__ uint64_t full_bar[STAGES], empty_bar[STAGES], sf_full[SLOTS], sf_empty[SLOTS], acc_full, acc_empty, drained;
   __shared__ float top_s[2][BM];
   __shared__ uint32_t tmem_holder;
   __shared__ volatile int failed;
-  __shared__ int started, fed, issued;    // stages whose copies were started, whose scales were, whose MMAs were
+  __shared__ int started, fed;            // stages whose copies were started, whose scales were handed over
+  __shared__ int their_started, their_failed;   // the other block's, when all is over
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   char* scales_s = smem + STAGES * kStage;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -141,7 +148,8 @@ gemm_fp8_pair_kernel(Params p, const __grid_constant__ CUtensorMap amap, const _
     }
     tma::mbar_init(&acc_full, 1);         // a commit, delivered to both blocks
     tma::mbar_init(&acc_empty, 16);       // the leader's: the epilogue warps of both blocks
-    failed = started = fed = issued = 0;
+    tma::mbar_init(&drained, 2);          // commits behind all that warps 1 and 2 issued, delivered to both blocks
+    failed = started = fed = 0;
     tma::fence_barrier_init();
   }
   if (warp == 2) tmem_alloc2(&tmem_holder, kTmemCols);
@@ -269,7 +277,6 @@ gemm_fp8_pair_kernel(Params p, const __grid_constant__ CUtensorMap amap, const _
         }
         if (ok) commit_both(&acc_full);
       }
-      issued = g;
       if (!ok) {
         report(p.status, kStatusWaitTimedOut, 101, (int)blockIdx.x, g);
         failed = 1;
@@ -358,15 +365,32 @@ gemm_fp8_pair_kernel(Params p, const __grid_constant__ CUtensorMap amap, const _
   __syncwarp();
   fence_before_sync();
   __syncthreads();
-  if (failed && leader && threadIdx.x == 64) {   // MMAs that still read both blocks' shared memory, copies still on their way to it
-    for (int i = max(0, issued - STAGES); i < issued; ++i) tma::mbar_wait(&empty_bar[i % STAGES], (i / STAGES) & 1);
-    for (int i = max(0, started - STAGES); i < started; ++i) {
-      if (i >= fed) tma::mbar_arrive(&full_bar[i % STAGES]);
-      tma::mbar_wait(&full_bar[i % STAGES], (i / STAGES) & 1);
-    }
+  if (threadIdx.x == 0) {
+    st_cluster(map_to_rank(tma::smem_addr(&their_started), rank ^ 1), started);
+    st_cluster(map_to_rank(tma::smem_addr(&their_failed), rank ^ 1), failed);
   }
   __syncwarp();
   cluster_sync();
+  if (failed || their_failed) {           // the same answer in both blocks
+    // MMAs, which read both blocks' shared memory, copies of scales, and the commits behind them
+    if (leader && lane == 0 && (warp == 1 || warp == 2)) commit_both(&drained);
+    if (warp == 2 && lane == 0) {
+      tma::mbar_wait(&drained, 0);
+      if (leader) {                       // both blocks' copies count on this block's barriers
+        const int last = max(started, their_started);
+        for (int i = max(0, last - STAGES); i < last; ++i) {
+          uint64_t* bar = &full_bar[i % STAGES];
+          const Owed o = owed_to_stage(i, started, their_started, fed, kStage);
+          if (o.expect) tma::mbar_expect_only(bar, o.expect);
+          if (o.complete) tma::mbar_complete_only(bar, o.complete);
+          for (int k = 0; k < o.arrivals; ++k) tma::mbar_arrive(bar);
+          tma::mbar_wait(bar, (i / STAGES) & 1);
+        }
+      }
+    }
+    __syncwarp();
+    cluster_sync();
+  }
   if (warp == 2) {
     fence_after_sync();
     tmem_dealloc2(tmem_base, kTmemCols);

@@ -73,7 +73,7 @@ gemm_fp8_kernel(Params p, const __grid_constant__ CUtensorMap wmap, const __grid
   using S = Shape<NP>;
   constexpr int STAGES = S::kStages, KBS = S::kKbs, EPI = S::kEpiWarps, COLS = S::kCols, CH = S::kChunk, ET = 32 * EPI;
   extern __shared__ char smem_raw[];
-  __shared__ uint64_t full_bar[STAGES], done_bar[STAGES], read_bar[STAGES];
+  __shared__ uint64_t full_bar[STAGES], done_bar[STAGES], read_bar[STAGES], raw_bar[RAW ? STAGES : 1];
   __shared__ __align__(16) float sx_s[CH][NP];
   __shared__ float sw_s[4][CH];
   __shared__ uint32_t tmem_holder;
@@ -124,7 +124,9 @@ gemm_fp8_kernel(Params p, const __grid_constant__ CUtensorMap wmap, const __grid
   if (threadIdx.x == 64 && !RAW) prefetch_map(&xmap);
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      tma::mbar_init(&full_bar[s], RAW ? 1 + EPI : 2);    // the weights' producer, and the rows' or the warps that convert them
+      tma::mbar_init(&full_bar[s], RAW ? 1 : 2);          // the producers: the weights', and the rows'
+      // the epilogue's warps, when they have converted a stage's rows: each has then read what the MMAs of the stage before left
+      if (RAW) tma::mbar_init(&raw_bar[s], EPI);
       tma::mbar_init(&done_bar[s], 1);    // the commit behind a stage's MMAs
       tma::mbar_init(&read_bar[s], EPI);  // the epilogue's warps
     }
@@ -180,7 +182,8 @@ gemm_fp8_kernel(Params p, const __grid_constant__ CUtensorMap wmap, const __grid
         for (int stage = 0; stage < STAGES; ++stage) {
           const int i = i0 + stage, n = n_kb - i * KBS;
           if (n <= 0) break;
-          ok = tma::mbar_wait_both(&read_bar[stage], ((i / STAGES) & 1) ^ 1, &full_bar[stage], (i / STAGES) & 1);
+          const uint32_t parity = (i / STAGES) & 1;
+          ok = tma::mbar_wait_both(RAW ? &raw_bar[RAW ? stage : 0] : &read_bar[stage], RAW ? parity : parity ^ 1, &full_bar[stage], parity);
           if (!ok) {
             report(p.status, kStatusWaitTimedOut, 71, tile, i);
             failed = 1;
@@ -261,7 +264,7 @@ gemm_fp8_kernel(Params p, const __grid_constant__ CUtensorMap wmap, const __grid
     }
     tma::fence_proxy_async();          // the MMAs read what was written here
     __syncwarp();
-    if (lane == 0) tma::mbar_arrive(&full_bar[stage]);
+    if (lane == 0) tma::mbar_arrive(&raw_bar[RAW ? stage : 0]);
   };
   float acc[COLS];
   const int quarter = warp & 3, row = quarter * 32 + lane;         // of the tile's weight rows: with GLU R gates, then R ups
@@ -296,7 +299,7 @@ gemm_fp8_kernel(Params p, const __grid_constant__ CUtensorMap wmap, const __grid
         if (lane == 0) report(p.status, kStatusWaitTimedOut, 72, tile, i);
         failed = 1;
       }
-      if (RAW && !failed) tma::mbar_wait(&full_bar[stage], (i / STAGES) & 1);    // long complete: the other warps' scales are seen
+      if (RAW && !failed) tma::mbar_wait(&raw_bar[RAW ? stage : 0], (i / STAGES) & 1);    // long complete: the other warps' scales are seen
       __syncwarp();
       fence_after_sync();
 #pragma unroll
@@ -322,7 +325,7 @@ gemm_fp8_kernel(Params p, const __grid_constant__ CUtensorMap wmap, const __grid
       }
       fence_before_sync();
       __syncwarp();
-      if (lane == 0) tma::mbar_arrive(&read_bar[stage]);
+      if (!RAW && lane == 0) tma::mbar_arrive(&read_bar[stage]);
       if (RAW && i + STAGES < n_st) raw_store(i + STAGES, raw[0]);
     }
     if (p.split > 1 || GLU) {
@@ -412,10 +415,9 @@ gemm_fp8_kernel(Params p, const __grid_constant__ CUtensorMap wmap, const __grid
   if (warp == 1) {
     if (failed && lane == 0) {         // MMAs that still read this block's shared memory, copies still on their way to it
       for (int i = max(0, issued - STAGES); i < issued; ++i) tma::mbar_wait(&done_bar[i % STAGES], (i / STAGES) & 1);
-      // (with RAW the epilogue has converted every stage all the same: only weights can be missing)
-      const int last = RAW ? n_st : max(started[0], started[1]);
+      const int last = RAW ? started[0] : max(started[0], started[1]);
       for (int i = max(0, last - STAGES); i < last; ++i) {
-        if (i >= started[0] || (!RAW && i >= started[1])) tma::mbar_arrive(&full_bar[i % STAGES]);     // for the operand that was not asked for
+        if (!RAW && (i >= started[0] || i >= started[1])) tma::mbar_arrive(&full_bar[i % STAGES]);     // for the operand that was not asked for
         tma::mbar_wait(&full_bar[i % STAGES], (i / STAGES) & 1);
       }
     }

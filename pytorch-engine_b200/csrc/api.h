@@ -334,6 +334,7 @@ int pe_quantize_rows_fp8(int dtype, const void* x, long long x_ld, const int* ro
     long long v_ld, float* scales, long long s_ld, int M, int K, int x_rows, int* status, cudaStream_t stream);
 int pe_quantize_weight_fp8(int dtype, const void* w, long long w_ld, void* values, long long v_ld, float* scales, int N, int K,
     cudaStream_t stream);
+int pe_settle_weights(cudaStream_t stream);
 int pe_rmsnorm_residual_fp8(float* residual, const void* delta, const float* weight, void* values, long long v_ld, float* scales,
     long long s_ld, int n_rows, int dim, float eps, cudaStream_t stream);
 

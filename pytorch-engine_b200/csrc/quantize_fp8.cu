@@ -126,9 +126,10 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* x, long lon
   }
 }
 
-// One thread block for 128 x 128 elements, which it holds in registers between the maximum and the conversion.  Its successor
-// in the stream may not start early: it may be a product that asks for these values before it waits (which only the dependents of a
-// grid with launch_dependents must do).
+// One thread block for 128 x 128 elements, which it holds in registers between the maximum and the conversion.  Its successor in the
+// stream may be a product that asks for these values before it waits for this grid.  So it lets nothing start early, which leaves a
+// successor to start when all blocks have ended, and a block ends behind a fence: what it wrote has then reached the memory that all
+// SMs and their copies (the async proxy's) read.
 template <typename T>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) quantize_weight_kernel(const T* w, long long w_ld, uint8_t* values, long long v_ld,
                                                                                     float* scales, int N, int K, bool vec) {
@@ -153,8 +154,16 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) quantize_weight_k
     const int r = rb * BLOCK + i * 16 + (threadIdx.x >> 4);
     if (r < N) store8<T>(values + (size_t)r * v_ld, c, K, v[i], s, a);
   }
-  if (threadIdx.x == 0) scales[blockIdx.x] = __uint_as_float(s);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    scales[blockIdx.x] = __uint_as_float(s);
+    __threadfence();
+    asm volatile("fence.proxy.async.global;\n" ::: "memory");
+  }
 }
+
+// Nothing, behind everything in front of it: see pe_settle_weights.
+__global__ void settle_kernel() {}
 
 // rmsnorm.cu's norm (with its residual add) whose result, rounded to bfloat16, is quantised on the way out: what rmsnorm.cu's
 // kernel and the one above would give, without the bfloat16 rows between them.  The sum of squares is taken in rmsnorm.cu's order, four
@@ -276,6 +285,15 @@ extern "C" int pe_quantize_weight_fp8(int dtype, const void* w, long long w_ld, 
   } else {
     return PE_ERR_UNSUPPORTED_DTYPE;
   }
+  if (e != cudaSuccess) return (int)e;
+  PE_LAUNCH_CHECK();
+  return PE_OK;
+}
+
+// What the stream has written up to here may be read as weights by the launches behind: a product asks for its weights while the
+// launch in front of it still runs, and this one, which does not start before all in front of it has completed, then stands between.
+extern "C" int pe_settle_weights(cudaStream_t stream) {
+  const cudaError_t e = pe::launch_after(pe::quant8::settle_kernel, dim3(1), dim3(32), 0, stream);
   if (e != cudaSuccess) return (int)e;
   PE_LAUNCH_CHECK();
   return PE_OK;

@@ -138,6 +138,7 @@ _SIGNATURES = {
     "pe_rows_to_pages_pair": [I, P, L, I, I, I, I, I, I, I, P, P, P, P, I, I, P, P, P, P],
     "pe_quantize_rows_fp8": [I, P, L, P, P, P, L, P, L, I, I, I, P, P],
     "pe_quantize_weight_fp8": [I, P, L, P, L, P, I, I, P],
+    "pe_settle_weights": [P],
     "pe_rmsnorm_residual_fp8": [P, P, P, P, L, P, L, I, I, F, P],
     "pe_gemm_fp8": [P, L, P, L, P, L, P, P, L, I, I, I, I, I, F, F, P, P, P, I, P, P],
     "pe_gemm_fp8_many_takes": [I, I, I, I, I],

@@ -1572,6 +1572,18 @@ def quantize_weight_fp8(w: torch.Tensor, values: torch.Tensor, scales: torch.Ten
     _count(1)
 
 
+def settle_weights(weight: torch.Tensor) -> None:
+    """Call it behind a copy or another operation that writes ``weight`` (values or scales) on its device's current stream, and in front
+    of a product with it.  A product of this package asks for its weight while the launch in front of it is still running; an empty launch
+    that waits for all before it then stands between.  Nothing is needed behind ``quantize_weight_fp8``, behind a wait of the
+    host, or with other launches of this package in between.  On the CPU it does nothing."""
+    if not weight.is_cuda:
+        return
+    with torch.cuda.device(weight.device):
+        check(library().pe_settle_weights(_stream()), "settle_weights")
+    _count(1)
+
+
 def rmsnorm_residual_fp8_supported(dim: int) -> bool:
     """Whether csrc/quantize_fp8.cu has the norm and the conversion in one kernel."""
     return dim % 4 == 0 and dim <= 51200
@@ -1683,8 +1695,8 @@ def gemm_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales:
     ``powers``: the caller knows that all scales are powers of two, as this module's conversions make them.  Many rows are then up to
     1.5 times as fast (csrc/gemm_fp8_pair.cu); the sums of K are taken in another order there.
 
-    ``w`` is a weight: the kernel starts to read it while the one launched before it is still running, so that one must
-    not be what writes it (``quantize_weight_fp8`` may be: it lets nothing start early)."""
+    ``w`` and ``w_scales`` are a weight: the kernel starts to read them while the one launched before it is still running, so that
+    one must not be what writes them (``quantize_weight_fp8`` may be, others with ``settle_weights`` behind them)."""
     _gemm_fp8("gemm_fp8", x, x_scales, w, w_scales, out, status, glu, None, None, powers)
 
 

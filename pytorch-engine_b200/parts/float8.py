@@ -71,7 +71,8 @@ def _all_powers(weights) -> Optional[bool]:
 class Float8Weight:
     """``values [N, K]`` (e4m3) and ``scales [fp8_blocks(N), fp8_blocks(K)]`` (float32); or several such matrices stacked in
     front, ``[G, N, K]`` and ``[G, ...]``.  Rows start on 16-byte boundaries (``to`` makes it so).  ``powers``: whether all scales are
-    powers of two, which makes products of many rows faster; None: not known (``to`` finds out)."""
+    powers of two, which makes products of many rows faster; None: not known (``to`` finds out).  What the methods here make can go
+    into a product at once; for values written by other means see ``ops.settle_weights``."""
 
     __slots__ = ("values", "scales", "powers")
     dtype = FP8
@@ -111,13 +112,19 @@ class Float8Weight:
         return cls(values, scales, True)
 
     @classmethod
+    def _settled(cls, values: torch.Tensor, scales: torch.Tensor, powers: Optional[bool]) -> "Float8Weight":
+        """A weight that copies in front of this call have written."""
+        ops.settle_weights(values)
+        return cls(values, scales, powers)
+
+    @classmethod
     def stack(cls, weights: Sequence["Float8Weight"]) -> "Float8Weight":
         """Matrices of one shape as one weight ``[G, N, K]``."""
         first = weights[0]
         values = _padded_empty((len(weights), *first.shape), first.device)
         for i, w in enumerate(weights):
             values[i].copy_(w.values)
-        return cls(values, torch.stack([w.scales for w in weights]).contiguous(), _all_powers(weights))
+        return cls._settled(values, torch.stack([w.scales for w in weights]).contiguous(), _all_powers(weights))
 
     @staticmethod
     def stacks_rows(weights: Sequence["Float8Weight"]) -> bool:
@@ -134,7 +141,7 @@ class Float8Weight:
         for w in weights:
             values[at:at + w.shape[0]].copy_(w.values)
             at += w.shape[0]
-        return cls(values, torch.cat([w.scales for w in weights]).contiguous(), _all_powers(weights))
+        return cls._settled(values, torch.cat([w.scales for w in weights]).contiguous(), _all_powers(weights))
 
     def with_zero_rows(self, rows: int) -> "Float8Weight":
         """The matrix with so many rows of zeros behind its last one, in whose block they must still lie."""
@@ -146,7 +153,7 @@ class Float8Weight:
         values = _padded_empty((n + rows, k), self.device)
         values[:n].copy_(self.values)
         values[n:].view(torch.uint8).zero_()
-        return Float8Weight(values, self.scales, self.powers)
+        return self._settled(values, self.scales, self.powers)
 
     def to(self, device) -> "Float8Weight":
         """On ``device``, with rows on 16-byte boundaries, and ``powers`` known (for which the host waits for the device)."""
@@ -158,7 +165,7 @@ class Float8Weight:
         if powers is None:
             bits = scales.view(torch.int32)
             powers = bool(((bits & 0x7fffff) == 0).logical_and_(bits > 0).logical_and_(bits != 0x7f800000).all())
-        return Float8Weight(values, scales, powers)
+        return self._settled(values, scales, powers)
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         n, k = self.shape[-2:]

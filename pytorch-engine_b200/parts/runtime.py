@@ -244,7 +244,10 @@ class Runtime:
     def linear(self, x: torch.Tensor, weight: torch.Tensor, out: Optional[torch.Tensor] = None,
                out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
         """``x [M, K] @ weight [N, K]^T -> [M, N]``.  With a ``Float8Weight`` the rows are quantised in blocks of 128 on the way
-        (``x`` may be ``Float8Rows`` already); ``out_dtype`` is then bfloat16 unless given."""
+        (``x`` may be ``Float8Rows`` already); ``out_dtype`` is then bfloat16 unless given.
+
+        A weight is read while the launch in front of the product may still be running: what has just been written to it on this
+        stream (by anything but ``Float8Weight``'s own methods) is settled with ``ops.settle_weights`` first."""
         if not self.is_cuda:
             raise KernelError("this package computes on a CUDA device only; there is no CPU path")
         if type(weight) is Float8Weight:

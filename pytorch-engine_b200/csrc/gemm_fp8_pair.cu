@@ -7,6 +7,10 @@
 // gives its four the same one.  Nothing is left to do between two blocks of K: sums stay in tensor memory over all of K, and two
 // SMs share a tile of 256 x 256 (cta_group::2), each with half of both operands in its shared memory.
 //
+// The tensor cores cut a sum to float32 after every 32 terms, where the other two kernels take a block's sum out and round: sums of
+// 12,288 terms of one sign are 111 * 2^-24 of their value off on average (4,096 terms: 22), all towards zero, against 2 * 2^-24 there
+// (1.2); of random signs 0.13 and 0.02 * 2^-24 of the terms' magnitudes.  A bfloat16 result is rounded by up to 65,536 * 2^-24.
+//
 // Scales lie in tensor memory too.  One warp turns the float32 scales of four k blocks into bytes, a word of them for each row of x
 // and for the two blocks of weight rows, as 32 lanes x 16 bytes for 128 rows; tcgen05.cp copies them up in front of the MMAs that use
 // them, byte i for the i-th of the four blocks.

@@ -117,3 +117,109 @@ def test_rows_that_end_inside_a_block(pe):
     assert torch.equal(got[:130], torch.cat([m.dequantize(BF16) for m in mats])) and bool((got[130:] == 0).all())
     with pytest.raises(ValueError):
         f8.Float8Weight(torch.ones(128, 40).to(E4M3), torch.ones(1, 1)).with_zero_rows(1)
+
+
+# ---- on the GPU ------------------------------------------------------------------------------------------------------------
+def prompt_of(d, n, seed=3):
+    vocab = d.get("vocab") or d["vocab_size"]
+    return torch.randint(0, vocab, (n,), generator=torch.Generator().manual_seed(seed)).tolist()
+
+
+def on_gpu(weights):
+    return {n: t.to(DEV) for n, t in weights.items()}
+
+
+def run(pe, eng, prompts, more=2):
+    """Logits of whole prompts, then of ``more`` single tokens of each: two tensors."""
+    slots = [eng.alloc_slot() for _ in prompts]
+    first = eng.step([pe.StepEntry(s, p, tuple(range(len(p)))) for s, p in zip(slots, prompts)]).float().cpu()
+    steps = [eng.step([pe.StepEntry(s, (5 + t,), (0,)) for s in slots]).float().cpu() for t in range(more)]
+    for s in slots:
+        eng.free_slot(s)
+    return first, torch.stack(steps)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("arch,key", [m for m in MODELS if m[0] != "qwen3"])
+def test_a_float32_run_of_8_bit_matrices(pe, arch, key):
+    """Against the plain model of the numbers, within the bound of that architecture's float32 runs."""
+    cfg, plan, d, module = describe(pe, arch, key)
+    eight, numbers = stored(pe, pe.weights.loader.expected_tensors(plan), weights_of(pe, arch, key, plan, d, module))
+    eng = pe.Engine(None, config=cfg, weights=on_gpu(eight), dtype="float32", max_context_len=128, max_cache_tokens=64 * 8, max_batch=2)
+    toks = prompt_of(d, 40)
+    got = eng.step([pe.StepEntry(eng.alloc_slot(), toks, tuple(range(40)))]).float().cpu()
+    assert rel_err(got, module.forward(d, numbers, toks).float()) < 3e-5
+
+
+def eight_bit_parts(eng):
+    """(kind, attribute) of the matrices that a model's parts keep in 8 bits, and of the others that could be."""
+    f8 = type(eng).__module__.split(".")[0]
+    Float8Weight = importlib.import_module(f8 + ".parts.float8").Float8Weight
+    kept, other = [], []
+    for built in eng.model.block_parts:
+        for part in built.values():
+            names = {"GQAttention": ("qkv", "o_proj"), "SwiGLU": ("gate_up", "down"), "RoutedExperts": ("gate_up", "down")}
+            for n in names.get(type(part).__name__, ()):
+                if type(part).__name__ == "RoutedExperts" and not part.n_experts:
+                    continue
+                (kept if type(getattr(part, n)) is Float8Weight else other).append((type(part).__name__, n))
+    return kept, other
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("arch,key", MODELS)
+def test_every_part_that_can_quantizes(pe, arch, key):
+    """``weight_format="float8"``: attention's, gated feed-forwards' and experts' matrices, in every arrangement; prompts and single
+    tokens run, from graphs the same as without."""
+    cfg, plan, d, module = describe(pe, arch, key)
+    weights = on_gpu(weights_of(pe, arch, key, plan, d, module))
+    prompts = [prompt_of(d, n, n) for n in (1, 9, 70)]
+    got = []
+    for graphs in (True, False):
+        eng = pe.Engine(None, config=cfg, weights=weights, weight_format="float8", max_context_len=128, max_cache_tokens=64 * 12, max_batch=4,
+                        enable_cuda_graph=graphs)
+        kept, other = eight_bit_parts(eng)
+        kinds = {s.kind for b in plan.blocks for _, s in b.parts.values()}
+        assert not other and bool(kept) == bool(kinds & {"attention", "swiglu", "routed_experts"})
+        got.append(run(pe, eng, prompts))
+    assert all(bool(torch.isfinite(t).all()) for pair in got for t in pair)
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("arch,key", [m for m in MODELS if m[0] in ("qwen3", "bobasun", "vabelorn")])
+def test_as_a_bfloat16_run_with_8_bit_operands(pe, arch, key):
+    """The same model in bfloat16, all its products taken over by one that rounds both operands to 8 bits and computes in float32:
+    biases, gates, norms and the order of a block are those of the 16-bit path.
+
+    The runs' activations differ by bfloat16's roundings, 2^-8 of a value, so up to 2 * 2^-8 / 2^-3 = 1/16 of a product's inputs fall
+    on different sides of an e4m3 rounding and differ by its step, 2^-3 of a value at the most: 3.1 % in the 2-norm.  A sublayer is
+    two products, a layer two sublayers: twice that of the stream if nothing else were in it, and the layers' errors add up like
+    random ones."""
+    f8 = pe.parts.float8
+    cfg, plan, d, module = describe(pe, arch, key)
+    weights = on_gpu(weights_of(pe, arch, key, plan, d, module))
+    prompts = [prompt_of(d, n, n) for n in (1, 9, 70)]
+    kw = dict(config=cfg, weights=weights, max_context_len=128, max_cache_tokens=64 * 12, max_batch=4, enable_cuda_graph=False)
+    got = run(pe, pe.Engine(None, weight_format="float8", **kw), prompts)
+    plain = pe.Engine(None, **kw)
+    numbers = {}
+    for built in plain.model.block_parts:
+        for part in built.values():
+            for n in {"GQAttention": ("qkv", "o_proj"), "SwiGLU": ("gate_up", "down")}.get(type(part).__name__, ()):
+                w = getattr(part, n)
+                numbers[w.data_ptr()] = f8.Float8Weight.quantize(w).dequantize()
+
+    def product(x, weight, out, out_dtype):
+        w = numbers.get(weight.data_ptr())
+        if w is None:
+            return None
+        y = f8.Float8Rows.quantize(x).dequantize() @ w.t()
+        return y.to(out_dtype or x.dtype) if out is None else out.copy_(y)
+
+    rt = plain.runtime
+    rt.gemm_backend, rt.own_small_gemm, rt.own_large_gemm = product, False, False
+    want = run(pe, plain, prompts)
+    bound = 0.0625 * len(plan.blocks) ** 0.5
+    for a, b in zip(got, want):
+        assert float((a - b).norm() / b.norm()) < bound

@@ -64,3 +64,65 @@ def test_a_duplicate_in_8_bits(pe, tmp_path):
     e = refused(pe, folder, plan, {**whole, name: eight, head: eight.clone()})
     assert [b[0] for b in e.bad_dtype] == [name] and e.conflicting == [(head, name)]
     assert refused(pe, folder, plan, {**whole, head: eight}).conflicting == [(head, name)]
+
+
+# ---- what the command line and a checkpoint lead to ------------------------------------------------------------------------
+@pytest.mark.parametrize("option,want", [([], None), (["--weights", "stored"], None), (["--weights", "float8"], "float8")])
+def test_the_command_line_hands_the_format_on(pe, monkeypatch, option, want):
+    from importlib import import_module
+
+    cli, seen = import_module("pytorch-engine_b200.cli"), {}
+
+    class Stop(Exception):
+        pass
+
+    class Engine:
+        @staticmethod
+        def from_random(cfg, seed, **kw):
+            seen.update(kw)
+            raise Stop
+
+    monkeypatch.setattr(pe, "Engine", Engine)
+    with pytest.raises(Stop):
+        cli.main(["--random", "tiny_b", "--prompt-ids", "1,2,3", *option])
+    assert seen["weight_format"] == want
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("key", ["A", "B", "D", "E"])
+def test_what_a_checkpoint_keeps(pe, tmp_path, key):
+    """A projection stays in 8 bits where each of its stored matrices but the last ends with a block of 128 rows; a feed-forward
+    where both of its do."""
+    from test_float8_model import make_folder
+
+    folder, cfg, _ = make_folder(tmp_path, TEST_CONFIGS[key], 4, pe)
+    d = cfg["head_dim"]
+    whole = lambda n: n % 128 == 0
+    wants = {"qkv": whole(cfg["num_attention_heads"] * d) and whole(cfg["num_key_value_heads"] * d), "o_proj": True,
+             "gate_up": whole(cfg["intermediate_size"]), "down": whole(cfg["intermediate_size"])}
+    eng = pe.Engine(folder, max_context_len=128, max_cache_tokens=64 * 4, max_batch=1)
+    for block in eng.model.blocks:
+        for part, n in ((block.mixer, "qkv"), (block.mixer, "o_proj"), (block.ffn, "gate_up"), (block.ffn, "down")):
+            assert (type(getattr(part, n)) is pe.parts.float8.Float8Weight) == wants[n], n
+
+
+@pytest.mark.gpu
+def test_cpu_tensors_are_refused(pe):
+    """On a machine that has the kernels: by name, before anything is launched."""
+    ops, dev = pe.kernels.ops, "cuda:0"
+    pe.kernels.library()
+    st = torch.zeros(4, dtype=torch.int32, device=dev)
+    x, w = torch.zeros(2, 128, dtype=torch.bfloat16), torch.zeros(64, 128).to(E4M3)
+    s, xs, out = torch.ones(1, 1), torch.ones(1, 2), torch.zeros(2, 64, dtype=torch.bfloat16)
+    calls = [lambda: ops.linear_fp8(x, w, s, out, st), lambda: ops.linear_fp8(x, w.to(dev), s.to(dev), out.to(dev), st),
+             lambda: ops.linear_fp8(x.to(dev), w.to(dev), s, out.to(dev), st), lambda: ops.linear_fp8(x.to(dev), w.to(dev), s.to(dev), out, st),
+             lambda: ops.linear_fp8(x.to(dev), w.to(dev), s.to(dev), out.to(dev), st.cpu()),
+             lambda: ops.gemm_fp8(x.to(E4M3), xs, w, s, out, st), lambda: ops.gemm_fp8(x.to(E4M3).to(dev), xs, w.to(dev), s.to(dev), out.to(dev), st),
+             lambda: ops.quantize_weight_fp8(torch.zeros(64, 128), w, s), lambda: pe.parts.float8.Float8Weight.quantize(torch.zeros(64, 128)),
+             lambda: ops.quantize_rows_fp8(x, x.to(E4M3), xs), lambda: pe.parts.float8.Float8Rows.quantize(x),
+             lambda: ops.rmsnorm_residual_fp8(torch.zeros(2, 128), None, torch.ones(128), x.to(E4M3), xs, 1e-6)]
+    for i, call in enumerate(calls):
+        with pytest.raises(pe.kernels.KernelError):
+            call()
+            pytest.fail(f"call {i} was not refused")
+    assert st.tolist()[0] == 0

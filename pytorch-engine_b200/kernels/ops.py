@@ -1500,9 +1500,10 @@ def _fp8_ld(t: torch.Tensor, what: str) -> int:
 
 def _fp8_scales_ld(scales: torch.Tensor, blocks: int, rows: int, what: str) -> int:
     strides = scales.stride()
-    if scales.dtype is not torch.float32 or scales.shape != (blocks, rows) or (strides[1] != 1 and rows != 1):
-        raise KernelError(f"{what}: scales [blocks of {FP8_BLOCK} features, rows] float32")
-    return max(strides[0], rows) if blocks > 1 else rows
+    if (scales.dtype is not torch.float32 or scales.shape != (blocks, rows) or (strides[1] != 1 and rows != 1)
+            or (strides[0] < rows and blocks > 1)):
+        raise KernelError(f"{what}: scales [blocks of {FP8_BLOCK} features, rows] float32, neighbouring rows' side by side, none shared")
+    return strides[0] if blocks > 1 else rows
 
 
 def _on_current(what: str, *tensors) -> None:

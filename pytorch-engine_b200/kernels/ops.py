@@ -1529,7 +1529,7 @@ def quantize_rows_fp8(x: torch.Tensor, values: torch.Tensor, scales: torch.Tenso
 def _quantize_rows(x, m, k, values: int, v_ld: int, scales: int, s_ld: int, row_map, live, status) -> None:
     """The launch, into memory that is known to fit; checks what is read."""
     rows = x.shape[0]
-    _on_current("quantize_rows_fp8", x, row_map, live)
+    _on_current("quantize_rows_fp8", x, row_map, live, status)
     if row_map is not None:
         _need(row_map.dtype == torch.int32 and row_map.is_contiguous() and row_map.numel() == m and status is not None,
               "quantize_rows_fp8: row_map int32, one per row, with a status word")
@@ -1657,6 +1657,8 @@ def _fp8_product(what: str, m: int, k: int, w, w_scales, out, glu, offsets, row_
     w_ld = w_stride[-2] if rows > 1 or groups > 1 else (k + 15) // 16 * 16
     if not ok or w_ld % 16:
         _fp8_product_error(what, m, k, w, w_scales, out, glu, offsets, row_weight, (*tensors, w, w_scales, out, offsets, row_weight))
+    if glu and glu[3] is not None:
+        _on_current(what, glu[3])
     return n, w_ld, groups, (0, 0.0, 1.0, None) if glu is None else _glu_args(glu or None, n)
 
 
@@ -1776,7 +1778,7 @@ def gemm_fp8_gated(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_s
                                  and row_weight.numel() >= m), f"{what}: row_weight float32, one per row, with offsets")
     x_ld, xs_ld = _fp8_ld(x, what), _fp8_scales_ld(x_scales, fp8_blocks(k), m, what)
     y_ld, ys_ld = _fp8_ld(values, what), _fp8_scales_ld(scales, fp8_blocks(n), m, what)
-    _on_current(what, x, x_scales, w, w_scales, values, scales, status, offsets, row_weight)
+    _on_current(what, x, x_scales, w, w_scales, values, scales, status, offsets, row_weight, glu[3] if glu else None)
     if m == 0:
         return
     kind, limit, alpha, bias = _glu_args(glu or None, n)

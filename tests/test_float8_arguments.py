@@ -35,3 +35,23 @@ def test_calls_with_such_scales(pe):
         with pytest.raises(KernelError):
             call()
     assert ops.launch_count() == before
+
+
+@pytest.mark.gpu
+def test_a_status_word_or_bias_elsewhere(pe):
+    """Both are written or read by the kernels: they lie where the kernels run."""
+    ops, f8, KernelError = pe.kernels.ops, pe.parts.float8, pe.kernels.KernelError
+    st, there = torch.zeros(4, dtype=torch.int32, device=DEV), torch.zeros(4, dtype=torch.int32)
+    x = torch.ones(4, 256, dtype=BF16, device=DEV)
+    r, w = f8.Float8Rows.quantize(x), f8.Float8Weight.quantize(torch.ones(256, 256, device=DEV))
+    pick = torch.zeros(4, dtype=torch.int32, device=DEV)
+    out = torch.empty(4, 128, dtype=BF16, device=DEV)
+    glu = ("silu", 0.0, 1.0, torch.zeros(256))
+    before = ops.launch_count()
+    for call in (lambda: ops.quantize_rows_fp8(x, r.values, r.scales, pick, None, there), lambda: ops.new_rows_fp8(x, pick, None, there),
+                 lambda: ops.linear_fp8(x, w.values, w.scales, out, there, ()), lambda: ops.linear_fp8(x, w.values, w.scales, out, st, glu),
+                 lambda: ops.gemm_fp8(r.values, r.scales, w.values, w.scales, out, there, ()),
+                 lambda: ops.gemm_fp8(r.values, r.scales, w.values, w.scales, out, st, glu)):
+        with pytest.raises(KernelError):
+            call()
+    assert ops.launch_count() == before

@@ -196,7 +196,7 @@ class GQAttention:
 
     def chains(self) -> bool:
         """Whether ``forward`` takes a ``residual`` (parts/block.py, PreNormBlock)."""
-        return (not self.general and type(self.qkv) is torch.Tensor and type(self.o_proj) is torch.Tensor
+        return (not self.general and type(self.qkv) is not Float8Weight and type(self.o_proj) is not Float8Weight
                 and ops.gemm_smallm_weight(self.qkv) and ops.gemm_smallm_weight(self.o_proj))
 
     @property

@@ -119,6 +119,20 @@ def test_rows_that_end_inside_a_block(pe):
         f8.Float8Weight(torch.ones(128, 40).to(E4M3), torch.ones(1, 1)).with_zero_rows(1)
 
 
+def test_weights_that_are_parameters(pe):
+    """``torch.nn.Parameter``s are tensors: an attention of 16-bit weights joins a chain of products all the same."""
+    from pytorch_engine_b200.engine.model import DecoderModel
+    from pytorch_engine_b200.parts.runtime import Runtime
+
+    cfg, plan, d, module = describe(pe, "qwen3", "D")
+    weights = {n: t.to(BF16) for n, t in weights_of(pe, "qwen3", "D", plan, d, module).items()}
+    models = [DecoderModel(plan, {n: kind(t) for n, t in weights.items()}, Runtime("cpu", BF16))
+              for kind in (torch.clone, lambda t: torch.nn.Parameter(t, requires_grad=False))]
+    assert type(models[1].blocks[0].mixer.o_proj) is torch.nn.Parameter
+    assert [[b.mixer.chains(), b.ffn.chains()] for b in models[1].blocks] == [[b.mixer.chains(), b.ffn.chains()] for b in models[0].blocks]
+    assert models[0].blocks[0].mixer.chains()
+
+
 # ---- on the GPU ------------------------------------------------------------------------------------------------------------
 def prompt_of(d, n, seed=3):
     vocab = d.get("vocab") or d["vocab_size"]

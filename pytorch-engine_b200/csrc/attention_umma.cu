@@ -882,12 +882,9 @@ extern "C" int pe_attention_umma_prefill_parts(const void* q, long long q_ld, lo
   // tiles, then barriers and the two-slot ring
   const size_t smem = (size_t)kh * kQPart + kKStages * (size_t)kh * kKPart + kVStages * kPageBytes + 256;
   auto kern = kh == 2 ? prefill_umma_kernel<2> : (kh == 3 ? prefill_umma_kernel<3> : prefill_umma_kernel<4>);
-  static bool attr_set[5] = {};
-  if (!attr_set[kh]) {
-    cudaError_t ce = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (ce != cudaSuccess) return (int)ce;
-    attr_set[kh] = true;
-  }
+  static bool asked[5][pe::kDevices] = {};
+  const int ae = pe::allow_smem_once(kern, smem, asked[kh]);
+  if (ae != 0) return ae;
   const int rows_blk = (BM / a.group) * a.group;
   const long long tiles = ((long long)max_q * a.group + rows_blk - 1) / rows_blk;
   const long long total = tiles * n_kv_heads * n_seqs * parts;

@@ -116,6 +116,21 @@ inline int allow_smem(K kernel, size_t bytes) {
   return 0;
 }
 
+// The same, asked for once on each device (it is the device's own setting): `asked` is one kernel's.
+constexpr int kDevices = 64;
+template <typename K>
+inline int allow_smem_once(K kernel, size_t bytes, bool (&asked)[kDevices]) {
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return (int)e;
+  const bool known = device >= 0 && device < kDevices;
+  if (known && asked[device]) return 0;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e != cudaSuccess) return (int)e;
+  if (known) asked[device] = true;
+  return 0;
+}
+
 // ---- element conversion ----------------------------------------------------------------------
 template <typename T> __device__ __forceinline__ float to_f32(T v);
 template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }

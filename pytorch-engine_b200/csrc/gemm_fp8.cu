@@ -468,12 +468,9 @@ static int launch_np(Params p, const void* x, long long x_ld, long long x_rows, 
   if (e == 0 && !RAW) e = make_map(&xmap, x, p.K, x_rows, x_ld, NP, p.whole, S::kKbs);
   if (e != 0) return e;
   if (RAW) xmap = wmap;                // not used
-  static bool attr_set = false;
-  if (!attr_set) {
-    cudaError_t ce = cudaFuncSetAttribute(gemm_fp8_kernel<NP, GLU, RAW>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem);
-    if (ce != cudaSuccess) return (int)ce;
-    attr_set = true;
-  }
+  static bool asked[kDevices] = {};
+  e = allow_smem_once(gemm_fp8_kernel<NP, GLU, RAW>, S::kSmem, asked);
+  if (e != 0) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)c.blocks);
   cfg.blockDim = dim3(S::kThreads);

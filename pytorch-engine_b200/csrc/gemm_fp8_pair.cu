@@ -403,12 +403,9 @@ gemm_fp8_pair_kernel(Params p, const __grid_constant__ CUtensorMap amap, const _
 
 template <int MODE, bool GROUPS>
 static int launch_mode(const Params& p, const CUtensorMap& amap, const CUtensorMap& bmap, cudaStream_t stream) {
-  static bool attr_set = false;
-  if (!attr_set) {
-    const cudaError_t ce = cudaFuncSetAttribute(gemm_fp8_pair_kernel<MODE, GROUPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
-    if (ce != cudaSuccess) return (int)ce;
-    attr_set = true;
-  }
+  static bool asked[kDevices] = {};
+  const int e = allow_smem_once(gemm_fp8_pair_kernel<MODE, GROUPS>, kSmem, asked);
+  if (e != 0) return e;
   // with groups: as many tiles of rows as there can be
   const long long most = GROUPS ? p.M / (2 * BM) + (p.n_groups < p.M ? p.n_groups : p.M) : p.m_tiles, tiles = most * p.n_tiles;
   const int pairs = (int)(tiles < pe::kSMs / 2 ? tiles : pe::kSMs / 2);

@@ -328,12 +328,9 @@ extern "C" int pe_gemm_umma_glu(const void* x, long long ldx, const void* w, voi
   if (e == 0) e = pe::tma::make_map_2d_bf16(&bmap, w, K, w_rows, K, BK, BN / 2);
   if (e != 0) return e < 0 ? e : PE_ERR_BAD_ARGUMENT;
   const size_t smem = 1024 + (size_t)STAGES * kStage;
-  static bool attr_set = false;
-  if (!attr_set) {
-    cudaError_t ce = cudaFuncSetAttribute(gemm_umma_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (ce != cudaSuccess) return (int)ce;
-    attr_set = true;
-  }
+  static bool asked[pe::kDevices] = {};
+  e = pe::allow_smem_once(gemm_umma_kernel, smem, asked);
+  if (e != 0) return e;
   const int tiles = p.m_tiles * p.n_tiles;
   const int grid = tiles < n_sms ? tiles : n_sms;
   pe::launch(gemm_umma_kernel, grid, kThreads, smem, stream, p, amap, bmap);

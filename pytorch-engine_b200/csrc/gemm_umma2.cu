@@ -723,14 +723,10 @@ static int pe::umma2::launch_pair(Params p, const void* x, long long ldx, const 
   if (e == 0) e = make_map_kblocks(&bmap, w, K, w_rows, K, BNH, KBS);
   if (e != 0) return e < 0 ? e : PE_ERR_BAD_ARGUMENT;
   const size_t plain_smem = 1024 + (size_t)STAGES * kStage, rope_smem = plain_smem + 8 * kRopeWarp;
-  static bool attr_set = false;
-  if (!attr_set) {
-    cudaError_t ce = cudaFuncSetAttribute(gemm_umma2_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)plain_smem);
-    if (ce == cudaSuccess)
-      ce = cudaFuncSetAttribute(gemm_umma2_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)rope_smem);
-    if (ce != cudaSuccess) return (int)ce;
-    attr_set = true;
-  }
+  static bool asked[2][pe::kDevices] = {};
+  e = pe::allow_smem_once(gemm_umma2_kernel<false>, plain_smem, asked[0]);
+  if (e == 0) e = pe::allow_smem_once(gemm_umma2_kernel<true>, rope_smem, asked[1]);
+  if (e != 0) return e;
   const int tiles = p.m_tiles * p.n_tiles;
   const int pairs = tiles < n_sms / 2 ? tiles : n_sms / 2;
   cudaLaunchConfig_t cfg = {};

@@ -21,3 +21,11 @@ def test_arrays_read_sixteen_bytes_at_a_time_are_aligned(path):
             declared = [l for l in lines[max(0, i - 12):i] if re.search(rf"\b(?:T|__nv_bfloat16|uint8_t|float|uint32_t) {name}\[", l)]
             if declared:
                 assert "alignas(16)" in declared[-1], f"{os.path.basename(path)}:{i + 1}: {declared[-1].strip()}"
+
+
+@pytest.mark.parametrize("path", SOURCES, ids=os.path.basename)
+def test_shared_memory_is_asked_for_on_every_device(path):
+    """The attribute is a device's own: who remembers that a kernel has it remembers on which device."""
+    text = open(path).read()
+    for once in re.findall(r"static bool (\w+(?:\[[^\]]*\])*) = ", text):
+        assert "kDevices]" in once, f"{os.path.basename(path)}: static bool {once}"

@@ -254,6 +254,8 @@ class Runtime:
             if out is None:
                 out = torch.empty(x.shape[0], weight.shape[0], dtype=out_dtype or torch.bfloat16, device=x.device)
             return self._float8_product(x, weight, out)
+        if type(x) is Float8Rows:
+            raise KernelError("linear: rows in 8 bits go into products with 8-bit weights only")
         if self.gemm_backend is not None:
             y = self.gemm_backend(x, weight, out, out_dtype)
             if y is not None:

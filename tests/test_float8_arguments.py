@@ -55,3 +55,12 @@ def test_a_status_word_or_bias_elsewhere(pe):
         with pytest.raises(KernelError):
             call()
     assert ops.launch_count() == before
+
+
+@pytest.mark.gpu
+def test_8_bit_rows_and_a_16_bit_weight(pe):
+    from pytorch_engine_b200.parts.runtime import Runtime
+
+    rows = pe.parts.float8.Float8Rows.quantize(torch.ones(3, 128, dtype=BF16, device=DEV))
+    with pytest.raises(pe.kernels.KernelError, match="8-bit weights"):
+        Runtime(DEV, BF16).linear(rows, torch.ones(64, 128, dtype=BF16, device=DEV))

@@ -87,8 +87,9 @@ class Engine:
         buffers of a step, beside the cache, grow with its tokens (about 100 KB per token at the 8B shape).
         ``weight_format``: None (as stored) or "float8": the projections of attention, gated feed-forwards and routed experts are
         quantised to e4m3 with a scale for each 128 x 128 elements when the model is built, and their inputs, in blocks of 128
-        features, in every step (bfloat16 runs only).  A checkpoint whose matrices are stored so (``name_scale_inv`` beside
-        ``name``) keeps them without it."""
+        features, in every step (bfloat16 runs only); other parts keep their types.  A checkpoint whose matrices are stored so
+        (``name_scale_inv`` beside ``name``) keeps them without it, where a part has 8-bit products and each of the matrices that it
+        stacks but the last ends with a block of rows.  ``memory_report()["float8_mib"]`` says what that came to."""
         t0 = time.perf_counter()
         if not torch.cuda.is_available():
             raise KernelError("no CUDA device is visible: this engine runs on a B200 (sm_100a) only and has no CPU path")
@@ -136,7 +137,7 @@ class Engine:
         if verbose:
             rep = self.memory_report()
             print(f"[pytorch-engine_b200] {config.architecture} | dtype={self.dtype} | ctx={self.max_context_len} | "
-                  f"weights={rep['weights_mib']} MiB | cache={rep['cache_mib']} MiB | load {self.load_time_s:.1f} s")
+                  f"weights={rep['weights_mib']} MiB ({rep['float8_mib']} in 8 bits) | cache={rep['cache_mib']} MiB | load {self.load_time_s:.1f} s")
 
     # ---- constructors ------------------------------------------------------------------------
     @classmethod
@@ -218,10 +219,12 @@ class Engine:
 
     # ---- reports -----------------------------------------------------------------------------
     def memory_report(self) -> Dict[str, float]:
-        """Bytes held, in MiB (the reference's ``vram_report``, pygguf_engine/engine.py:471-508)."""
+        """Bytes held, in MiB (the reference's ``vram_report``, pygguf_engine/engine.py:471-508); ``float8_mib``: the part of the
+        weights that is kept in 8 bits (what ``weight_format`` or a checkpoint came to)."""
         mib = 1024.0 ** 2
         return {
             "weights_mib": round(self.model.weight_bytes() / mib, 2),
+            "float8_mib": round(self.model.weight_bytes(float8_only=True) / mib, 2),
             "cache_mib": round(self.cache.nbytes() / mib, 2),
             "workspace_mib": round(self.runner.workspace_bytes() / mib, 2),
             "allocated_mib": round(torch.cuda.memory_allocated(self.device) / mib, 2),

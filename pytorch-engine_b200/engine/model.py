@@ -137,13 +137,16 @@ class DecoderModel:
         self.final_norm.add_forward(stream, pending, normed, rows=ctx.want_rows)
         return self.head.forward(normed)
 
-    def weight_bytes(self) -> int:
+    def weight_bytes(self, float8_only: bool = False) -> int:
+        """Bytes of the weights that the parts hold; ``float8_only``: of those that are kept in 8 bits, with their scales."""
         seen = set()
         total = 0
 
         def visit(obj):
             nonlocal total
             for v in vars(obj).values():
+                if float8_only and type(v) is not Float8Weight:
+                    continue
                 for t in (v.values, v.scales) if type(v) is Float8Weight else (v,):
                     if isinstance(t, torch.Tensor) and t.data_ptr() not in seen:
                         seen.add(t.data_ptr())

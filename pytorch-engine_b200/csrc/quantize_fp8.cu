@@ -313,12 +313,9 @@ extern "C" int pe_rmsnorm_residual_fp8(float* residual, const void* delta, const
   // threads as for rmsnorm.cu's kernel, whose sums these are
   int threads = dim >= 2048 ? 512 : (dim >= 512 ? 256 : 128);
   if (n_rows <= 64 && dim > 2048) threads = 1024;
-  cudaError_t e;
-  if (smem > 47 * 1024) {              // with the static part beyond the 48 KB that need no asking
-    e = cudaFuncSetAttribute(rmsnorm_residual_fp8_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return (int)e;
-  }
-  e = pe::launch(rmsnorm_residual_fp8_kernel, dim3(n_rows), dim3(threads), smem, stream, residual, (const __nv_bfloat16*)delta, weight, (uint8_t*)values, v_ld, scales, s_ld, dim, eps);
+  const int ae = pe::allow_smem(rmsnorm_residual_fp8_kernel, smem);
+  if (ae != 0) return ae;
+  const cudaError_t e = pe::launch(rmsnorm_residual_fp8_kernel, dim3(n_rows), dim3(threads), smem, stream, residual, (const __nv_bfloat16*)delta, weight, (uint8_t*)values, v_ld, scales, s_ld, dim, eps);
   if (e != cudaSuccess) return (int)e;
   PE_LAUNCH_CHECK();
   return PE_OK;

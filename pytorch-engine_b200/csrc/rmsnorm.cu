@@ -377,15 +377,6 @@ __global__ void __launch_bounds__(1024) rmsnorm_of_sum_vec4_kernel(float* __rest
   }
 }
 
-template <typename K>
-static int set_smem(K kernel, size_t bytes) {
-  if (bytes > 47 * 1024) {             // with the kernels' static part beyond the 48 KB that need no asking
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-    if (e != cudaSuccess) return (int)e;
-  }
-  return 0;
-}
-
 }  // namespace pe
 
 extern "C" int pe_rmsnorm_residual(int dtype, float* residual, const void* delta, const float* weight, void* out,
@@ -404,11 +395,11 @@ extern "C" int pe_rmsnorm_residual(int dtype, float* residual, const void* delta
   if (vec && n_rows <= 64 && dim > 2048) threads = 1024;
   if (dtype == PE_F32) {
     auto k = vec ? pe::rmsnorm_vec4_kernel<float, float> : pe::rmsnorm_kernel<float, float>;
-    if ((e = pe::set_smem(k, smem))) return e;
+    if ((e = pe::allow_smem(k, smem))) return e;
     pe::launch(k, n_rows, threads, smem, stream, residual, (const float*)delta, weight, (float*)out, rows, n_rows, dim, eps);
   } else if (dtype == PE_BF16) {
     auto k = vec ? pe::rmsnorm_vec4_kernel<__nv_bfloat16, __nv_bfloat16> : pe::rmsnorm_kernel<__nv_bfloat16, __nv_bfloat16>;
-    if ((e = pe::set_smem(k, smem))) return e;
+    if ((e = pe::allow_smem(k, smem))) return e;
     pe::launch(k, n_rows, threads, smem, stream, residual, (const __nv_bfloat16*)delta, weight, (__nv_bfloat16*)out, rows, n_rows, dim, eps);
   } else {
     return PE_ERR_UNSUPPORTED_DTYPE;
@@ -451,11 +442,11 @@ extern "C" int pe_rmsnorm_rows(int dtype, const void* x, long long x_ld, const f
   int e;
   if (dtype == PE_F32) {
     auto k = pe::rmsnorm_plain_kernel<float>;
-    if ((e = pe::set_smem(k, smem))) return e;
+    if ((e = pe::allow_smem(k, smem))) return e;
     pe::launch(k, n_rows, threads, smem, stream, (const float*)x, x_ld, weight, (float*)out, n_rows, dim, eps);
   } else {
     auto k = pe::rmsnorm_plain_kernel<__nv_bfloat16>;
-    if ((e = pe::set_smem(k, smem))) return e;
+    if ((e = pe::allow_smem(k, smem))) return e;
     pe::launch(k, n_rows, threads, smem, stream, (const __nv_bfloat16*)x, x_ld, weight, (__nv_bfloat16*)out, n_rows, dim, eps);
   }
   PE_LAUNCH_CHECK();
@@ -480,11 +471,11 @@ extern "C" int pe_rmsnorm_add(int dtype, float* stream, const void* delta, const
   int e;
   if (dtype == PE_F32) {
     auto k = vec ? pe::rmsnorm_add_vec4_kernel<float> : pe::rmsnorm_add_kernel<float>;
-    if ((e = pe::set_smem(k, smem))) return e;
+    if ((e = pe::allow_smem(k, smem))) return e;
     pe::launch(k, n_rows, threads, smem, stream_, stream, (const float*)delta, weight, (float*)cast, n_rows, dim, eps);
   } else if (dtype == PE_BF16) {
     auto k = vec ? pe::rmsnorm_add_vec4_kernel<__nv_bfloat16> : pe::rmsnorm_add_kernel<__nv_bfloat16>;
-    if ((e = pe::set_smem(k, smem))) return e;
+    if ((e = pe::allow_smem(k, smem))) return e;
     pe::launch(k, n_rows, threads, smem, stream_, stream, (const __nv_bfloat16*)delta, weight, (__nv_bfloat16*)cast, n_rows, dim, eps);
   } else {
     return PE_ERR_UNSUPPORTED_DTYPE;
@@ -513,11 +504,11 @@ extern "C" int pe_rmsnorm_residual_sum(int dtype, float* residual, const void* c
   int e;
   if (dtype == PE_F32) {
     auto k = vec ? pe::rmsnorm_sum_vec4_kernel<float, float> : pe::rmsnorm_sum_kernel<float, float>;
-    if ((e = pe::set_smem(k, smem))) return e;
+    if ((e = pe::allow_smem(k, smem))) return e;
     pe::launch(k, n_rows, threads, smem, stream, residual, list, weight, (float*)out, rows, n_rows, dim, eps);
   } else if (dtype == PE_BF16) {
     auto k = vec ? pe::rmsnorm_sum_vec4_kernel<__nv_bfloat16, __nv_bfloat16> : pe::rmsnorm_sum_kernel<__nv_bfloat16, __nv_bfloat16>;
-    if ((e = pe::set_smem(k, smem))) return e;
+    if ((e = pe::allow_smem(k, smem))) return e;
     pe::launch(k, n_rows, threads, smem, stream, residual, list, weight, (__nv_bfloat16*)out, rows, n_rows, dim, eps);
   } else {
     return PE_ERR_UNSUPPORTED_DTYPE;
@@ -555,12 +546,12 @@ extern "C" int pe_rmsnorm_of_sum(int dtype, float* stream, const void* delta, fl
 #undef PE_OF_SUM
   } else if (dtype == PE_F32) {
     int e;
-    if ((e = pe::set_smem(pe::rmsnorm_of_sum_kernel<float>, smem))) return e;
+    if ((e = pe::allow_smem(pe::rmsnorm_of_sum_kernel<float>, smem))) return e;
     pe::launch(pe::rmsnorm_of_sum_kernel<float>, n_rows, threads, smem, stream_, stream, (const float*)delta, alpha, scale, weight,
                (float*)cast, n_rows, dim, eps);
   } else {
     int e;
-    if ((e = pe::set_smem(pe::rmsnorm_of_sum_kernel<__nv_bfloat16>, smem))) return e;
+    if ((e = pe::allow_smem(pe::rmsnorm_of_sum_kernel<__nv_bfloat16>, smem))) return e;
     pe::launch(pe::rmsnorm_of_sum_kernel<__nv_bfloat16>, n_rows, threads, smem, stream_, stream, (const __nv_bfloat16*)delta, alpha,
                scale, weight, (__nv_bfloat16*)cast, n_rows, dim, eps);
   }
